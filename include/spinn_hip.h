@@ -254,6 +254,178 @@ enum { SPINN_BINARY_MOD = 4 };
 int spinn_hip_binary_typed(int op, int dtype, const void *a, int64_t na, const void *b, int64_t nb, void *y,
                            int64_t n, void *stream);
 
+/* ---- a decoding step: linear layers, paged key-value cache, beam search ----
+ *
+ * No counterparts in the reference, whose graphs are fp32 and run once per input. dtype is
+ * ENNF_TYPE_FLOAT32 (1), FLOAT16 (10) or BFLOAT16 (16); sums, softmax statistics and
+ * accumulated weights are fp32, results are rounded once to dtype. Strides count elements
+ * of dtype unless stated otherwise. Tensors start at multiples of their element's size;
+ * workspaces at multiples of 16 bytes, as spinn_hip_malloc returns them. A workspace
+ * needs no clearing and holds nothing between calls; calls that may run at the same
+ * time need one each. All entry points can be captured into a graph. */
+
+/* Activations of spinn_hip_linear; the first values are those of SPINN_ACT_*. */
+enum {
+    SPINN_LINEAR_NONE = 0,
+    SPINN_LINEAR_RELU = 1,
+    SPINN_LINEAR_SILU = 3,     /* v / (1 + exp(-v)) */
+    SPINN_LINEAR_GELU = 6,     /* v/2 (1 + erf(v / sqrt 2)) */
+    SPINN_LINEAR_GELU_TANH = 7 /* v/2 (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+};
+
+/*
+ * y[i,j] = act( sum_k x[i,k] * w(j,k) + bias[j] + residual[i,j] ), bias and residual optional
+ * (the residual comes before the activation, as in spinn_hip_conv).
+ * w(j,k) is w[j*k_dim + k] when trans_w (a fully connected layer's [N,K]), else w[k*n + j]
+ * (a MatMul's [K,N]); it is laid out once by spinn_hip_linear_pack_weights and read from
+ * `packed_w` alone afterwards. Rows of x, residual and y are ldx, ldres and ldy apart
+ * (0 = dense: k, n, n). y may be the residual itself (same address and stride); otherwise
+ * y overlaps no input.
+ * x starts at a multiple of 16 bytes unless x_unaligned is set, which asks for workspace;
+ * row strides and sizes are free. m = 0 is an empty batch.
+ */
+typedef struct {
+    int32_t m, n, k;
+    int32_t dtype;       /* of x, w, bias, residual and y */
+    int32_t trans_w;
+    int32_t act;         /* SPINN_LINEAR_* */
+    int32_t x_unaligned;
+    int32_t reserved;    /* 0 */
+    int64_t ldx, ldres, ldy;
+} SpinnHipLinearDesc;
+
+/* Bytes of the packed weights: depends on n, k and dtype alone. 0 = descriptor refused. */
+size_t spinn_hip_linear_packed_size(const SpinnHipLinearDesc *d);
+/* packed_w starts at a multiple of 16 bytes. */
+int spinn_hip_linear_pack_weights(const SpinnHipLinearDesc *d, const void *w, void *packed_w, void *stream);
+size_t spinn_hip_linear_workspace_size(const SpinnHipLinearDesc *d);
+int spinn_hip_linear(const SpinnHipLinearDesc *d, const void *x, const void *packed_w, const void *bias,
+                     const void *residual, void *y, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A paged key-value cache. Keys and values are in two arrays of n_pages pages; a page
+ * holds page_size slots of kv_heads rows of head_dim contiguous elements:
+ *   row(page, head, slot) = base + page*page_stride + head*head_stride + slot*slot_stride,
+ * the same for both. Sequence s keeps slot i in page page_table[s*max_pages + i/page_size],
+ * at i % page_size. A page number outside [0, n_pages) holds nothing: its slots are not
+ * read (as if masked) and not written. Rows overlap nowhere, except that sequences
+ * may share pages that no call writes.
+ */
+typedef struct {
+    int32_t dtype;
+    int32_t seqs;
+    int32_t kv_heads;
+    int32_t head_dim;    /* 1..SPINN_HIP_KV_MAX_DIM */
+    int32_t page_size;
+    int32_t n_pages;
+    int32_t max_pages;   /* page numbers per sequence; max_pages * page_size < 2^31 */
+    int32_t reserved;    /* 0 */
+    int64_t page_stride, head_stride, slot_stride;
+} SpinnHipKvDesc;
+#define SPINN_HIP_KV_MAX_DIM 256
+
+/* Write new tokens' rows: token t's k[t*k_stride + head*head_dim + i] (v alike) goes to
+ * slot[t] of sequence seq[t] (seq = NULL: of sequence t, tokens <= seqs). Where given, `acc`
+ * and `pos` [seqs, kv_heads, acc_stride] take 0 and position[t] (NULL: slot[t]) at that
+ * slot in every head (slots from acc_stride on have none). A token whose sequence or slot
+ * is outside the cache, or whose page holds nothing, is skipped entirely. Two tokens of
+ * one call must not name the same slot. */
+int spinn_hip_kv_append(const SpinnHipKvDesc *d, int64_t tokens, const int32_t *seq, const int32_t *slot,
+                        const int32_t *position, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                        const int32_t *page_table, void *k_pages, void *v_pages, float *acc, int32_t *pos,
+                        int64_t acc_stride, void *stream);
+
+/*
+ * Attention of one new token per sequence over the cache:
+ *   o[s,h] = sum_i p_i v_i, p = softmax over the visible slots i < lengths[s] of scale * q[s,h].k_i,
+ * query head h reading kv head h / (heads / kv_heads). lengths are on the device, cut to
+ * [0, max_len]; mask [seqs, mask_stride] (uint8, NULL = all) hides slots where it is 0, whatever
+ * their rows hold. A row with nothing visible gives o = 0 and lse = -inf. Visible keys and
+ * values are finite.
+ * q and o: heads * head_dim contiguous per sequence, q_stride and o_stride apart. lse [seqs, heads]
+ * (NULL = not wanted): log of the softmax's denominator.
+ * accumulate: acc_out[s,g,i] = acc[s,g,i] + sum of p_i over the query heads of kv head g, for
+ * i < lengths[s]; acc_out, [seqs, kv_heads, acc_stride] as acc, may be acc itself; slots from
+ * lengths[s] on stay as they are.
+ */
+typedef struct {
+    SpinnHipKvDesc kv;
+    int32_t heads;       /* multiple of kv_heads */
+    int32_t max_len;     /* <= max_pages * page_size; the split and the workspace go by it */
+    float scale;
+    int32_t accumulate;
+    int64_t q_stride, o_stride, mask_stride, acc_stride;
+} SpinnHipKvAttentionDesc;
+
+size_t spinn_hip_kv_attention_workspace_size(const SpinnHipKvAttentionDesc *d);
+int spinn_hip_kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k_pages, const void *v_pages,
+                           const int32_t *page_table, const int32_t *lengths, const uint8_t *mask, const float *acc,
+                           float *acc_out, void *o, float *lse, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
+/*
+ * Cut every sequence to `budget` slots, for each kv head by itself. Of the n = lengths[s]
+ * (cut to [0, max_len]) slots, if n > budget, the budget highest stay: first those whose
+ * token is safe (pos < sinks, or pos >= next_pos[s] - recent), then by accumulated weight
+ * acc (NaN lowest), equal ones by the lower slot. Slots that stay keep their place where it
+ * is below the budget; the others move, in slot order, into the places below it that fell
+ * free. K and V rows move within the pages. acc_out and pos_out [seqs, kv_heads, acc_stride]
+ * take the staying slots' values at their new places (each may be its input itself);
+ * lengths_out[s] = min(n, budget) (may be lengths itself). What lies behind it stays
+ * as it was. Sequences share no page that is moved within. next_pos[s] is the position
+ * that the sequence's next token gets.
+ */
+typedef struct {
+    SpinnHipKvDesc kv;
+    int32_t budget;      /* >= 0 */
+    int32_t recent, sinks;
+    int32_t max_len;     /* <= max_pages * page_size, <= acc_stride */
+    int64_t acc_stride;
+} SpinnHipKvEvictDesc;
+
+size_t spinn_hip_kv_evict_workspace_size(const SpinnHipKvEvictDesc *d);
+int spinn_hip_kv_evict(const SpinnHipKvEvictDesc *d, const int32_t *page_table, const int32_t *lengths,
+                       const int32_t *next_pos, const float *acc, const int32_t *pos, float *acc_out,
+                       int32_t *pos_out, int32_t *lengths_out, void *k_pages, void *v_pages, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/*
+ * The k best continuations of each batch item over its beams and the vocabulary:
+ *   key(b, t) = scores[b] + logits[b,t] - log sum_u exp(logits[b,u])
+ * in descending order, equal keys by the lower beam, then the lower token. logits [batch * beams
+ * rows of vocab, logits_stride apart]; scores fp32 [batch, beams], -inf = an empty beam.
+ * A beam with finished[b] != 0 (uint8 [batch, beams], NULL = none) has one continuation, end_token
+ * at its score; its other keys are -inf. NaN logits and scores count as -inf, +inf as the
+ * largest finite fp32. Keys are compared in 64 bits (within a beam, the logits are).
+ * out_scores fp32, out_parents and out_tokens int32 [batch, k].
+ */
+typedef struct {
+    int32_t dtype;
+    int32_t batch, beams, vocab; /* beams <= SPINN_HIP_BEAM_MAX */
+    int32_t k;                   /* 1..min(SPINN_HIP_BEAM_MAX_K, beams * vocab) */
+    int32_t end_token;           /* read where finished is given */
+    int64_t logits_stride;
+} SpinnHipBeamDesc;
+#define SPINN_HIP_BEAM_MAX 64
+#define SPINN_HIP_BEAM_MAX_K 128
+
+size_t spinn_hip_beam_select_workspace_size(const SpinnHipBeamDesc *d);
+int spinn_hip_beam_select(const SpinnHipBeamDesc *d, const void *logits, const float *scores, const uint8_t *finished,
+                          float *out_scores, int32_t *out_parents, int32_t *out_tokens, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Rows of beam states after their parents: for every state, batch item b and j < k, row b*k + j of
+ * dst = row b*beams + parents[b*k + j] of src (the first row_bytes of it). A parent outside
+ * [0, beams) leaves its row of dst as it was. Strides are bytes; dst overlaps no src. Up to
+ * SPINN_HIP_MAX_BLOCKS states in one launch. */
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t row_bytes, src_stride, dst_stride;
+} SpinnHipBeamState;
+int spinn_hip_beam_reorder(const SpinnHipBeamState *states, int n_states, int32_t batch, int32_t beams, int32_t k,
+                           const int32_t *parents, void *stream);
+
 /* ---- device, memory, stream, event and graph plumbing for the host runtime ---- */
 
 int spinn_hip_init(int device);

@@ -1,0 +1,557 @@
+// kv_attention.hip - a paged key-value cache: rows appended to it, and the attention of one new
+// token per sequence over it.
+//
+// Per query head: s_i = scale q.k_i, p_i = exp(s_i - m) / sum_j exp(s_j - m), o = sum_i p_i v_i,
+// in one pass with the running maximum m and sum: a tile of slots raises m to m', and what
+// was summed so far is scaled by exp(m - m'). Every row of the cache is read once, for all the
+// query heads of its kv head, so the bound is memory: 2 rows a slot against 4 * heads * head_dim flops.
+//
+// The matrix cores then have time to spare (one new token fills few of a tile's 16 columns, and
+// at 5 TB/s they are still under 5 % busy), which decides the layout: nothing goes through LDS in the
+// loop. S^T = K Q^T has slots as rows, and lane (g = l/16, n = l%16) ends up with
+// head n, slots 4g..4g+3 of each half tile: exactly the elements that the second product wants
+// from it as its operand (contraction over slots may run in any order, so V's rows
+// are fetched in that order). O^T = V^T P^T: a lane fetches the same 16-byte columns of
+// eight slots, a full row per 16 lanes, and transposes them in registers (one
+// v_perm per two elements).
+#include "decode.h"
+
+namespace spinn {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kTile = 32;     // slots per step of a wave: two halves of 16 rows
+constexpr int kHeadTile = 16; // query heads of one kv head per workgroup
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+struct AttendArgs {
+    const void *q, *k, *v;
+    const int32_t *table, *lengths;
+    const uint8_t *mask;
+    void *o;
+    float *lse;
+    float *part_o, *part_ml; // [seqs][heads][splits][dim], [..][2] (maximum and sum, base 2)
+    float *scores;           // [seqs][heads][score_row], base 2; null when no weights are wanted
+    int64_t q_stride, o_stride, mask_stride, page_stride, head_stride, slot_stride, score_row;
+    float scale2; // scale * log2 e
+    int32_t seqs, heads, kv_heads, group, dim, page_size, page_shift, n_pages, max_pages, max_len;
+    int32_t splits, chunk; // chunk: slots per split, a multiple of kTile * kWaves
+    int32_t head_tiles;
+};
+
+__device__ __forceinline__ int page_of(const AttendArgs &a, int slot) {
+    return a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page_size;
+}
+
+// 16 bytes at p, element by element: those from `left` on (elements to the row's end) are zero.
+template <class T>
+__device__ __forceinline__ u32x4 load_edge(const T *p, int left) {
+    typedef typename Bits<T>::type B;
+    constexpr int N = 16 / sizeof(T);
+    u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < left) {
+            const uint32_t b = (uint32_t) reinterpret_cast<const B *>(p)[i];
+            if constexpr (N == 4) r[i] = b;
+            else r[i / 2] |= b << (16 * (i % 2));
+        }
+    return r;
+}
+
+// T: element; DP: head_dim padded to 64, 128 or 256; VEC: rows are whole 16-byte runs;
+// UNI: pages are multiples of 16 slots, so that each half tile lies in one page.
+template <class T, int DP, bool VEC, bool UNI>
+__global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
+    constexpr int E = 16 / (int)sizeof(T);    // elements per 16 bytes
+    constexpr int KC = DP / kFrag<T>;         // fragments of a row of K or Q
+    constexpr int DPL = DP / 16;              // a lane's elements of a V row: DPL n .. +DPL-1
+    constexpr int VB = DPL * (int)sizeof(T);  // their bytes
+    constexpr int VW = VB / 4;                // and words
+    constexpr float kPScale = sizeof(T) == 2 && !__is_same(T, __bf16) ? 16384.f : 1.f;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+
+    int b = blockIdx.x;
+    const int ht = b % a.head_tiles;
+    b /= a.head_tiles;
+    const int sp = b % a.splits;
+    b /= a.splits;
+    const int kvh = b % a.kv_heads, seq = b / a.kv_heads;
+    const int h0 = kvh * a.group + ht * kHeadTile;              // first query head of the tile
+    const int nh = min(kHeadTile, a.group - ht * kHeadTile);    // query heads in it
+    const int len = min(max(a.lengths[seq], 0), a.max_len);
+    const int begin = sp * a.chunk, end = min(len, begin + a.chunk);
+    const int32_t *table = a.table + (int64_t)seq * a.max_pages;
+    const uint8_t *mask = a.mask ? a.mask + (int64_t)seq * a.mask_stride : nullptr;
+
+    // Q: lane (g, n) holds head n, the same k as the K fragments
+    u32x4 q[KC];
+    {
+        const T *qp = (const T *)a.q + (int64_t)seq * a.q_stride + (int64_t)(h0 + min(n, nh - 1)) * a.dim;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int d0 = c * kFrag<T> + g * E;
+            q[c] = load_edge<T>(qp + d0, n < nh ? a.dim - d0 : 0);
+        }
+    }
+
+    f32x4 acc[DPL] = {};
+    float m = -INFINITY, l = 0.f;
+    const T *kb = (const T *)a.k + (int64_t)kvh * a.head_stride;
+    const T *vb = (const T *)a.v + (int64_t)kvh * a.head_stride;
+
+    for (int t0 = begin + wave * kTile; t0 < end; t0 += kTile * kWaves) {
+        u32x4 kr[2][KC];
+        uint32_t vr[8][VW];
+        uint32_t seen = 0; // bit j: the lane's j-th slot (4g+j, then 16+4g+j-4) is visible
+        const T *vrow[8];
+        // rows: addresses first, so that all of a tile's loads are in flight together
+        if constexpr (UNI) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int s0 = min(t0 + 16 * h, (len - 1) & ~15);
+                const int pi = page_of(a, s0);
+                int page = table[pi];
+                const bool ok = (unsigned)page < (unsigned)a.n_pages;
+                page = ok ? page : 0;
+                const int64_t at = (int64_t)page * a.page_stride + (int64_t)(s0 - pi * a.page_size) * a.slot_stride;
+                const T *kp = kb + at + (int64_t)n * a.slot_stride + g * E;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const bool in = c * kFrag<T> + g * E < a.dim;
+                    kr[h][c] = in ? *reinterpret_cast<const u32x4 *>(kp + c * kFrag<T>) : (u32x4){0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    vrow[4 * h + j] = vb + at + (int64_t)(4 * g + j) * a.slot_stride;
+                    if (ok && t0 + 16 * h + 4 * g + j < end) seen |= 1u << (4 * h + j);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int slot = min(t0 + 16 * h + n, len - 1);
+                const int pi = page_of(a, slot);
+                int page = table[pi];
+                page = (unsigned)page < (unsigned)a.n_pages ? page : 0;
+                const T *kp = kb + (int64_t)page * a.page_stride + (int64_t)(slot - pi * a.page_size) * a.slot_stride + g * E;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const int left = a.dim - (c * kFrag<T> + g * E);
+                    if constexpr (VEC)
+                        kr[h][c] = left > 0 ? *reinterpret_cast<const u32x4 *>(kp + c * kFrag<T>) : (u32x4){0, 0, 0, 0};
+                    else
+                        kr[h][c] = load_edge<T>(kp + c * kFrag<T>, left);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int want = t0 + 16 * h + 4 * g + j;
+                    const int vs = min(want, len - 1);
+                    const int vi = page_of(a, vs);
+                    int vpage = table[vi];
+                    const bool ok = (unsigned)vpage < (unsigned)a.n_pages;
+                    vpage = ok ? vpage : 0;
+                    vrow[4 * h + j] = vb + (int64_t)vpage * a.page_stride + (int64_t)(vs - vi * a.page_size) * a.slot_stride;
+                    if (ok && want < end) seen |= 1u << (4 * h + j);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const T *vp = vrow[j] + n * DPL;
+            if constexpr (VEC) {
+                // in 16-byte runs (8 where a lane's share is 8); a row ends between runs
+                constexpr int R = VB >= 16 ? 16 : VB;
+#pragma unroll
+                for (int r = 0; r < VB / R; ++r) {
+                    const bool in = n * DPL + r * (R / (int)sizeof(T)) < a.dim;
+                    if constexpr (R == 16) {
+                        const u32x4 w = in ? *reinterpret_cast<const u32x4 *>(vp + r * E) : (u32x4){0, 0, 0, 0};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) vr[j][4 * r + i] = w[i];
+                    } else {
+                        const u32x2 w = in ? *reinterpret_cast<const u32x2 *>(vp) : (u32x2){0, 0};
+                        vr[j][0] = w[0];
+                        vr[j][1] = w[1];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < (VB + 15) / 16; ++r) {
+                    const u32x4 w = load_edge<T>(vp + r * E, min(a.dim - n * DPL - r * E, DPL - r * E));
+#pragma unroll
+                    for (int i = 0; i < (VW < 4 ? VW : 4); ++i) vr[j][4 * r + i] = w[i];
+                }
+            }
+        }
+        if (mask) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int slot = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                if (seen >> j & 1u)
+                    if (mask[slot] == 0) seen &= ~(1u << j);
+            }
+        }
+
+        // scores, base 2
+        float s[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < KC; ++i) mfma_frag(c, kr[h][i], q[i], T());
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * h + i] = (seen >> (4 * h + i) & 1u) ? c[i] * a.scale2 : -INFINITY;
+        }
+        if (a.scores && n < nh) {
+            float *row = a.scores + ((int64_t)seq * a.heads + h0 + n) * a.score_row + t0 + 4 * g;
+            *reinterpret_cast<f32x4 *>(row) = (f32x4){s[0], s[1], s[2], s[3]};
+            *reinterpret_cast<f32x4 *>(row + 16) = (f32x4){s[4], s[5], s[6], s[7]};
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top, m);
+        const float base = top == -INFINITY ? 0.f : top;
+        if (__any(top > m)) {
+            const float alpha = exp2_hw(m - base);
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < DPL; ++c) acc[c] *= alpha;
+            m = top;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = exp2_hw(s[j] - base);
+            l += p[j];
+        }
+        // rows that are not visible may hold anything, and 0 * NaN is NaN
+        if (__any(seen != 0xffu)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(seen >> j & 1u))
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) vr[j][i] = 0u;
+        }
+
+        if constexpr (sizeof(T) == 2) {
+            // p as two 16-bit parts, the rounding and what it left: the product then carries p to
+            // 2^-16 and better, for one more pass of a unit that is idle. fp16 takes p times 2^14:
+            // its least number is 2^-24, which weights of a long sequence fall under.
+            u32x4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t wh = 0, wl = 0;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float v = p[2 * i + e] * kPScale;
+                    const T r = (T)v;
+                    const T rest = (T)(v - (float)r);
+                    wh |= (uint32_t) __builtin_bit_cast(uint16_t, r) << (16 * e);
+                    wl |= (uint32_t) __builtin_bit_cast(uint16_t, rest) << (16 * e);
+                }
+                hi[i] = wh;
+                lo[i] = wl;
+            }
+#pragma unroll
+            for (int c = 0; c < DPL; ++c) {
+                u32x4 f; // V^T: row c of the lane's columns, its eight slots
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c / 2], vr[2 * i][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+                mfma_frag(acc[c], f, hi, T());
+                mfma_frag(acc[c], f, lo, T());
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < DPL; ++c)
+                    acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[j][c]), p[j], acc[c], 0, 0, 0);
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // The waves' parts, joined in wave order: acc[c][r] of lane (g, n) is head n, element DPL (4g + r) + c.
+    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    extern __shared__ float so[]; // [kWaves][nh][DP + 1]
+    constexpr int kRow = DP + 1;
+    if (g == 0) {
+        sm[wave][n] = m;
+        sl[wave][n] = l;
+    }
+    __syncthreads();
+    float M = sm[0][n];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sm[w][n]);
+    const float mbase = M == -INFINITY ? 0.f : M;
+    const float mine = exp2_hw(m - mbase) * (1.f / kPScale);
+    if (n < nh) {
+        float *row = so + (wave * nh + n) * kRow;
+#pragma unroll
+        for (int c = 0; c < DPL; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) row[DPL * (4 * g + r) + c] = acc[c][r] * mine;
+    }
+    __syncthreads();
+    const bool whole = a.splits == 1;
+    for (int h = wave; h < nh; h += kWaves) {
+        float Mh = sm[0][h];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) Mh = fmaxf(Mh, sm[w][h]);
+        const float bh = Mh == -INFINITY ? 0.f : Mh;
+        float L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) L += sl[w][h] * exp2_hw(sm[w][h] - bh);
+        const int64_t sh = (int64_t)seq * a.heads + h0 + h;
+        const float inv = whole && L > 0.f ? 1.f / L : (whole && L == 0.f ? 0.f : (whole ? L : 1.f));
+        if (whole || Mh != -INFINITY)
+            for (int d = lane; d < a.dim; d += 64) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) v += so[(w * nh + h) * kRow + d];
+                if (whole) ((T *)a.o)[(int64_t)seq * a.o_stride + (int64_t)(h0 + h) * a.dim + d] = (T)(v * inv);
+                else a.part_o[(sh * a.splits + sp) * a.dim + d] = v;
+            }
+        if (lane == 0) {
+            if (whole && a.lse) a.lse[sh] = L == 0.f ? -INFINITY : (Mh + __log2f(L)) * kLn2;
+            if (a.part_ml) {
+                a.part_ml[(sh * a.splits + sp) * 2] = Mh;
+                a.part_ml[(sh * a.splits + sp) * 2 + 1] = L;
+            }
+        }
+    }
+}
+
+// Maximum and sum of one head over its splits, by the lanes of a wave; the same in every lane.
+__device__ __forceinline__ void join_ml(const float *ml, int splits, int lane, float &M, float &L) {
+    M = -INFINITY;
+    for (int i = lane; i < splits; i += 64) M = fmaxf(M, ml[2 * i]);
+#pragma unroll
+    for (int off = 32; off; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+    const float base = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+    for (int i = lane; i < splits; i += 64) L += ml[2 * i + 1] * exp2_hw(ml[2 * i] - base);
+#pragma unroll
+    for (int off = 32; off; off >>= 1) L += __shfl_xor(L, off);
+}
+
+// Blocks below join_blocks: one (sequence, head) each, the splits' sums joined in split order
+// by strands of threads and the strands in order. The others: 1024 slots of one (sequence, kv head),
+// the heads' weights added up.
+constexpr int kAccSlots = 1024;
+template <class T>
+__global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int join_blocks, const float *__restrict__ acc_in,
+                                                      float *acc_out, int64_t acc_stride, int acc_chunks) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x < join_blocks) {
+        const int sh = blockIdx.x, seq = sh / a.heads, h = sh - seq * a.heads;
+        const float *ml = a.part_ml + (int64_t)sh * a.splits * 2;
+        float M, L;
+        join_ml(ml, a.splits, lane, M, L);
+        const float base = M == -INFINITY ? 0.f : M;
+        // a strand of `cols` threads takes every strands-th split
+        const int cols = a.dim <= 64 ? 64 : (a.dim <= 128 ? 128 : 256);
+        const int strands = 256 / cols, strand = threadIdx.x / cols, d = threadIdx.x % cols;
+        float v = 0.f;
+        if (d < a.dim)
+            for (int i = strand; i < a.splits; i += strands) {
+                const float mi = ml[2 * i];
+                if (mi != -INFINITY) v += a.part_o[((int64_t)sh * a.splits + i) * a.dim + d] * exp2_hw(mi - base);
+            }
+        __shared__ float sum[256];
+        sum[threadIdx.x] = v;
+        __syncthreads();
+        if (strand == 0 && d < a.dim) {
+            for (int i = 1; i < strands; ++i) v += sum[i * cols + d];
+            ((T *)a.o)[(int64_t)seq * a.o_stride + (int64_t)h * a.dim + d] = (T)(L == 0.f ? 0.f : v / L);
+        }
+        if (threadIdx.x == 0 && a.lse) a.lse[sh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * kLn2;
+        return;
+    }
+    const int b = blockIdx.x - join_blocks;
+    const int chunk = b % acc_chunks, sg = b / acc_chunks, seq = sg / a.kv_heads, kvh = sg - seq * a.kv_heads;
+    const int len = min(max(a.lengths[seq], 0), a.max_len);
+    const int s0 = chunk * kAccSlots;
+    if (s0 >= len) return;
+    extern __shared__ float hml[]; // [group][2]: base and 1 / sum
+    const int64_t first = (int64_t)seq * a.heads + (int64_t)kvh * a.group;
+    for (int h = wave; h < a.group; h += 4) {
+        float M, L;
+        join_ml(a.part_ml + (first + h) * a.splits * 2, a.splits, lane, M, L);
+        if (lane == 0) {
+            hml[2 * h] = M == -INFINITY ? 0.f : M;
+            hml[2 * h + 1] = L == 0.f ? 0.f : 1.f / L;
+        }
+    }
+    __syncthreads();
+    const int64_t row = (int64_t)sg * acc_stride;
+    const int stop = min(len, s0 + kAccSlots);
+    for (int i = s0 + threadIdx.x; i < stop; i += 256) {
+        float v = 0.f;
+        for (int h = 0; h < a.group; ++h)
+            v += exp2_hw(a.scores[(first + h) * a.score_row + i] - hml[2 * h]) * hml[2 * h + 1];
+        acc_out[row + i] = acc_in[row + i] + v;
+    }
+}
+
+// One workgroup per (token, kv head)-strided run of rows: threads over a token's elements.
+template <class T>
+__global__ __launch_bounds__(256) void kv_append_kernel(SpinnHipKvDesc d, int64_t tokens, const int32_t *seq,
+                                                        const int32_t *slot, const int32_t *position, const T *k,
+                                                        int64_t k_stride, const T *v, int64_t v_stride,
+                                                        const int32_t *table, T *k_pages, T *v_pages, float *acc,
+                                                        int32_t *pos, int64_t acc_stride) {
+    typedef typename Bits<T>::type B;
+    const int row = d.kv_heads * d.head_dim;
+    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
+        const int s = seq ? seq[t] : (int)t;
+        const int at = slot[t];
+        if ((unsigned)s >= (unsigned)d.seqs || at < 0) continue;
+        const int pi = at / d.page_size;
+        if (pi >= d.max_pages) continue;
+        const int page = table[(int64_t)s * d.max_pages + pi];
+        if ((unsigned)page >= (unsigned)d.n_pages) continue;
+        const int64_t base = (int64_t)page * d.page_stride + (int64_t)(at - pi * d.page_size) * d.slot_stride;
+        for (int i = threadIdx.x; i < row; i += blockDim.x) {
+            const int h = i / d.head_dim;
+            const int64_t to = base + (int64_t)h * d.head_stride + (i - h * d.head_dim);
+            reinterpret_cast<B *>(k_pages)[to] = reinterpret_cast<const B *>(k)[t * k_stride + i];
+            reinterpret_cast<B *>(v_pages)[to] = reinterpret_cast<const B *>(v)[t * v_stride + i];
+        }
+        if (at < acc_stride)
+            for (int h = threadIdx.x; h < d.kv_heads; h += blockDim.x) {
+                const int64_t e = ((int64_t)s * d.kv_heads + h) * acc_stride + at;
+                if (acc) acc[e] = 0.f;
+                if (pos) pos[e] = position ? position[t] : at;
+            }
+    }
+}
+
+struct Plan {
+    int head_tiles, splits, chunk;
+    int64_t score_row;
+    size_t o_bytes, ml_bytes, score_bytes;
+};
+
+Plan plan(const SpinnHipKvAttentionDesc *d) {
+    Plan p;
+    const int group = d->heads / d->kv.kv_heads;
+    p.head_tiles = (group + kHeadTile - 1) / kHeadTile;
+    const int64_t units = (int64_t)d->kv.seqs * d->kv.kv_heads * p.head_tiles;
+    constexpr int step = kTile * kWaves;
+    const int64_t steps = std::max<int64_t>(1, (d->max_len + step - 1) / step);
+    // four workgroups per CU
+    const int64_t want = (4 * (int64_t)device_cu_count() + units - 1) / units;
+    const int64_t per = std::max<int64_t>(2, (steps + want - 1) / want); // steps per split
+    p.splits = (int)((steps + per - 1) / per);
+    p.chunk = (int)(per * step);
+    const int64_t rows = (int64_t)d->kv.seqs * d->heads;
+    p.score_row = ((int64_t)d->max_len + kTile - 1) / kTile * kTile;
+    p.o_bytes = p.splits > 1 ? round16((size_t)rows * p.splits * d->kv.head_dim * 4) : 0;
+    p.ml_bytes = p.splits > 1 || d->accumulate ? round16((size_t)rows * p.splits * 8) : 0;
+    p.score_bytes = d->accumulate ? (size_t)rows * p.score_row * 4 : 0;
+    return p;
+}
+
+template <class T, int DP>
+void launch_attend(const AttendArgs &a, bool vec, bool uni, dim3 grid, hipStream_t st) {
+    const size_t lds = (size_t)kWaves * std::min(a.group, kHeadTile) * (DP + 1) * sizeof(float);
+    if (vec && uni) kv_attend_kernel<T, DP, true, true><<<grid, 64 * kWaves, lds, st>>>(a);
+    else if (vec) kv_attend_kernel<T, DP, true, false><<<grid, 64 * kWaves, lds, st>>>(a);
+    else kv_attend_kernel<T, DP, false, false><<<grid, 64 * kWaves, lds, st>>>(a);
+}
+
+} // namespace
+
+size_t kv_attention_workspace_bytes(const SpinnHipKvAttentionDesc *d) {
+    const Plan p = plan(d);
+    return p.o_bytes + p.ml_bytes + p.score_bytes;
+}
+
+int kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k, const void *v, const int32_t *table,
+                 const int32_t *lengths, const uint8_t *mask, const float *acc, float *acc_out, void *o, float *lse,
+                 void *ws, hipStream_t st) {
+    const Plan p = plan(d);
+    const SpinnHipKvDesc &kv = d->kv;
+    AttendArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.table = table;
+    a.lengths = lengths;
+    a.mask = mask;
+    a.o = o;
+    a.lse = lse;
+    char *w = (char *)ws;
+    a.part_o = p.o_bytes ? (float *)w : nullptr;
+    a.part_ml = p.ml_bytes ? (float *)(w + p.o_bytes) : nullptr;
+    a.scores = p.score_bytes ? (float *)(w + p.o_bytes + p.ml_bytes) : nullptr;
+    a.q_stride = d->q_stride;
+    a.o_stride = d->o_stride;
+    a.mask_stride = d->mask_stride;
+    a.page_stride = kv.page_stride;
+    a.head_stride = kv.head_stride;
+    a.slot_stride = kv.slot_stride;
+    a.score_row = p.score_row;
+    a.scale2 = d->scale * kLog2e;
+    a.seqs = kv.seqs;
+    a.heads = d->heads;
+    a.kv_heads = kv.kv_heads;
+    a.group = d->heads / kv.kv_heads;
+    a.dim = kv.head_dim;
+    a.page_size = kv.page_size;
+    a.page_shift = (kv.page_size & (kv.page_size - 1)) == 0 ? __builtin_ctz(kv.page_size) : -1;
+    a.n_pages = kv.n_pages;
+    a.max_pages = kv.max_pages;
+    a.max_len = d->max_len;
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    a.head_tiles = p.head_tiles;
+    const int64_t blocks = (int64_t)kv.seqs * kv.kv_heads * p.head_tiles * p.splits;
+    const int acc_chunks = (d->max_len + kAccSlots - 1) / kAccSlots;
+    const int64_t join_blocks = p.splits > 1 ? (int64_t)kv.seqs * d->heads : 0;
+    const int64_t acc_blocks = d->accumulate ? (int64_t)kv.seqs * kv.kv_heads * acc_chunks : 0;
+    if (blocks > INT32_MAX || join_blocks + acc_blocks > INT32_MAX) return SPINN_HIP_EUNSUPPORTED;
+    const size_t hml = (size_t)a.group * 8;
+    if (hml > 32768) return SPINN_HIP_EUNSUPPORTED;
+    const int rc = with_dtype(kv.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        const int e = 16 / (int)sizeof(T);
+        const bool vec = kv.head_dim % e == 0 && kv.page_stride % e == 0 && kv.head_stride % e == 0 &&
+                         kv.slot_stride % e == 0 && aligned16(k) && aligned16(v);
+        const bool uni = kv.page_size % 16 == 0;
+        const dim3 grid((unsigned)blocks);
+        if (kv.head_dim <= 64) launch_attend<T, 64>(a, vec, uni, grid, st);
+        else if (kv.head_dim <= 128) launch_attend<T, 128>(a, vec, uni, grid, st);
+        else launch_attend<T, 256>(a, vec, uni, grid, st);
+        return check_launch();
+    });
+    if (rc || join_blocks + acc_blocks == 0) return rc;
+    return with_dtype(kv.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        kv_join_kernel<T><<<(unsigned)(join_blocks + acc_blocks), 256, hml, st>>>(a, (int)join_blocks, acc, acc_out,
+                                                                                  d->acc_stride, acc_chunks);
+        return check_launch();
+    });
+}
+
+int kv_append(const SpinnHipKvDesc *d, int64_t tokens, const int32_t *seq, const int32_t *slot, const int32_t *position,
+              const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *table, void *k_pages,
+              void *v_pages, float *acc, int32_t *pos, int64_t acc_stride, hipStream_t st) {
+    return with_dtype(d->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        const unsigned grid = (unsigned)std::min<int64_t>(tokens, 65536);
+        kv_append_kernel<T><<<grid, 256, 0, st>>>(*d, tokens, seq, slot, position, (const T *)k, k_stride, (const T *)v,
+                                                  v_stride, table, (T *)k_pages, (T *)v_pages, acc, pos, acc_stride);
+        return check_launch();
+    });
+}
+
+} // namespace spinn

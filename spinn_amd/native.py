@@ -35,6 +35,9 @@ BINARY_ADD, BINARY_SUB, BINARY_MUL, BINARY_DIV, BINARY_MOD = 0, 1, 2, 3, 4
 TOPK_MAX_K = 1024
 UNARY_RELU, UNARY_SIGMOID, UNARY_SILU = 0, 1, 2
 MAX_BLOCKS = 16
+TYPE_FLOAT32, TYPE_FLOAT16, TYPE_BFLOAT16 = 1, 10, 16  # ENNF_TYPE_*
+LINEAR_NONE, LINEAR_RELU, LINEAR_SILU, LINEAR_GELU, LINEAR_GELU_TANH = 0, 1, 3, 6, 7
+KV_MAX_DIM, BEAM_MAX, BEAM_MAX_K = 256, 64, 128
 
 
 class ConvDesc(C.Structure):
@@ -66,6 +69,38 @@ class GatherDesc(C.Structure):
 class BlockCopy(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row", C.c_int64), ("src_off", C.c_int64),
                 ("dst_row", C.c_int64), ("dst_off", C.c_int64), ("len", C.c_int64)]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("m", "n", "k", "dtype", "trans_w", "act", "x_unaligned", "reserved")] + \
+               [(n, C.c_int64) for n in ("ldx", "ldres", "ldy")]
+
+
+class KvDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "seqs", "kv_heads", "head_dim", "page_size", "n_pages", "max_pages",
+                                         "reserved")] + \
+               [(n, C.c_int64) for n in ("page_stride", "head_stride", "slot_stride")]
+
+
+class KvAttentionDesc(C.Structure):
+    _fields_ = [("kv", KvDesc), ("heads", C.c_int32), ("max_len", C.c_int32), ("scale", C.c_float),
+                ("accumulate", C.c_int32), ("q_stride", C.c_int64), ("o_stride", C.c_int64),
+                ("mask_stride", C.c_int64), ("acc_stride", C.c_int64)]
+
+
+class KvEvictDesc(C.Structure):
+    _fields_ = [("kv", KvDesc), ("budget", C.c_int32), ("recent", C.c_int32), ("sinks", C.c_int32),
+                ("max_len", C.c_int32), ("acc_stride", C.c_int64)]
+
+
+class BeamDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "batch", "beams", "vocab", "k", "end_token")] + \
+               [("logits_stride", C.c_int64)]
+
+
+class BeamState(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("row_bytes", C.c_int64), ("src_stride", C.c_int64),
+                ("dst_stride", C.c_int64)]
 
 
 class SpinnTensor(C.Structure):
@@ -166,6 +201,20 @@ _SIGS = {
     "spinn_hip_cast": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
     "spinn_hip_binary_typed": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
                                          C.c_int64, C.c_void_p]),
+    "spinn_hip_linear_packed_size": (C.c_size_t, [C.POINTER(LinearDesc)]),
+    "spinn_hip_linear_pack_weights": (C.c_int, [C.POINTER(LinearDesc), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "spinn_hip_linear_workspace_size": (C.c_size_t, [C.POINTER(LinearDesc)]),
+    "spinn_hip_linear": (C.c_int, [C.POINTER(LinearDesc)] + [C.c_void_p] * 6 + [C.c_size_t, C.c_void_p]),
+    "spinn_hip_kv_append": (C.c_int, [C.POINTER(KvDesc), C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.c_int64, C.c_void_p, C.c_int64] + [C.c_void_p] * 5 + [C.c_int64, C.c_void_p]),
+    "spinn_hip_kv_attention_workspace_size": (C.c_size_t, [C.POINTER(KvAttentionDesc)]),
+    "spinn_hip_kv_attention": (C.c_int, [C.POINTER(KvAttentionDesc)] + [C.c_void_p] * 11 + [C.c_size_t, C.c_void_p]),
+    "spinn_hip_kv_evict_workspace_size": (C.c_size_t, [C.POINTER(KvEvictDesc)]),
+    "spinn_hip_kv_evict": (C.c_int, [C.POINTER(KvEvictDesc)] + [C.c_void_p] * 11 + [C.c_size_t, C.c_void_p]),
+    "spinn_hip_beam_select_workspace_size": (C.c_size_t, [C.POINTER(BeamDesc)]),
+    "spinn_hip_beam_select": (C.c_int, [C.POINTER(BeamDesc)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
+    "spinn_hip_beam_reorder": (C.c_int, [C.POINTER(BeamState), C.c_int, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
+                                         C.c_void_p]),
     "spinn_hip_init": (C.c_int, [C.c_int]),
     "spinn_hip_device_count": (C.c_int, [C.POINTER(C.c_int)]),
     "spinn_hip_malloc": (C.c_int, [C.POINTER(C.c_void_p), C.c_size_t]),

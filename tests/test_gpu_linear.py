@@ -1,0 +1,133 @@
+"""spinn_hip_linear against the formula in 64 bits: types, layouts, ragged sizes, strides, epilogues.
+
+The bound of each element is derived in tests/decodeops.py (linear_ref)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from tests.decodeops import BF16, F16, F32, NAMES, TORCH, assert_close, gen, linear_pack, linear_ref, ptr, randn, stream, workspace
+
+pytestmark = pytest.mark.gpu
+
+
+def run(N, dtype, m, n, k, act=0, bias=False, res=False, trans_w=1, padx=0, padr=0, pady=0, off=0, seed=0, in_place=False):
+    """One call on rows of wider buffers; everything around y has to stay as it was."""
+    L, g, t = N.lib(), gen(seed + 7919 * m + 31 * n + k), TORCH[dtype]
+    x = randn(g, m, k + padx, dtype=dtype)
+    w = randn(g, *((n, k) if trans_w else (k, n)), dtype=dtype, scale=k ** -0.5)
+    b = randn(g, n, dtype=dtype) if bias else None
+    r = randn(g, m, n + padr, dtype=dtype) if res else None
+    if in_place:
+        pady = padr
+    xb = torch.full((off + m * (k + padx),), float("nan"), dtype=t, device="cuda")
+    xd = xb[off:].view(m, k + padx)
+    xd.copy_(x)
+    if padx:
+        xd[:, k:] = float("nan")  # behind a row: not read into any sum
+    rd = None if r is None else r.cuda()
+    yd = rd if in_place else torch.full((m + 2, n + pady), 777.0, dtype=t, device="cuda")
+    d = N.LinearDesc(m=m, n=n, k=k, dtype=dtype, trans_w=trans_w, act=act, x_unaligned=int(off % (16 // t.itemsize) != 0),
+                     ldx=k + padx, ldres=n + padr, ldy=n + pady)
+    packed = linear_pack(N, d, w.cuda())
+    size = L.spinn_hip_linear_workspace_size(C.byref(d))
+    ws = workspace(size)
+    print(f"[linear] {NAMES[dtype]} m={m} n={n} k={k} act={act} ws={size}", flush=True)
+    y0 = yd if in_place else yd[1:]
+    N.check(L.spinn_hip_linear(C.byref(d), ptr(xd), ptr(packed), ptr(None if b is None else b.cuda()), ptr(rd), ptr(y0),
+                               ptr(ws), size, stream()), "spinn_hip_linear")
+    torch.cuda.synchronize()
+    ref, tol = linear_ref(x[:, :k], w, trans_w, b, None if r is None else r[:, :n], act, dtype)
+    assert_close(y0[:m, :n], ref, tol, f"{NAMES[dtype]} {m}x{n}x{k}")
+    if in_place:
+        assert torch.equal(yd[:, n:].cpu(), r[:, n:])
+    else:
+        assert (yd[0] == 777).all() and (yd[m + 1] == 777).all() and (yd[:, n:] == 777).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("mnk", [(1, 1, 1), (1, 1000, 2048), (3, 17, 31), (16, 64, 64), (17, 65, 96), (33, 130, 257),
+                                 (64, 256, 128), (65, 300, 520), (128, 128, 64), (300, 200, 72), (1000, 1030, 200)], ids=str)
+def test_linear_sizes(hip, torch_gpu, dtype, mnk):
+    run(hip, dtype, *mnk, act=3, bias=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("mnk", [(2048, 4096, 96), (4100, 4200, 64), (1030, 1100, 136)], ids=str)
+def test_linear_many_tiles(hip, torch_gpu, dtype, mnk):
+    """Grids on the large tiles, with rows, columns and K that end inside one."""
+    run(hip, dtype, *mnk, bias=True, res=True)
+
+
+@pytest.mark.parametrize("act", [0, 1, 3, 6, 7])
+@pytest.mark.parametrize("bias,res", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("m", [5, 70, 600])
+def test_linear_epilogue(hip, torch_gpu, act, bias, res, m):
+    run(hip, F16, m, 520, 64, act=act, bias=bias, res=res)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m", [4, 90, 700])
+@pytest.mark.parametrize("trans_w", [0, 1])
+def test_linear_weight_layouts(hip, torch_gpu, dtype, m, trans_w):
+    run(hip, dtype, m, 333, 100, trans_w=trans_w, bias=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("m", [2, 100, 520])
+@pytest.mark.parametrize("padx,padr,pady,off", [(8, 0, 0, 0), (5, 0, 0, 0), (0, 3, 5, 0), (0, 8, 16, 0), (0, 0, 0, 3), (8, 4, 4, 8)])
+def test_linear_strides(hip, torch_gpu, dtype, m, padx, padr, pady, off):
+    """Rows inside wider buffers, x off its 16-byte boundary, residual and y in runs of 4 and not."""
+    run(hip, dtype, m, 260, 128, res=True, bias=True, padx=padx, padr=padr, pady=pady, off=off)
+
+
+@pytest.mark.parametrize("m", [1, 200, 600])
+def test_linear_in_place(hip, torch_gpu, m):
+    """y over its own residual, the residual stream of a network."""
+    run(hip, BF16, m, 256, 192, res=True, bias=True, padr=8, in_place=True)
+
+
+def test_linear_far_rows(hip, torch_gpu):
+    """Rows whose offsets pass 32 bits of bytes."""
+    N, L = hip, hip.lib()
+    m, n, k, ld = 3, 40, 64, 1 << 28
+    buf = torch.zeros(2 * ld + 64, dtype=torch.float32, device="cuda")
+    x = torch.as_strided(buf, (m, k), (ld, 1))
+    g = gen(1)
+    xc, w = randn(g, m, k), randn(g, n, k, scale=0.125)
+    x.copy_(xc)
+    d = N.LinearDesc(m=m, n=n, k=k, dtype=F32, trans_w=1, act=0, ldx=ld)
+    packed = linear_pack(N, d, w.cuda())
+    y = torch.empty(m, n, device="cuda")
+    assert L.spinn_hip_linear_workspace_size(C.byref(d)) == 0
+    N.check(L.spinn_hip_linear(C.byref(d), ptr(x), ptr(packed), None, None, ptr(y), None, 0, stream()), "linear")
+    assert_close(y, *linear_ref(xc, w, 1, None, None, 0, F32), "far rows")
+
+
+def test_linear_values(hip, torch_gpu):
+    """Infinities and NaN reach the outputs of their row and column alone; ReLU and SiLU of large
+    magnitudes; an empty batch."""
+    N, L = hip, hip.lib()
+    for m in (4, 70, 600):
+        n, k = 128, 64
+        g = gen(m)
+        x, w = randn(g, m, k, dtype=BF16), randn(g, n, k, dtype=BF16, scale=0.125)
+        x[1, 5], x[3, 0] = float("inf"), float("nan")
+        w[7, 9] = float("inf")
+        d = N.LinearDesc(m=m, n=n, k=k, dtype=BF16, trans_w=1, act=0)
+        packed, xd = linear_pack(N, d, w.cuda()), x.cuda()
+        y = torch.empty(m, n, device="cuda", dtype=torch.bfloat16)
+        N.check(L.spinn_hip_linear(C.byref(d), ptr(xd), ptr(packed), None, None, ptr(y), None, 0, stream()), "linear")
+        ref = x.double() @ w.double().t()
+        y = y.cpu().double()
+        assert torch.equal(y.isnan(), ref.isnan())
+        assert torch.equal(torch.where(y.isinf(), y, 0.0), torch.where(ref.isinf(), ref, 0.0))
+        big = (torch.randn(m, n, generator=g) * 30000).clamp(-60000, 60000).half()
+        d = N.LinearDesc(m=m, n=n, k=k, dtype=F16, trans_w=1, act=3)
+        packed, xd = linear_pack(N, d, torch.zeros(n, k, dtype=torch.float16, device="cuda")), torch.zeros(m, k, dtype=torch.float16, device="cuda")
+        y, bd = torch.empty(m, n, device="cuda", dtype=torch.float16), big.cuda()
+        N.check(L.spinn_hip_linear(C.byref(d), ptr(xd), ptr(packed), None, ptr(bd), ptr(y), None, 0, stream()), "linear")
+        ref = torch.nn.functional.silu(big.double()).half()
+        assert torch.equal(y.cpu(), ref + 0.0)
+    d = N.LinearDesc(m=0, n=n, k=k, dtype=F16, trans_w=1, act=3)
+    assert L.spinn_hip_linear(C.byref(d), None, None, None, None, None, None, 0, None) == 0
