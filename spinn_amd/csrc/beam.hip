@@ -3,10 +3,10 @@
 //
 // key(b,t) = score_b + x_bt - lse_b. Within a beam the keys order as the logits do, so one pass over a
 // chunk of a row finds the chunk's share of lse (its maximum and its sum of exponentials) and its k
-// first candidates together, from registers. The second launch joins a batch item's chunks.
-// Both pick k of n unique 64-bit ranks the same way: of the threads' own maxima the k-th largest
-// bounds the k-th largest of all from below, few elements pass it (at most k threads hold any),
-// and those few are ranked by counting. Bound: memory, each logit read once.
+// first candidates together, from registers: a lower bound for the k-th comes from the lanes' own
+// maxima, and the few elements that pass it are ranked by counting. The second launch joins a
+// batch item's chunks, merging their ordered lists by their heads.
+// Bound: memory, each logit read once; short rows by the latency of two launches.
 #include "decode.h"
 
 namespace spinn {
@@ -17,9 +17,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // fp32 to an unsigned number of the same order, both zeros equal; NaN as -inf, +inf as the largest finite.
 __device__ __forceinline__ float clean(float v) {
-    if (v != v) return -INFINITY;
-    v = v == 0.f ? 0.f : v;
-    return fminf(v, 3.402823466e38f);
+    return fminf(fmaxf(v, -INFINITY), 3.402823466e38f); // fmaxf of a NaN is its other operand
 }
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -31,6 +29,63 @@ __device__ __forceinline__ float unordered(uint32_t o) {
 __device__ __forceinline__ uint64_t ordered64(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v == 0.0 ? 0.0 : v);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+// Maximum over a wave of unsigned numbers, in every lane.
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_max(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, false);
+    const uint64_t o = (uint64_t)hi << 32 | lo;
+    return o > v ? o : v;
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+    const uint32_t o = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    v = dpp_umax<0x111>(v);
+    v = dpp_umax<0x112>(v);
+    v = dpp_umax<0x114>(v);
+    v = dpp_umax<0x118>(v);
+    v = dpp_umax<0x142>(v);
+    v = dpp_umax<0x143>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+    v = dpp_max<0x111>(v); // row_shr 1, 2, 4, 8: lane 15 of each row of 16 has the row's
+    v = dpp_max<0x112>(v);
+    v = dpp_max<0x114>(v);
+    v = dpp_max<0x118>(v);
+    v = dpp_max<0x142>(v); // row_bcast 15 and 31: lane 63 has all
+    v = dpp_max<0x143>(v);
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+
+// Order by logit, then by the lower token; never 0.
+__device__ __forceinline__ uint64_t rank32(float v, int token) {
+    return (uint64_t)ordered(v == 0.f ? 0.f : v) << 32 | (uint32_t)~token;
+}
+// -inf in every element of a word.
+__device__ __forceinline__ uint32_t no_logits(float) { return 0xff800000u; }
+__device__ __forceinline__ uint32_t no_logits(_Float16) { return 0xfc00fc00u; }
+__device__ __forceinline__ uint32_t no_logits(__bf16) { return 0xff80ff80u; }
+// Maximum over a wave, in every lane.
+template <int CTRL>
+__device__ __forceinline__ float dpp_fmax(float v) {
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v),
+                                                                         CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float wave_fmax(float v) {
+    v = dpp_fmax<0x111>(v);
+    v = dpp_fmax<0x112>(v);
+    v = dpp_fmax<0x114>(v);
+    v = dpp_fmax<0x118>(v);
+    v = dpp_fmax<0x142>(v);
+    v = dpp_fmax<0x143>(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 struct BeamArgs {
@@ -46,6 +101,9 @@ struct BeamArgs {
     int32_t batch, beams, vocab, k, end, chunks;
 };
 
+// Lanes whose elements the list of a chunk has room for: k and more.
+__host__ __device__ constexpr int beam_lanes(int k) { return 2 * k + 16 < kBeamThreads ? 2 * k + 16 : kBeamThreads; }
+
 // Elements per thread of a chunk of kBeamThreads * EPT.
 template <class T, int EPT, bool VEC>
 __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
@@ -57,106 +115,164 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
     const float score = clean(a.scores[row]);
     const bool ended = a.finished && a.finished[row], empty = score == -INFINITY;
 
-    // runs of E elements, a workgroup's runs side by side: equal logits then spread over the threads
+    if (ended || empty) { // the end token, where it is this chunk's, and the lowest others at -inf
+        const int in_chunk = min(a.vocab - base, kBeamThreads * EPT);
+        const int lead = ended && !empty && a.end >= base && a.end < base + in_chunk ? a.end : -1;
+        uint64_t *out = a.candidate + (int64_t)blockIdx.x * a.k;
+        for (int i = tid; i < a.k; i += kBeamThreads) {
+            int t = base + i;
+            if (lead >= 0) t = i == 0 ? lead : (t - 1 < lead ? t - 1 : t);
+            out[i] = i < in_chunk ? rank32(i == 0 && lead >= 0 ? 0.f : -INFINITY, t) : 0ull;
+        }
+        if (tid == 0) {
+            a.chunk_max[blockIdx.x] = -INFINITY;
+            a.chunk_sum[blockIdx.x] = 0.0;
+        }
+        return;
+    }
+    // runs of E elements, a workgroup's runs side by side: equal logits then spread over the threads.
+    // What lies behind the row is -inf like a hidden token, and comes after all tokens.
     float v[EPT];
-    int first[EPT / E]; // token of each run's first element
-#pragma unroll
-    for (int r = 0; r < EPT / E; ++r) first[r] = base + (r * kBeamThreads + tid) * E;
-    if (ended || empty) {
-#pragma unroll
-        for (int i = 0; i < EPT; ++i) v[i] = ended && !empty && first[i / E] + i % E == a.end ? 0.f : -INFINITY;
-    } else if constexpr (VEC) {
+    const int first = base + tid * E; // token of the first run
+    auto token = [&](int i) { return first + (i / E) * kBeamThreads * E + i % E; };
+    if constexpr (VEC) {
+        u32x4 w[EPT / E];
 #pragma unroll
         for (int r = 0; r < EPT / E; ++r) { // a row is whole runs
-            u32x4 w = {0, 0, 0, 0};
-            if (first[r] < a.vocab) w = *reinterpret_cast<const u32x4 *>(x + first[r]);
-            const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[r * E + i] = (float)e[i];
+            w[r] = (u32x4)(no_logits(T()));
+            if (token(r * E) < a.vocab) w[r] = *reinterpret_cast<const u32x4 *>(x + token(r * E));
         }
+#pragma unroll
+        for (int r = 0; r < EPT / E; ++r)
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[r * E + i] = (float)reinterpret_cast<const T *>(&w[r])[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            const int t = first[i / E] + i % E;
-            v[i] = t < a.vocab ? (float)x[t] : 0.f;
-        }
+        for (int i = 0; i < EPT; ++i) v[i] = token(i) < a.vocab ? (float)x[token(i)] : -INFINITY;
     }
-    // the thread's maximum, by value and then by the lower token
-    float best = -INFINITY;
-    uint64_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-        const int t = first[i / E] + i % E;
-        v[i] = clean(v[i]);
-        const uint64_t u = t < a.vocab ? (uint64_t)ordered(v[i]) << 32 | (uint32_t)~t : 0ull;
-        mine = u > mine ? u : mine;
-        if (t < a.vocab) best = fmaxf(best, v[i]);
-    }
-
-    __shared__ uint64_t top[kBeamThreads];
-    __shared__ float wmax[kBeamThreads / 64];
-    __shared__ double wsum[kBeamThreads / 64];
+    constexpr int kWaves = kBeamThreads / 64;
+    __shared__ float wmax[kWaves], wfloor[kWaves];
+    __shared__ double wsum[kWaves];
     __shared__ uint64_t bound;
-    __shared__ int count;
-    extern __shared__ uint64_t list[]; // [k * EPT]
-    top[tid] = mine;
+    __shared__ int count, passing;
+    extern __shared__ uint64_t list[]; // [beam_lanes(k) * EPT]
+    const int q = (a.k + kWaves - 1) / kWaves;
+    float best, floor, m;
+    double sum;
+    for (;;) {
+        best = -INFINITY; // a NaN leaves it as it is
 #pragma unroll
-    for (int off = 32; off; off >>= 1) best = fmaxf(best, __shfl_xor(best, off));
-    if (lane == 0) wmax[wave] = best;
-    if (tid == 0) {
-        bound = 0;
-        count = 0;
-    }
-    __syncthreads();
-    float m = wmax[0];
+        for (int i = 0; i < EPT; ++i) best = fmaxf(best, v[i]);
+        // Of each wave the q-th largest lane maximum, 4 q >= k: at least q of its elements reach it, so k
+        // of the chunk reach the least of the four (-inf, which all reach, where a chunk has fewer).
+        float nth = -INFINITY, left = best;
+        m = -INFINITY;
+        for (int i = 0; i < q; ++i) {
+            nth = wave_fmax(left);
+            if (i == 0) m = nth;
+            if (nth == -INFINITY) break;
+            if (lane == __ffsll((unsigned long long)__ballot(left == nth)) - 1) left = -INFINITY;
+        }
+        if (lane == 0) {
+            wmax[wave] = m;
+            wfloor[wave] = nth;
+        }
+        if (tid == 0) {
+            count = 0;
+            passing = 0;
+            bound = 0;
+        }
+        __syncthreads();
+        floor = wfloor[0];
+        m = wmax[0];
 #pragma unroll
-    for (int w = 1; w < kBeamThreads / 64; ++w) m = fmaxf(m, wmax[w]);
+        for (int w = 1; w < kWaves; ++w) {
+            m = fmaxf(m, wmax[w]);
+            floor = fminf(floor, wfloor[w]);
+        }
+        const uint64_t pass = __ballot(best >= floor);
+        if (lane == 0 && pass) atomicAdd(&passing, __popcll(pass));
 
-    // share of the sum: exponentials in fp32, added in fp64, so that beams compare to about 1e-8
-    if (!ended && !empty) {
-        double sum = 0.0;
+        // share of the sum: exponentials in fp32, added in fp64, so that beams compare to about 1e-8
+        sum = 0.0;
         if (m != -INFINITY) {
+            // exp(v - m) = 2^(v L - m L), in one rounding; what m L lost is a factor of the whole sum
+            const float shift = m * kLog2e, lost = fmaf(m, kLog2e, -shift);
+            if (fabsf(m) < 1e30f) {
 #pragma unroll
-            for (int i = 0; i < EPT; i += 4) {
-                float part = 0.f;
+                for (int i = 0; i < EPT; i += 4) {
+                    float part = 0.f;
 #pragma unroll
-                for (int j = i; j < i + 4; ++j)
-                    part += first[j / E] + j % E < a.vocab ? __builtin_amdgcn_exp2f((v[j] - m) * kLog2e) : 0.f;
-                sum += (double)part;
+                    for (int j = i; j < i + 4; ++j) part += __builtin_amdgcn_exp2f(fmaf(v[j], kLog2e, -shift));
+                    sum += (double)part;
+                }
+                sum *= (double)__builtin_amdgcn_exp2f(-lost);
+            } else {
+                for (int i = 0; i < EPT; ++i) sum += (double)__builtin_amdgcn_exp2f((v[i] - m) * kLog2e);
             }
         }
 #pragma unroll
         for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off);
         if (lane == 0) wsum[wave] = sum;
+        __syncthreads();
+        sum = wsum[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += wsum[w];
+        if (m < INFINITY && sum == sum) break;
+        // a NaN or +inf among the logits: once more without them
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) v[i] = clean(v[i]);
+        __syncthreads();
     }
-
-    // the k-th largest of the threads' maxima (unique but for the 0 of threads without elements)
-    if (a.k < kBeamThreads && mine != 0) {
-        int above = 0;
-        for (int i = 0; i < kBeamThreads; ++i) above += top[i] > mine;
-        if (above == a.k - 1) bound = mine;
+    if (floor > -INFINITY && passing <= beam_lanes(a.k)) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) n += v[i] >= floor;
+        if (n) {
+            int to = atomicAdd(&count, n);
+#pragma unroll
+            for (int i = 0; i < EPT; ++i)
+                if (v[i] >= floor) list[to++] = rank32(v[i], token(i));
+        }
+    } else {
+        // One wave's part of the row is far above another's, or many logits are equal: the k-th of all lane
+        // maxima instead, ties told apart by their tokens, from the waves' sorted ones (kept where the list
+        // comes later). At most k lanes reach it.
+        int at = 0;
+#pragma unroll
+        for (int i = EPT - 1; i >= 0; --i) {
+            v[i] = clean(v[i]);
+            at = v[i] == best ? token(i) : at;
+        }
+        const uint64_t mine = at < a.vocab ? rank32(best, at) : 0ull;
+        const int most = a.k < 64 ? a.k : 64;
+        uint64_t left = mine;
+        for (int i = 0; i < most; ++i) {
+            const uint64_t top = wave_max(left);
+            if (lane == 0) list[wave * most + i] = top;
+            if (left == top) left = 0;
+        }
+        __syncthreads();
+        int over = 0;
+        if (mine != 0)
+            for (int i = 0; i < kWaves * most; ++i) over += list[i] > mine;
+        if (mine != 0 && over == a.k - 1) bound = mine;
+        __syncthreads();
+        const uint64_t least = bound;
+        if (mine != 0 && mine >= least) {
+#pragma unroll
+            for (int i = 0; i < EPT; ++i)
+                if (token(i) < a.vocab) {
+                    const uint64_t u = rank32(v[i], token(i));
+                    if (u >= least) list[atomicAdd(&count, 1)] = u;
+                }
+        }
     }
     __syncthreads();
     if (tid == 0) {
-        a.chunk_max[blockIdx.x] = ended ? 0.f : m;
-        double sum = 1.0;
-        if (!ended && !empty) {
-            sum = wsum[0];
-#pragma unroll
-            for (int w = 1; w < kBeamThreads / 64; ++w) sum += wsum[w];
-        }
+        a.chunk_max[blockIdx.x] = m;
         a.chunk_sum[blockIdx.x] = sum;
     }
-    const uint64_t least = bound;
-    if (mine != 0 && mine >= least) {
-#pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-            const int t = first[i / E] + i % E;
-            const uint64_t u = t < a.vocab ? (uint64_t)ordered(v[i]) << 32 | (uint32_t)~t : 0ull;
-            if (u != 0 && u >= least) list[atomicAdd(&count, 1)] = u;
-        }
-    }
-    __syncthreads();
     // ranks by counting: which slot of the list an element got does not matter
     const int n = count;
     uint64_t *out = a.candidate + (int64_t)blockIdx.x * a.k;
@@ -171,9 +287,6 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
 
 // One workgroup per batch item: lse per beam, then the k first of the chunks' candidates in the order
 // of (key, lower beam, logit, lower token).
-constexpr int kJoinThreads = 512;
-constexpr int kJoinList = 1024; // candidates that pass the bound and are ranked by counting
-
 struct Rank {
     uint64_t key; // of the double, ordered; 0 = none
     uint32_t tie; // beams - beam
@@ -182,51 +295,74 @@ struct Rank {
 __device__ __forceinline__ bool above(const Rank &p, const Rank &q) {
     return p.key != q.key ? p.key > q.key : (p.tie != q.tie ? p.tie > q.tie : p.cand > q.cand);
 }
-
-__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a) {
-    constexpr int kWaves = kJoinThreads / 64;
-    const int item = blockIdx.x, tid = threadIdx.x;
-    const int lane = tid & 63, wave = tid >> 6;
-    __shared__ double lse[SPINN_HIP_BEAM_MAX], score[SPINN_HIP_BEAM_MAX];
-    __shared__ Rank list[kJoinList]; // first the threads' maxima, then what passes the bound
-    __shared__ Rank bound, best[kWaves];
-    __shared__ int count;
-    if (tid == 0) {
-        bound = Rank{0, 0, 0};
-        count = 0;
+// The lane whose rank is above all others' in the wave (any lane where there is none).
+__device__ __forceinline__ int first_lane(const Rank &r) {
+    const uint32_t high = (uint32_t)(r.key >> 32);
+    uint64_t tied = __ballot(high == wave_umax(high));
+    if (__popcll(tied) > 1) {
+        const uint64_t top = wave_max(r.key);
+        const uint64_t t = wave_max(r.key == top ? r.tie : 0u);
+        const bool in = r.key == top && r.tie == t;
+        const uint64_t c = wave_max(in ? r.cand : 0ull);
+        tied = __ballot(in && r.cand == c);
     }
-    for (int b = wave; b < a.beams; b += kWaves) {
+    return __ffsll((unsigned long long)tied) - 1;
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ Rank lane_rank(const Rank &r, int lane) {
+    return Rank{lane_u64(r.key, lane), (uint32_t)__builtin_amdgcn_readlane((int)r.tie, lane), lane_u64(r.cand, lane)};
+}
+
+constexpr int kJoinWaves = 16;    // at most
+constexpr int kJoinCached = 2048; // candidates held in LDS with their keys
+
+// Every lane has the heads of its lists (one, until there are more lists than lanes), and a
+// wave takes the first of them k times without a barrier; then one wave does the same with the waves' lists.
+template <bool CACHED>
+__global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a, int merging) {
+    const int item = blockIdx.x, tid = threadIdx.x, waves = blockDim.x >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ double lse[SPINN_HIP_BEAM_MAX], score[SPINN_HIP_BEAM_MAX];
+    __shared__ uint64_t key_at[CACHED ? kJoinCached : 1], cand_at[CACHED ? kJoinCached : 1];
+    extern __shared__ Rank merged[]; // [merging][k], where several waves merge
+    const int lists = a.beams * a.chunks, total = lists * a.k, per_beam = a.chunks * a.k;
+    const uint64_t *cand = a.candidate + (int64_t)item * total;
+    if constexpr (CACHED)
+        for (int i = tid; i < total; i += blockDim.x) cand_at[i] = cand[i];
+    for (int b = wave; b < a.beams; b += waves) {
         const int row = item * a.beams + b;
         const float *cm = a.chunk_max + (int64_t)row * a.chunks;
         const double *cs = a.chunk_sum + (int64_t)row * a.chunks;
+        const float sc = a.scores[row];
         float m = -INFINITY;
         for (int i = lane; i < a.chunks; i += 64) m = fmaxf(m, cm[i]);
-#pragma unroll
-        for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+        m = wave_fmax(m);
         double s = 0.0;
         if (m != -INFINITY)
             for (int i = lane; i < a.chunks; i += 64) s += cs[i] * exp((double)cm[i] - (double)m);
 #pragma unroll
         for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
         if (lane == 0) {
-            const bool ended = a.finished && a.finished[row];
-            score[b] = (double)clean(a.scores[row]);
-            lse[b] = ended || m == -INFINITY ? 0.0 : (double)m + log(s);
+            score[b] = (double)clean(sc);
+            lse[b] = m == -INFINITY ? 0.0 : (double)m + log(s);
         }
     }
     __syncthreads();
-    // lists of k, each in order: thread t takes every kJoinThreads-th candidate counted by
-    // place first, so that the lists' heads lie with different threads
-    const int lists = a.beams * a.chunks, total = lists * a.k;
-    const uint64_t *cand = a.candidate + (int64_t)item * total;
-    auto rank_of = [&](int i) {
-        const int place = i / lists, which = i - place * lists, b = which / a.chunks;
-        Rank r;
-        r.cand = cand[(int64_t)which * a.k + place];
-        r.tie = (uint32_t)(a.beams - b);
-        const float x = unordered((uint32_t)(r.cand >> 32));
-        r.key = r.cand == 0 ? 0ull : ordered64(x == -INFINITY ? -INFINITY : score[b] + ((double)x - lse[b]));
-        return r;
+    auto key_of = [&](uint64_t c, int b) {
+        const float x = unordered((uint32_t)(c >> 32));
+        return c == 0 ? 0ull : ordered64(x == -INFINITY ? -INFINITY : score[b] + ((double)x - lse[b]));
+    };
+    if constexpr (CACHED) {
+        for (int i = tid; i < total; i += blockDim.x) key_at[i] = key_of(cand_at[i], i / per_beam);
+        __syncthreads();
+    }
+    auto rank_of = [&](int list, int place) {
+        const int i = list * a.k + place, b = list / a.chunks;
+        if constexpr (CACHED) return Rank{key_at[i], (uint32_t)(a.beams - b), cand_at[i]};
+        else return Rank{key_of(cand[i], b), (uint32_t)(a.beams - b), cand[i]};
     };
     auto put = [&](const Rank &r, int rank) {
         const int64_t at = (int64_t)item * a.k + rank;
@@ -235,60 +371,72 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(BeamArgs a) {
         a.out_parents[at] = a.beams - (int)r.tie;
         a.out_tokens[at] = (int32_t) ~(uint32_t)r.cand;
     };
-    Rank mine{0, 0, 0};
-    for (int i = tid; i < total; i += kJoinThreads) {
-        const Rank r = rank_of(i);
-        if (r.key != 0 && above(r, mine)) mine = r;
-    }
-    list[tid] = mine;
-    __syncthreads();
-    if (mine.key != 0) {
-        int n = 0;
-        for (int i = 0; i < kJoinThreads; ++i) n += above(list[i], mine);
-        if (n == a.k - 1) bound = mine;
-    }
-    __syncthreads();
-    const Rank least = bound;
-    if (mine.key != 0 && !above(least, mine))
-        for (int i = tid; i < total; i += kJoinThreads) {
-            const Rank r = rank_of(i);
-            if (r.key != 0 && !above(least, r)) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kJoinList) list[at] = r;
+    if (wave < merging) {
+        const int first = wave * 64 + lane, step = merging * 64;
+        const bool one = lists <= step; // list per lane
+        int pos = 0;
+        auto at = [&](int place) { return first < lists && place < a.k ? rank_of(first, place) : Rank{0, 0, 0}; };
+        // the lane's first candidate after `last` over several lists, each in order
+        auto after = [&](const Rank &last) {
+            Rank r{0, 0, 0};
+            for (int l = first; l < lists; l += step)
+                for (int p = 0; p < a.k; ++p) {
+                    const Rank c = rank_of(l, p);
+                    if (c.key == 0) break;
+                    if (above(last, c)) {
+                        if (above(c, r)) r = c;
+                        break;
+                    }
+                }
+            return r;
+        };
+        Rank mine, follow{0, 0, 0}, taken{0, 0, 0};
+        if (one) {
+            mine = at(0);
+            follow = at(1);
+            pos = 2;
+        } else {
+            mine = after(Rank{~0ull, ~0u, ~0ull});
+        }
+        for (int i = 0; i < a.k; ++i) {
+            const int w = first_lane(mine);
+            const Rank r = lane_rank(mine, w);
+            if (lane == (i & 63)) taken = r;
+            if ((i & 63) == 63 || i == a.k - 1) {
+                const int to = (i & ~63) + lane;
+                if (to <= i) {
+                    if (merging == 1) put(taken, to);
+                    else merged[wave * a.k + to] = taken;
+                }
+            }
+            if (lane == w) {
+                if (one) {
+                    mine = follow;
+                    follow = at(pos++);
+                } else if (r.key != 0) {
+                    mine = after(r);
+                }
             }
         }
-    __syncthreads();
-    const int n = count;
-    if (n <= kJoinList) {
-        for (int i = tid; i < n; i += kJoinThreads) {
-            const Rank r = list[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += above(list[j], r);
-            if (rank < a.k) put(r, rank);
-        }
-        return;
     }
-    // more pass than the list holds (one thread's candidates far above the others'): one place at a time
-    Rank last{~0ull, ~0u, ~0ull};
-    for (int place = 0; place < a.k; ++place) {
-        Rank r{0, 0, 0};
-        for (int i = tid; i < total; i += kJoinThreads) {
-            const Rank c = rank_of(i);
-            if (c.key != 0 && above(last, c) && above(c, r)) r = c;
+    if (merging == 1) return;
+    __syncthreads();
+    if (wave) return;
+    int pos = 0;
+    auto head = [&]() { return lane < merging && pos < a.k ? merged[lane * a.k + pos] : Rank{0, 0, 0}; };
+    Rank mine = head(), taken{0, 0, 0};
+    for (int i = 0; i < a.k; ++i) {
+        const int w = first_lane(mine);
+        const Rank r = lane_rank(mine, w);
+        if (lane == (i & 63)) taken = r;
+        if ((i & 63) == 63 || i == a.k - 1) {
+            const int to = (i & ~63) + lane;
+            if (to <= i) put(taken, to);
         }
-#pragma unroll
-        for (int off = 32; off; off >>= 1) {
-            const Rank o{__shfl_xor(r.key, off), __shfl_xor(r.tie, off), __shfl_xor(r.cand, off)};
-            if (above(o, r)) r = o;
+        if (lane == w) {
+            ++pos;
+            mine = head();
         }
-        __syncthreads(); // the last place's readers are done
-        if (lane == 0) best[wave] = r;
-        __syncthreads();
-        r = best[0];
-        for (int w = 1; w < kWaves; ++w)
-            if (above(best[w], r)) r = best[w];
-        if (tid == 0) put(r, place);
-        last = r;
     }
 }
 
@@ -320,7 +468,7 @@ Plan plan(const SpinnHipBeamDesc *d) {
     const int64_t rows = (int64_t)d->batch * d->beams;
     auto chunks = [&](int ept) { return ((int64_t)d->vocab + kBeamThreads * ept - 1) / (kBeamThreads * ept); };
     // long chunks leave less to join, short ones fill the device
-    p.ept = 32;
+    p.ept = beam_lanes(d->k) <= 64 ? 64 : 32; // (the list of a chunk: 32 KB of LDS for 64 lanes)
     while (p.ept > 8 && rows * chunks(p.ept) < 2 * (int64_t)device_cu_count()) p.ept /= 2;
     p.chunks = (int)chunks(p.ept);
     p.max_bytes = round16((size_t)rows * p.chunks * 4);
@@ -332,7 +480,7 @@ Plan plan(const SpinnHipBeamDesc *d) {
 template <class T, int EPT>
 void launch_chunks(const BeamArgs &a, bool vec, hipStream_t st) {
     const unsigned grid = (unsigned)((int64_t)a.batch * a.beams * a.chunks);
-    const size_t lds = (size_t)a.k * EPT * 8;
+    const size_t lds = (size_t)std::max(beam_lanes(a.k) * EPT, 4 * std::min(a.k, 64)) * 8;
     if (vec) beam_chunk_kernel<T, EPT, true><<<grid, kBeamThreads, lds, st>>>(a);
     else beam_chunk_kernel<T, EPT, false><<<grid, kBeamThreads, lds, st>>>(a);
 }
@@ -370,13 +518,19 @@ int beam_select(const SpinnHipBeamDesc *d, const void *logits, const float *scor
         typedef decltype(t) T;
         const int e = 16 / (int)sizeof(T);
         const bool vec = d->vocab % e == 0 && d->logits_stride % e == 0 && aligned16(logits);
-        if (p.ept == 32) launch_chunks<T, 32>(a, vec, st);
+        if (p.ept == 64) launch_chunks<T, 64>(a, vec, st);
+        else if (p.ept == 32) launch_chunks<T, 32>(a, vec, st);
         else if (p.ept == 16) launch_chunks<T, 16>(a, vec, st);
         else launch_chunks<T, 8>(a, vec, st);
         return check_launch();
     });
     if (rc) return rc;
-    beam_join_kernel<<<(unsigned)a.batch, kJoinThreads, 0, st>>>(a);
+    const int64_t lists = (int64_t)a.beams * a.chunks;
+    const int merging = (int)std::min<int64_t>(kJoinWaves, (lists + 63) / 64);
+    const int waves = std::max(merging, std::min(kJoinWaves, std::max(4, a.beams))); // a wave per beam's lse
+    const size_t lds = merging > 1 ? (size_t)merging * a.k * sizeof(Rank) : 0;
+    if (lists * a.k <= kJoinCached) beam_join_kernel<true><<<(unsigned)a.batch, 64 * waves, lds, st>>>(a, merging);
+    else beam_join_kernel<false><<<(unsigned)a.batch, 64 * waves, lds, st>>>(a, merging);
     return check_launch();
 }
 

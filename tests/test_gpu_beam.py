@@ -83,6 +83,10 @@ def test_select_one_thread_holds_the_best(hip, torch_gpu, k):
     x, s = make(k, F32, 1, 4, 30000)
     x[0, 2, 4096:4096 + 64] = 30 + torch.arange(64.0)
     select(hip, F32, x, s, k)
+    for runs in (1, 8, 256):  # ascending rows, and rows that ascend within every run: parts of a chunk far above others
+        y = torch.sort(x[0].reshape(4, 30000 // 8 // 25, -1), 2)[0].reshape(1, 4, 30000)
+        y = y + (torch.arange(30000) // runs % 64).float() * 0.5
+        select(hip, F32, y, s, k)
     x, s = make(k + 1, F32, 1, 4, 30000)
     x[0] = torch.sort(x[0], 1)[0]
     select(hip, F32, x, s, k)

@@ -79,6 +79,13 @@ def test_attention_head_groups(hip, torch_gpu, dtype, heads, kv):
     attend(hip, c, [200, 77], heads=heads, accumulate=True)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+def test_attention_many_long_heads(hip, torch_gpu, dtype):
+    """The most query heads a workgroup takes, at the longest rows: the most that it joins on chip."""
+    c = Cache(gen(2), dtype, 1, 2, 256, 16, 500)
+    attend(hip, c, [500], heads=32, accumulate=True)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
 @pytest.mark.parametrize("slots", [1, 2, 31, 32, 33, 127, 128, 129, 255, 257, 1000, 5000])
 def test_attention_lengths(hip, torch_gpu, dtype, slots):
