@@ -21,7 +21,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kTile = 32;     // slots per step of a wave: two halves of 16 rows
+constexpr int kStep = 128;    // slots of a split are a multiple of this
 constexpr int kHeadTile = 16; // query heads of one kv head per workgroup
 constexpr int kWaves = 4;
 
@@ -33,17 +33,25 @@ struct AttendArgs {
     const uint8_t *mask;
     void *o;
     float *lse;
-    float *part_o, *part_ml; // [seqs][heads][splits][dim], [..][2] (maximum and sum, base 2)
+    float *part_o, *part_ml; // [seqs][heads][splits][part_row], [..][2] (maximum and sum, base 2)
     float *scores;           // [seqs][heads][score_row], base 2; null when no weights are wanted
     int64_t q_stride, o_stride, mask_stride, page_stride, head_stride, slot_stride, score_row;
     float scale2; // scale * log2 e
-    int32_t seqs, heads, kv_heads, group, dim, page_size, page_shift, n_pages, max_pages, max_len;
+    int32_t seqs, heads, kv_heads, group, dim, page_size, n_pages, max_pages, max_len;
+    uint32_t page_mul, page_shift; // slot / page_size = slot * page_mul >> 32 + page_shift (page_mul 0: slot)
+    int32_t q_runs;        // query rows are whole 16-byte runs
+    int32_t part_row;      // dim rounded up to a multiple of 4
     int32_t splits, chunk; // chunk: slots per split, a multiple of kTile * kWaves
-    int32_t head_tiles;
+    int32_t head_tiles, parts; // parts: seqs * kv_heads * splits
 };
 
+// A number that no kernel writes meanwhile, at an index that is the same in every lane: through the scalar cache.
+__device__ __forceinline__ int32_t scalar_at(const int32_t *p, int i) {
+    return ((const __attribute__((address_space(4))) int32_t *)p)[i];
+}
+
 __device__ __forceinline__ int page_of(const AttendArgs &a, int slot) {
-    return a.page_shift >= 0 ? slot >> a.page_shift : slot / a.page_size;
+    return a.page_mul ? (int)(__umulhi((uint32_t)slot, a.page_mul) >> a.page_shift) : slot;
 }
 
 // 16 bytes at p, element by element: those from `left` on (elements to the row's end) are zero.
@@ -71,20 +79,32 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
     constexpr int DPL = DP / 16;              // a lane's elements of a V row: DPL n .. +DPL-1
     constexpr int VB = DPL * (int)sizeof(T);  // their bytes
     constexpr int VW = VB / 4;                // and words
+    constexpr int H = sizeof(T) == 2 ? 2 : 1; // halves of 16 slots in a wave's step: a 16-bit product takes 32
+    constexpr int kTile = 16 * H;
+    static_assert(kStep % (kTile * kWaves) == 0, "");
     constexpr float kPScale = sizeof(T) == 2 && !__is_same(T, __bf16) ? 16384.f : 1.f;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
 
-    int b = blockIdx.x;
-    const int ht = b % a.head_tiles;
-    b /= a.head_tiles;
+    // the head tiles of a part, which read the same rows, are workgroups of one XCD (b % 8) one after the other
+    const int per = 8 * a.head_tiles, ht = (int)(blockIdx.x % per) >> 3;
+    int b = (int)(blockIdx.x / per) * 8 + (int)(blockIdx.x & 7);
+    if (b >= a.parts) return;
     const int sp = b % a.splits;
     b /= a.splits;
     const int kvh = b % a.kv_heads, seq = b / a.kv_heads;
     const int h0 = kvh * a.group + ht * kHeadTile;              // first query head of the tile
     const int nh = min(kHeadTile, a.group - ht * kHeadTile);    // query heads in it
-    const int len = min(max(a.lengths[seq], 0), a.max_len);
+    const int len = min(max(scalar_at(a.lengths, seq), 0), a.max_len);
     const int begin = sp * a.chunk, end = min(len, begin + a.chunk);
+    if (begin >= len && sp > 0) { // nothing here (a sequence's first part writes o and lse where it is the only one)
+        if ((int)threadIdx.x < nh) {
+            float *ml = a.part_ml + (((int64_t)seq * a.heads + h0 + threadIdx.x) * a.splits + sp) * 2;
+            ml[0] = -INFINITY;
+            ml[1] = 0.f;
+        }
+        return;
+    }
     const int32_t *table = a.table + (int64_t)seq * a.max_pages;
     const uint8_t *mask = a.mask ? a.mask + (int64_t)seq * a.mask_stride : nullptr;
 
@@ -95,7 +115,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             const int d0 = c * kFrag<T> + g * E;
-            q[c] = load_edge<T>(qp + d0, n < nh ? a.dim - d0 : 0);
+            if (VEC && a.q_runs) q[c] = n < nh && d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
+            else q[c] = load_edge<T>(qp + d0, n < nh ? a.dim - d0 : 0);
         }
     }
 
@@ -104,118 +125,142 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
     const T *kb = (const T *)a.k + (int64_t)kvh * a.head_stride;
     const T *vb = (const T *)a.v + (int64_t)kvh * a.head_stride;
 
-    for (int t0 = begin + wave * kTile; t0 < end; t0 += kTile * kWaves) {
-        u32x4 kr[2][KC];
-        uint32_t vr[8][VW];
-        uint32_t seen = 0; // bit j: the lane's j-th slot (4g+j, then 16+4g+j-4) is visible
-        const T *vrow[8];
-        // rows: addresses first, so that all of a tile's loads are in flight together
-        if constexpr (UNI) {
+    // UNI: where each half of a tile starts. The page number comes through the scalar cache (a vector load would
+    // wait for all rows in flight before it) a step ahead of its use.
+    // Otherwise every lane looks up its rows' pages, a step ahead, too.
+    constexpr int L = UNI ? H : 5 * H; // page numbers of a tile: of the halves, or of the lane's K rows and V rows
+    auto slot_of = [&](int t0, int i) {
+        if constexpr (UNI) return min(t0 + 16 * i, (len - 1) & ~15);
+        else return min(t0 + (i < H ? 16 * i + n : 16 * ((i - H) >> 2) + 4 * g + ((i - H) & 3)), len - 1);
+    };
+    int coming[L];  // page numbers of the next tile
+    int64_t at[L];  // where the current tile's rows are
+    uint32_t there; // bit i: they are in a page
+    auto look_up = [&](int t0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int s0 = min(t0 + 16 * h, (len - 1) & ~15);
-                const int pi = page_of(a, s0);
-                int page = table[pi];
-                const bool ok = (unsigned)page < (unsigned)a.n_pages;
-                page = ok ? page : 0;
-                const int64_t at = (int64_t)page * a.page_stride + (int64_t)(s0 - pi * a.page_size) * a.slot_stride;
-                const T *kp = kb + at + (int64_t)n * a.slot_stride + g * E;
+        for (int i = 0; i < L; ++i) {
+            const int pi = page_of(a, slot_of(t0, i));
+            if constexpr (UNI) coming[i] = scalar_at(table, pi);
+            else coming[i] = table[pi];
+        }
+    };
+    auto place = [&](int t0) {
+        there = 0;
 #pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const bool in = c * kFrag<T> + g * E < a.dim;
-                    kr[h][c] = in ? *reinterpret_cast<const u32x4 *>(kp + c * kFrag<T>) : (u32x4){0, 0, 0, 0};
-                }
+        for (int i = 0; i < L; ++i) {
+            const int slot = slot_of(t0, i);
+            const bool ok = (unsigned)coming[i] < (unsigned)a.n_pages;
+            there |= (uint32_t)ok << i;
+            at[i] = (int64_t)(ok ? coming[i] : 0) * a.page_stride + (int64_t)(slot - page_of(a, slot) * a.page_size) * a.slot_stride;
+        }
+    };
+    // K's rows of a tile: lane (g, n) takes row n of each half
+    u32x4 kr[H][KC];
+    auto load_k = [&](int t0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    vrow[4 * h + j] = vb + at + (int64_t)(4 * g + j) * a.slot_stride;
-                    if (ok && t0 + 16 * h + 4 * g + j < end) seen |= 1u << (4 * h + j);
-                }
-            }
-        } else {
+        for (int h = 0; h < H; ++h) {
+            const T *kp = kb + at[h];
+            if constexpr (UNI) kp += (int64_t)n * a.slot_stride;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int slot = min(t0 + 16 * h + n, len - 1);
-                const int pi = page_of(a, slot);
-                int page = table[pi];
-                page = (unsigned)page < (unsigned)a.n_pages ? page : 0;
-                const T *kp = kb + (int64_t)page * a.page_stride + (int64_t)(slot - pi * a.page_size) * a.slot_stride + g * E;
-#pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const int left = a.dim - (c * kFrag<T> + g * E);
-                    if constexpr (VEC)
-                        kr[h][c] = left > 0 ? *reinterpret_cast<const u32x4 *>(kp + c * kFrag<T>) : (u32x4){0, 0, 0, 0};
-                    else
-                        kr[h][c] = load_edge<T>(kp + c * kFrag<T>, left);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int want = t0 + 16 * h + 4 * g + j;
-                    const int vs = min(want, len - 1);
-                    const int vi = page_of(a, vs);
-                    int vpage = table[vi];
-                    const bool ok = (unsigned)vpage < (unsigned)a.n_pages;
-                    vpage = ok ? vpage : 0;
-                    vrow[4 * h + j] = vb + (int64_t)vpage * a.page_stride + (int64_t)(vs - vi * a.page_size) * a.slot_stride;
-                    if (ok && want < end) seen |= 1u << (4 * h + j);
-                }
+            for (int c = 0; c < KC; ++c) {
+                const int d0 = c * kFrag<T> + g * E;
+                if constexpr (VEC) kr[h][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(kp + d0) : (u32x4){0, 0, 0, 0};
+                else kr[h][c] = load_edge<T>(kp + d0, a.dim - d0);
             }
         }
+    };
+    // V's: lane (g, n) takes its columns of rows 4g..4g+3 of each half; which of them are visible
+    uint32_t vr[4 * H][VW];
+    uint32_t seen; // bit j: the lane's j-th slot, t0 + 16 (j/4) + 4g + j%4, is one of the part's
+    uint8_t shown[4 * H];
+    auto load_v = [&](int t0) {
+        seen = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const T *vp = vrow[j] + n * DPL;
-            if constexpr (VEC) {
-                // in 16-byte runs (8 where a lane's share is 8); a row ends between runs
-                constexpr int R = VB >= 16 ? 16 : VB;
+        for (int h = 0; h < H; ++h) {
 #pragma unroll
-                for (int r = 0; r < VB / R; ++r) {
-                    const bool in = n * DPL + r * (R / (int)sizeof(T)) < a.dim;
-                    if constexpr (R == 16) {
-                        const u32x4 w = in ? *reinterpret_cast<const u32x4 *>(vp + r * E) : (u32x4){0, 0, 0, 0};
+            for (int j = 0; j < 4; ++j) {
+                const T *vp = vb + n * DPL;
+                if constexpr (UNI) vp += at[h] + (int64_t)(4 * g + j) * a.slot_stride;
+                else vp += at[H + 4 * h + j];
+                const int slot = t0 + 16 * h + 4 * g + j;
+                if ((there >> (UNI ? h : H + 4 * h + j) & 1u) && slot < end) {
+                    seen |= 1u << (4 * h + j);
+                    if (mask) shown[4 * h + j] = mask[slot]; // read where it is needed
+                }
+                uint32_t(&to)[VW] = vr[4 * h + j];
+                if constexpr (VEC) {
+                    // in 16-byte runs (8 where a lane's share is 8); a row ends between runs
+                    constexpr int R = VB >= 16 ? 16 : VB;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) vr[j][4 * r + i] = w[i];
-                    } else {
-                        const u32x2 w = in ? *reinterpret_cast<const u32x2 *>(vp) : (u32x2){0, 0};
-                        vr[j][0] = w[0];
-                        vr[j][1] = w[1];
+                    for (int r = 0; r < VB / R; ++r) {
+                        const bool in = n * DPL + r * (R / (int)sizeof(T)) < a.dim;
+                        if constexpr (R == 16) {
+                            const u32x4 w = in ? *reinterpret_cast<const u32x4 *>(vp + r * E) : (u32x4){0, 0, 0, 0};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) to[4 * r + i] = w[i];
+                        } else {
+                            const u32x2 w = in ? *reinterpret_cast<const u32x2 *>(vp) : (u32x2){0, 0};
+                            to[0] = w[0];
+                            to[1] = w[1];
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < (VB + 15) / 16; ++r) {
+                        const u32x4 w = load_edge<T>(vp + r * E, min(a.dim - n * DPL - r * E, DPL - r * E));
+#pragma unroll
+                        for (int i = 0; i < (VW < 4 ? VW : 4); ++i) to[4 * r + i] = w[i];
                     }
                 }
-            } else {
-#pragma unroll
-                for (int r = 0; r < (VB + 15) / 16; ++r) {
-                    const u32x4 w = load_edge<T>(vp + r * E, min(a.dim - n * DPL - r * E, DPL - r * E));
-#pragma unroll
-                    for (int i = 0; i < (VW < 4 ? VW : 4); ++i) vr[j][4 * r + i] = w[i];
-                }
             }
         }
+    };
+
+    // The registers of K are free once the scores are there and those of V at the end of a step: each takes
+    // the next tile's rows at once, which then travel during the other's products.
+    int t0 = begin + wave * kTile;
+    if (t0 < end) {
+        look_up(t0);
+        place(t0);
+        load_k(t0);
+        load_v(t0);
+        look_up(t0 + kTile * kWaves);
+    }
+    for (; t0 < end; t0 += kTile * kWaves) {
+        const int t1 = t0 + kTile * kWaves;
+        uint32_t vis = seen;
         if (mask) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int slot = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
-                if (seen >> j & 1u)
-                    if (mask[slot] == 0) seen &= ~(1u << j);
-            }
+            for (int j = 0; j < 4 * H; ++j)
+                if (shown[j] == 0) vis &= ~(1u << j);
         }
 
         // scores, base 2
-        float s[8];
+        float s[4 * H];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
             f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < KC; ++i) mfma_frag(c, kr[h][i], q[i], T());
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * h + i] = (seen >> (4 * h + i) & 1u) ? c[i] * a.scale2 : -INFINITY;
+            for (int i = 0; i < 4; ++i) s[4 * h + i] = (vis >> (4 * h + i) & 1u) ? c[i] * a.scale2 : -INFINITY;
+        }
+        if (t1 < end) {
+            place(t1);
+            look_up(t1 + kTile * kWaves);
+            load_k(t1);
         }
         if (a.scores && n < nh) {
             float *row = a.scores + ((int64_t)seq * a.heads + h0 + n) * a.score_row + t0 + 4 * g;
-            *reinterpret_cast<f32x4 *>(row) = (f32x4){s[0], s[1], s[2], s[3]};
-            *reinterpret_cast<f32x4 *>(row + 16) = (f32x4){s[4], s[5], s[6], s[7]};
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+                *reinterpret_cast<f32x4 *>(row + 16 * h) = (f32x4){s[4 * h], s[4 * h + 1], s[4 * h + 2], s[4 * h + 3]};
         }
-        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 4 * H; ++j) top = fmaxf(top, s[j]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        top = fmaxf(top, m);
         const float base = top == -INFINITY ? 0.f : top;
         if (__any(top > m)) {
             const float alpha = exp2_hw(m - base);
@@ -224,17 +269,17 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
             for (int c = 0; c < DPL; ++c) acc[c] *= alpha;
             m = top;
         }
-        float p[8];
+        float p[4 * H];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4 * H; ++j) {
             p[j] = exp2_hw(s[j] - base);
             l += p[j];
         }
         // rows that are not visible may hold anything, and 0 * NaN is NaN
-        if (__any(seen != 0xffu)) {
+        if (__any(vis != (1u << 4 * H) - 1)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!(seen >> j & 1u))
+            for (int j = 0; j < 4 * H; ++j)
+                if (!(vis >> j & 1u))
 #pragma unroll
                     for (int i = 0; i < VW; ++i) vr[j][i] = 0u;
         }
@@ -243,37 +288,37 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
             // p as two 16-bit parts, the rounding and what it left: the product then carries p to
             // 2^-16 and better, for one more pass of a unit that is idle. fp16 takes p times 2^14:
             // its least number is 2^-24, which weights of a long sequence fall under.
-            u32x4 hi, lo;
+            uint32_t hi[2 * H], lo[2 * H];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t wh = 0, wl = 0;
+            for (int i = 0; i < 2 * H; ++i) {
+                hi[i] = lo[i] = 0;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float v = p[2 * i + e] * kPScale;
                     const T r = (T)v;
                     const T rest = (T)(v - (float)r);
-                    wh |= (uint32_t) __builtin_bit_cast(uint16_t, r) << (16 * e);
-                    wl |= (uint32_t) __builtin_bit_cast(uint16_t, rest) << (16 * e);
+                    hi[i] |= (uint32_t) __builtin_bit_cast(uint16_t, r) << (16 * e);
+                    lo[i] |= (uint32_t) __builtin_bit_cast(uint16_t, rest) << (16 * e);
                 }
-                hi[i] = wh;
-                lo[i] = wl;
             }
 #pragma unroll
             for (int c = 0; c < DPL; ++c) {
-                u32x4 f; // V^T: row c of the lane's columns, its eight slots
+                uint32_t f[2 * H]; // V^T: row c of the lane's columns, its slots
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 2 * H; ++i)
                     f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c / 2], vr[2 * i][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
-                mfma_frag(acc[c], f, hi, T());
-                mfma_frag(acc[c], f, lo, T());
+                const u32x4 fv = {f[0], f[1], f[2], f[3]};
+                mfma_frag(acc[c], fv, (u32x4){hi[0], hi[1], hi[2], hi[3]}, T());
+                mfma_frag(acc[c], fv, (u32x4){lo[0], lo[1], lo[2], lo[3]}, T());
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4 * H; ++j)
 #pragma unroll
                 for (int c = 0; c < DPL; ++c)
                     acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[j][c]), p[j], acc[c], 0, 0, 0);
         }
+        if (t1 < end) load_v(t1);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -317,7 +362,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) v += so[(w * nh + h) * kRow + d];
                 if (whole) ((T *)a.o)[(int64_t)seq * a.o_stride + (int64_t)(h0 + h) * a.dim + d] = (T)(v * inv);
-                else a.part_o[(sh * a.splits + sp) * a.dim + d] = v;
+                else a.part_o[(sh * a.splits + sp) * a.part_row + d] = v;
             }
         if (lane == 0) {
             if (whole && a.lse) a.lse[sh] = L == 0.f ? -INFINITY : (Mh + __log2f(L)) * kLn2;
@@ -356,21 +401,28 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int join_blo
         float M, L;
         join_ml(ml, a.splits, lane, M, L);
         const float base = M == -INFINITY ? 0.f : M;
-        // a strand of `cols` threads takes every strands-th split
-        const int cols = a.dim <= 64 ? 64 : (a.dim <= 128 ? 128 : 256);
-        const int strands = 256 / cols, strand = threadIdx.x / cols, d = threadIdx.x % cols;
-        float v = 0.f;
-        if (d < a.dim)
+        // strands of threads, each over the row's runs of 4, take every strands-th split
+        __shared__ float sum[256 * 4];
+        const int runs = (a.dim + 3) / 4;
+        int cols = 1;
+        while (cols < runs) cols *= 2;
+        const int strands = 256 / cols, strand = threadIdx.x / cols, d = threadIdx.x % cols * 4;
+        const float *po = a.part_o + (int64_t)sh * a.splits * a.part_row + d;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (d < a.dim) {
+#pragma unroll 4
             for (int i = strand; i < a.splits; i += strands) {
                 const float mi = ml[2 * i];
-                if (mi != -INFINITY) v += a.part_o[((int64_t)sh * a.splits + i) * a.dim + d] * exp2_hw(mi - base);
+                // (a split with nothing visible wrote no row)
+                if (mi != -INFINITY) v += *reinterpret_cast<const f32x4 *>(po + (int64_t)i * a.part_row) * exp2_hw(mi - base);
             }
-        __shared__ float sum[256];
-        sum[threadIdx.x] = v;
+        }
+        *reinterpret_cast<f32x4 *>(sum + threadIdx.x * 4) = v;
         __syncthreads();
-        if (strand == 0 && d < a.dim) {
-            for (int i = 1; i < strands; ++i) v += sum[i * cols + d];
-            ((T *)a.o)[(int64_t)seq * a.o_stride + (int64_t)h * a.dim + d] = (T)(L == 0.f ? 0.f : v / L);
+        if ((int)threadIdx.x < a.dim) {
+            float r = 0.f;
+            for (int i = 0; i < strands; ++i) r += sum[i * cols * 4 + threadIdx.x];
+            ((T *)a.o)[(int64_t)seq * a.o_stride + (int64_t)h * a.dim + threadIdx.x] = (T)(L == 0.f ? 0.f : r / L);
         }
         if (threadIdx.x == 0 && a.lse) a.lse[sh] = L == 0.f ? -INFINITY : (M + __log2f(L)) * kLn2;
         return;
@@ -445,16 +497,19 @@ Plan plan(const SpinnHipKvAttentionDesc *d) {
     const int group = d->heads / d->kv.kv_heads;
     p.head_tiles = (group + kHeadTile - 1) / kHeadTile;
     const int64_t units = (int64_t)d->kv.seqs * d->kv.kv_heads * p.head_tiles;
-    constexpr int step = kTile * kWaves;
-    const int64_t steps = std::max<int64_t>(1, (d->max_len + step - 1) / step);
-    // four workgroups per CU
-    const int64_t want = (4 * (int64_t)device_cu_count() + units - 1) / units;
-    const int64_t per = std::max<int64_t>(2, (steps + want - 1) / want); // steps per split
-    p.splits = (int)((steps + per - 1) / per);
-    p.chunk = (int)(per * step);
+    const int64_t steps = std::max<int64_t>(1, (d->max_len + kStep - 1) / kStep);
+    // Parts of about 1 MB at most: a workgroup's start and end cost as much as 100 KB of reading (32 sequences of 37 to 8000
+    // slots, 8 x 128 bf16: 159 us at 128 KB, 141 at 256, 132 at 512, 122 at 1 MB, 137 unsplit).
+    // Shorter ones, down to a step per wave, where longer ones would leave CUs idle.
+    const int64_t fill = (steps * units + 2 * device_cu_count() - 1) / (2 * device_cu_count());
+    const int64_t bytes = (int64_t)2 * kStep * d->kv.head_dim * dtype_bytes(d->kv.dtype);
+    const int64_t most = std::max<int64_t>(1, std::min(fill, (1048576 + bytes - 1) / bytes)); // steps per split
+    p.splits = (int)((steps + most - 1) / most);
+    const int64_t per = (steps + p.splits - 1) / p.splits; // alike
+    p.chunk = (int)(per * kStep);
     const int64_t rows = (int64_t)d->kv.seqs * d->heads;
-    p.score_row = ((int64_t)d->max_len + kTile - 1) / kTile * kTile;
-    p.o_bytes = p.splits > 1 ? round16((size_t)rows * p.splits * d->kv.head_dim * 4) : 0;
+    p.score_row = ((int64_t)d->max_len + 31) / 32 * 32;
+    p.o_bytes = p.splits > 1 ? (size_t)rows * p.splits * ((d->kv.head_dim + 3) & ~3) * 4 : 0;
     p.ml_bytes = p.splits > 1 || d->accumulate ? round16((size_t)rows * p.splits * 8) : 0;
     p.score_bytes = d->accumulate ? (size_t)rows * p.score_row * 4 : 0;
     return p;
@@ -507,14 +562,22 @@ int kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k,
     a.group = d->heads / kv.kv_heads;
     a.dim = kv.head_dim;
     a.page_size = kv.page_size;
-    a.page_shift = (kv.page_size & (kv.page_size - 1)) == 0 ? __builtin_ctz(kv.page_size) : -1;
+    // Rounded up, page_mul is off by less than 1, so the product for a slot below 2^31 by less than 2^31: under
+    // one part in page_size of 2^(32 + shift) as long as page_size <= 2^(shift + 1).
+    if (kv.page_size > 1) {
+        a.page_shift = 31 - __builtin_clz((unsigned)kv.page_size - 1);
+        a.page_mul = (uint32_t)((((uint64_t)1 << (32 + a.page_shift)) + kv.page_size - 1) / kv.page_size);
+    }
     a.n_pages = kv.n_pages;
     a.max_pages = kv.max_pages;
     a.max_len = d->max_len;
+    a.part_row = (kv.head_dim + 3) & ~3;
     a.splits = p.splits;
     a.chunk = p.chunk;
     a.head_tiles = p.head_tiles;
-    const int64_t blocks = (int64_t)kv.seqs * kv.kv_heads * p.head_tiles * p.splits;
+    const int64_t parts = (int64_t)kv.seqs * kv.kv_heads * p.splits;
+    const int64_t blocks = (parts + 7) / 8 * 8 * p.head_tiles;
+    a.parts = (int32_t)parts;
     const int acc_chunks = (d->max_len + kAccSlots - 1) / kAccSlots;
     const int64_t join_blocks = p.splits > 1 ? (int64_t)kv.seqs * d->heads : 0;
     const int64_t acc_blocks = d->accumulate ? (int64_t)kv.seqs * kv.kv_heads * acc_chunks : 0;
@@ -527,6 +590,7 @@ int kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k,
         const bool vec = kv.head_dim % e == 0 && kv.page_stride % e == 0 && kv.head_stride % e == 0 &&
                          kv.slot_stride % e == 0 && aligned16(k) && aligned16(v);
         const bool uni = kv.page_size % 16 == 0;
+        a.q_runs = kv.head_dim % e == 0 && d->q_stride % e == 0 && aligned16(q);
         const dim3 grid((unsigned)blocks);
         if (kv.head_dim <= 64) launch_attend<T, 64>(a, vec, uni, grid, st);
         else if (kv.head_dim <= 128) launch_attend<T, 128>(a, vec, uni, grid, st);
