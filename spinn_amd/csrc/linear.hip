@@ -10,8 +10,9 @@
 //    16 MT x 16 NT, K spread over a workgroup's waves, operands straight from memory into
 //    registers, the waves' sums joined in LDS in wave order.
 //  * many rows: the matrix cores bound it. linear_tile_kernel: both operands through LDS, whole
-//    fragments copied there without passing registers, two stages.
+//    fragments copied there without passing registers, four of them along K.
 #include "decode.h"
+#include <type_traits>
 
 namespace spinn {
 namespace {
@@ -30,70 +31,101 @@ inline bool x_loose(const SpinnHipLinearDesc *d) {
     return d->x_unaligned || d->ldx % e || d->k % e;
 }
 
-__device__ __forceinline__ float gelu_erf(float v) { return 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); }
+// v Phi(v) with erfc by Abramowitz and Stegun 7.1.26 (|error| < 1.5e-7 of 1, so under 1e-7 |v| here, against
+// 6e-8 |v| for a correctly rounded erf): a dozen instructions for the library's forty, in an epilogue
+// that is unrolled over up to 128 values.
+__device__ __forceinline__ float gelu_erf(float v) {
+    const float x = fabsf(v) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    const float p = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+    const float half = 0.5f * t * p * __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f); // erfc(x) / 2
+    return v * (v < 0.f ? half : 1.f - half);
+}
 // v/2 (1 + tanh u) = v / (1 + exp(-2u))
 __device__ __forceinline__ float gelu_tanh(float v) {
     const float u = 0.7978845608028654f * (v + 0.044715f * v * v * v);
     return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * (-2.f * 1.4426950408889634f)));
 }
-__device__ __forceinline__ float linear_act(float v, int act) {
+template <int ACT>
+__device__ __forceinline__ float linear_act(float v) {
+    if constexpr (ACT == SPINN_LINEAR_RELU) return v < 0.f ? 0.f : v;
+    else if constexpr (ACT == SPINN_LINEAR_SILU) return silu(v);
+    else if constexpr (ACT == SPINN_LINEAR_GELU) return gelu_erf(v);
+    else if constexpr (ACT == SPINN_LINEAR_GELU_TANH) return gelu_tanh(v);
+    else return v;
+}
+// f(integral_constant<activation>)
+template <class F>
+__device__ __forceinline__ void with_act(int act, F f) {
     switch (act) {
-    case SPINN_LINEAR_RELU: return v < 0.f ? 0.f : v;
-    case SPINN_LINEAR_SILU: return silu(v);
-    case SPINN_LINEAR_GELU: return gelu_erf(v);
-    case SPINN_LINEAR_GELU_TANH: return gelu_tanh(v);
-    default: return v;
+    case SPINN_LINEAR_RELU: f(std::integral_constant<int, SPINN_LINEAR_RELU>()); break;
+    case SPINN_LINEAR_SILU: f(std::integral_constant<int, SPINN_LINEAR_SILU>()); break;
+    case SPINN_LINEAR_GELU: f(std::integral_constant<int, SPINN_LINEAR_GELU>()); break;
+    case SPINN_LINEAR_GELU_TANH: f(std::integral_constant<int, SPINN_LINEAR_GELU_TANH>()); break;
+    default: f(std::integral_constant<int, SPINN_LINEAR_NONE>()); break;
     }
 }
 
 struct LinearArgs {
-    const void *x, *bias, *res; // x: rows, or fragments [M/16][frags]
+    const void *x, *bias, *res; // x: rows, or granules [M/16][frags/2]
     const char *w;              // packed
     void *y;
     int64_t ldx, ldres, ldy;
     int32_t m, n, k, act;
     int32_t kf;      // fragments along K
     int32_t ntiles;  // of 16 columns
-    int32_t vec;     // residual and y are read and written in runs of 4
+    int32_t vec;     // rows of residual and y are whole runs of 16 bytes
 };
 
-// Four neighbouring columns n.. of a row.
-template <class T>
-__device__ __forceinline__ void finish4(const LinearArgs &a, int row, int n, f32x4 v) {
-    if (row >= a.m || n >= a.n) return;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const int64_t ry = (int64_t)row * a.ldy + n, rr = (int64_t)row * a.ldres + n;
-    if (a.vec && n + 3 < a.n) {
-        if (a.bias) {
-            const T *b = (const T *)a.bias + n;
+// C neighbouring columns n.. of a row: bias and residual as they are in memory, the sum, the activation, the result.
+// Loads and stores are 16-byte runs where all C columns exist and the rows allow it, else element by element.
+template <class T, int C>
+struct Columns {
+    static_assert(C * sizeof(T) % 8 == 0, "");
+    typedef T Run __attribute__((ext_vector_type(C)));
+    typedef float Sum __attribute__((ext_vector_type(C)));
+    static constexpr int kAlign = C * sizeof(T) < 16 ? C * sizeof(T) : 16;
+    typedef Run AlignedRun __attribute__((aligned(kAlign)));
+    __device__ __forceinline__ static Run load(const T *p, int left, bool runs) {
+        Run r;
+        if (runs && left >= C) {
+            r = *reinterpret_cast<const AlignedRun *>(p);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += (float)b[i];
+            for (int i = 0; i < C; ++i) r[i] = i < left ? p[i] : (T)0.f;
         }
-        if (a.res) {
-            const T4 r = *reinterpret_cast<const T4 *>((const T *)a.res + rr);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += (float)r[i];
-        }
-        T4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = (T)linear_act(v[i], a.act);
-        *reinterpret_cast<T4 *>((T *)a.y + ry) = o;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < a.n) {
-                float s = v[i];
-                if (a.bias) s += (float)((const T *)a.bias)[n + i];
-                if (a.res) s += (float)((const T *)a.res)[rr + i];
-                ((T *)a.y)[ry + i] = (T)linear_act(s, a.act);
-            }
+        return r;
     }
-}
+    template <int ACT>
+    __device__ __forceinline__ static void store(T *p, int left, bool runs, Sum v) {
+        Run r;
+#pragma unroll
+        for (int i = 0; i < C; ++i) r[i] = (T)linear_act<ACT>(v[i]);
+        if (runs && left >= C) {
+            *reinterpret_cast<AlignedRun *>(p) = r;
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (i < left) p[i] = r[i];
+        }
+    }
+};
 
 // First column of the four that accumulator block `tile` of a lane with l/16 = g holds.
 __device__ __forceinline__ int first_col(int tile, int g) { return (tile >> 2) * 64 + 16 * g + 4 * (tile & 3); }
 
-// XP: x is laid out as fragments.
+// x goes to LDS in granules of 16 rows by two fragments, 128 bytes (a cache line) of every row: row r's eight
+// 16-byte runs at 128 r, run c in place c ^ (r / 2), so that the 16 lanes that read run c of 16 rows at once
+// meet all banks. (64-byte pieces of rows, a fragment at a time, ask the L2 for every line twice:
+// 348 against 275 us for the whole 4096 x 8192 x 4096 product.)
+constexpr int kGranule = 2 * kFragBytes;
+// Byte of the run that operand lane `lane` reads for the granule's fragment `half`.
+__device__ __forceinline__ int granule_at(int lane, int half) {
+    const int r = lane & 15, c = half * 4 + (lane >> 4);
+    return r * 128 + ((c ^ (r >> 1)) << 4);
+}
+
+// XP: x is laid out as granules.
 template <class T, int MT, int NT, int NW, bool XP>
 __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
     constexpr int E = 16 / (int)sizeof(T);
@@ -108,7 +140,7 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
     for (int i = 0; i < MT; ++i) {
         if constexpr (XP) {
             const int mt = min(m0 + i, (a.m - 1) >> 4);
-            xp[i] = (const char *)a.x + (int64_t)mt * a.kf * kFragBytes + lane * 16;
+            xp[i] = (const char *)a.x + (int64_t)mt * a.kf * kFragBytes;
         } else {
             const int row = min((m0 + i) * 16 + (lane & 15), a.m - 1);
             xp[i] = (const char *)((const T *)a.x + (int64_t)row * a.ldx + (lane >> 4) * E);
@@ -125,7 +157,7 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
             for (int j = 0; j < NT; ++j) w[u][j] = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)f * kFragBytes);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if constexpr (XP) x[u][i] = *reinterpret_cast<const u32x4 *>(xp[i] + (int64_t)f * kFragBytes);
+                if constexpr (XP) x[u][i] = *reinterpret_cast<const u32x4 *>(xp[i] + (int64_t)(f >> 1) * kGranule + granule_at(lane, f & 1));
                 else {
                     const bool in = f * kFrag<T> + (lane >> 4) * E < a.k;
                     x[u][i] = in ? *reinterpret_cast<const u32x4 *>(xp[i] + (int64_t)f * 64) : (u32x4){0, 0, 0, 0};
@@ -146,102 +178,220 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int b = wave; b < MT * NT; b += NW) {
-        f32x4 v = part[0][b][lane];
+    // a wave finishes every NW-th block; what it adds is on its way while the others' sums come together
+    constexpr int B = (MT * NT + NW - 1) / NW;
+    typedef Columns<T, 4> Col;
+    typename Col::Run bias[B], res[B];
+    int rows[B], cols[B], left[B];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) v += part[w][b][lane];
-        const int i = b / NT, j = b % NT;
-        if (t0 + j < a.ntiles) finish4<T>(a, (m0 + i) * 16 + (lane & 15), first_col(t0 + j, lane >> 4), v);
+    for (int k = 0; k < B; ++k) {
+        const int b = wave + k * NW, tile = t0 + b % NT;
+        rows[k] = (m0 + b / NT) * 16 + (lane & 15);
+        cols[k] = first_col(tile, lane >> 4);
+        left[k] = b < MT * NT && tile < a.ntiles && rows[k] < a.m ? a.n - cols[k] : 0;
+        if (left[k] > 0) {
+            if (a.bias) bias[k] = Col::load((const T *)a.bias + cols[k], left[k], false);
+            if (a.res) res[k] = Col::load((const T *)a.res + (int64_t)rows[k] * a.ldres + cols[k], left[k], a.vec);
+        }
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < B; ++k)
+        if (left[k] > 0) {
+            const int b = wave + k * NW;
+            f32x4 v = part[0][b][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v += part[w][b][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (a.bias) v[i] += (float)bias[k][i];
+                if (a.res) v[i] += (float)res[k][i];
+            }
+            T *y = (T *)a.y + (int64_t)rows[k] * a.ldy + cols[k];
+            with_act(a.act, [&](auto act) { Col::template store<decltype(act)::value>(y, left[k], a.vec, v); });
+        }
 }
 
 __device__ __forceinline__ void copy_to_lds(const char *src, char *lds) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
                                      (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
+// All but this wave's last `LEFT` copies have landed, its LDS reads are done, and so are every other wave's.
+template <int LEFT>
+__device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
 
-// BM x BN of y per workgroup of WVM x WVN waves.
+// BM x BN of y per workgroup of WVM x WVN waves. LDS holds three granules of x and four fragments of w along K:
+// while fragment f is computed, the reads of f + 1 go to registers (x's as each is used up), and
+// f + 2 .. f + 4 are on their way from memory. One barrier per fragment.
 template <class T, int BM, int BN, int WVM, int WVN, bool XP>
-__global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs a, int mblocks) {
+__global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs a, int mblocks, int nblocks) {
     constexpr int E = 16 / (int)sizeof(T);
     constexpr int NW = WVM * WVN;
-    constexpr int TM = BM / WVM / 16, TN = BN / WVN / 16; // a wave's blocks
-    constexpr int S = 2;                                  // fragments along K per stage
-    constexpr int FX = BM / 16 * S, FW = BN / 16 * S;     // fragments of a stage
-    constexpr int PW = (FX + FW) / NW;                    // a wave's share of the copies
-    static_assert((FX + FW) % NW == 0 && FX % PW == 0, "a wave copies fragments of one operand");
-    __shared__ __attribute__((aligned(16))) char lds[2][(FX + FW) * kFragBytes];
+    constexpr int TM = BM / WVM / 16, TN = BN / WVN / 16;  // a wave's blocks
+    constexpr int PX = BM / 16 * 2 / NW, PW = BN / 16 / NW; // a wave's 1 KB copies of a granule and of a fragment
+    static_assert(BM / 16 * 2 % NW == 0 && BN / 16 % NW == 0, "");
+    constexpr int kX = BM / 16 * kGranule, kW = BN / 16 * kFragBytes;
+    __shared__ __attribute__((aligned(16))) char lds[3 * kX + 4 * kW];
+    char *const ldw = lds + 3 * kX;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int bm = blockIdx.x % mblocks, bn = blockIdx.x / mblocks;
+    // workgroup b runs on XCD b % 8: an XCD takes neighbouring tiles, columns of 4 tiles high, so that
+    // its CUs share rows of x and of w in its L2
+    int bm, bn;
+    {
+        const int tiles = mblocks * nblocks, q = tiles / 8, r = tiles % 8, x = blockIdx.x % 8;
+        const int id = x * q + min(x, r) + (int)blockIdx.x / 8;
+        constexpr int G = 4;
+        const int group = id / (G * nblocks), high = min(G, mblocks - group * G);
+        const int in = id - group * G * nblocks;
+        bm = group * G + in % high;
+        bn = in / high;
+    }
     const int mt0 = bm * (BM / 16), nt0 = bn * (BN / 16);
 
-    // fragment c of a stage: x's first, [tile][s]
-    const char *src[PW];
-    const bool wx = wave * PW < FX;
+    // copy p of a granule: eight rows, lane l run l % 8 of row l / 8 as it lies in LDS
+    const char *xs[PX];
+    int run[PX]; // first k of the lane's run in a granule
 #pragma unroll
-    for (int p = 0; p < PW; ++p) {
-        const int c = wave * PW + p;
-        if (wx) {
-            if constexpr (XP) {
-                const int mt = min(mt0 + c / S, (a.m - 1) >> 4);
-                src[p] = (const char *)a.x + ((int64_t)mt * a.kf + c % S) * kFragBytes + lane * 16;
-            } else {
-                const int row = min((mt0 + c / S) * 16 + (lane & 15), a.m - 1);
-                src[p] = (const char *)((const T *)a.x + (int64_t)row * a.ldx + (c % S) * kFrag<T> + (lane >> 4) * E);
-            }
+    for (int p = 0; p < PX; ++p) {
+        const int c = wave * PX + p, r = (c & 1) * 8 + (lane >> 3);
+        run[p] = ((lane & 7) ^ (r >> 1)) * E;
+        if constexpr (XP) {
+            const int mt = min(mt0 + (c >> 1), (a.m - 1) >> 4);
+            xs[p] = (const char *)a.x + (int64_t)mt * a.kf * kFragBytes + (c & 1) * kFragBytes + lane * 16;
         } else {
-            const int nt = min(nt0 + (c - FX) / S, a.ntiles - 1);
-            src[p] = a.w + ((int64_t)nt * a.kf + (c - FX) % S) * kFragBytes + lane * 16;
+            const int row = min((mt0 + (c >> 1)) * 16 + r, a.m - 1);
+            xs[p] = (const char *)((const T *)a.x + (int64_t)row * a.ldx + run[p]);
         }
     }
-    const char *zeros = a.w + (int64_t)a.ntiles * a.kf * kFragBytes;
-    auto fetch = [&](int f, int buf) {
+    const char *ws[PW];
 #pragma unroll
-        for (int p = 0; p < PW; ++p) {
-            const int c = wave * PW + p;
-            const char *s;
-            if (wx && !XP) {
-                // runs behind a row's end come from the packed weights' zeros
-                const bool in = (f + c % S) * kFrag<T> + (lane >> 4) * E < a.k;
-                s = in ? src[p] + (int64_t)f * 64 : zeros;
-            } else {
-                s = src[p] + (int64_t)f * kFragBytes;
-            }
-            copy_to_lds(s, lds[buf] + c * kFragBytes);
+    for (int p = 0; p < PW; ++p) {
+        const int nt = min(nt0 + wave * PW + p, a.ntiles - 1);
+        ws[p] = a.w + (int64_t)nt * a.kf * kFragBytes + lane * 16;
+    }
+    const char *zeros = a.w + (int64_t)a.ntiles * a.kf * kFragBytes;
+    auto fetch_x = [&](int g, int place) { // granule g
+        char *to = lds + place * kX + wave * PX * kFragBytes;
+        if (XP || (g + 1) * 2 * kFrag<T> <= a.k) {
+#pragma unroll
+            for (int p = 0; p < PX; ++p) copy_to_lds(xs[p] + (int64_t)g * (XP ? kGranule : 128), to + p * kFragBytes);
+        } else { // the runs behind a row's end come from the packed weights' zeros
+#pragma unroll
+            for (int p = 0; p < PX; ++p)
+                copy_to_lds(g * 2 * kFrag<T> + run[p] < a.k ? xs[p] + (int64_t)g * 128 : zeros, to + p * kFragBytes);
         }
+    };
+    auto fetch_w = [&](int f) {
+        char *to = ldw + (f & 3) * kW + wave * PW * kFragBytes;
+#pragma unroll
+        for (int p = 0; p < PW; ++p) copy_to_lds(ws[p] + (int64_t)f * kFragBytes, to + p * kFragBytes);
     };
 
     const int wm = wave % WVM, wn = wave / WVM;
+    const char *const lx[2] = {lds + wm * TM * kGranule + granule_at(lane, 0), lds + wm * TM * kGranule + granule_at(lane, 1)};
+    const char *const lw = ldw + wn * TN * kFragBytes + lane * 16;
+    auto read = [&](const char *p) { return *reinterpret_cast<const u32x4 *>(p); };
     f32x4 acc[TM][TN] = {};
-    fetch(0, 0);
-    for (int f = 0, buf = 0; f < a.kf; f += S, buf ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0x0f70); // vmcnt(0): this wave's copies have landed
-        __syncthreads();                    // everyone's have, and the other buffer has been read
-        if (f + S < a.kf) fetch(f + S, buf ^ 1);
-        const char *lx = lds[buf] + (wm * TM * S) * kFragBytes + lane * 16;
-        const char *lw = lds[buf] + (FX + wn * TN * S) * kFragBytes + lane * 16;
+    u32x4 x[TM], w[2][TN];
+
+    const int kf = a.kf; // even
+    fetch_x(0, 0);
+    fetch_w(0);
+    if (kf > 2) fetch_x(1, 1);
+    fetch_w(1);
+    if (kf > 2) fetch_w(2);
+    if (kf > 4) fetch_x(2, 2);
+    if (kf > 2) fetch_w(3);
+    if (kf > 4) stage_ready<2 * PX + 3 * PW>();
+    else stage_ready<0>();
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            u32x4 x[TM], w[TN];
+    for (int j = 0; j < TN; ++j) w[0][j] = read(lw + j * kFragBytes);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) w[j] = *reinterpret_cast<const u32x4 *>(lw + (j * S + s) * kFragBytes);
+    for (int i = 0; i < TM; ++i) x[i] = read(lx[0] + i * kGranule);
+    // One fragment f, half = f % 2. x's granule is in place `here`, the next one in `next`; every wave has read fragment f, so
+    // its place takes f + 4, and an odd one's granule the third after it.
+    auto step = [&](int f, auto half_, int here, int next) {
+        constexpr int half = decltype(half_)::value;
+        const bool more = f + 1 < kf;
+        // copies since fragment f + 1 was asked for: w of f + 2, f + 3, and one granule of x
+        if (f + 4 < kf) stage_ready<PX + 2 * PW>();
+        else if (more) stage_ready<0>();
+        if (half && f + 5 < kf) fetch_x(f / 2 + 3, here);
+        if (f + 4 < kf) fetch_w(f + 4);
+        const char *px = half ? lx[0] + next * kX : lx[1] + here * kX;
+        if (more) {
+            const char *pw = lw + ((f + 1) & 3) * kW;
 #pragma unroll
-            for (int i = 0; i < TM; ++i) x[i] = *reinterpret_cast<const u32x4 *>(lx + (i * S + s) * kFragBytes);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) mfma_frag(acc[i][j], w[j], x[i], T());
+            for (int j = 0; j < TN; ++j) w[!half][j] = read(pw + j * kFragBytes);
         }
+        if constexpr (sizeof(T) == 4) { // neighbouring instructions on different accumulators
+            constexpr int I = 2;
+#pragma unroll
+            for (int i0 = 0; i0 < TM; i0 += I) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = i0; i < i0 + I; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __builtin_bit_cast(float, (uint32_t)w[half][j][e]),
+                                __builtin_bit_cast(float, (uint32_t)x[i][e]), acc[i][j], 0, 0, 0);
+                if (more) {
+#pragma unroll
+                    for (int i = i0; i < i0 + I; ++i) x[i] = read(px + i * kGranule);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) mfma_frag(acc[i][j], w[half][j], x[i], T());
+                if (more) x[i] = read(px + i * kGranule);
+            }
+        }
+    };
+    for (int f = 0, here = 0; f < kf; f += 2) {
+        const int next = here == 2 ? 0 : here + 1;
+        step(f, std::integral_constant<int, 0>(), here, next);
+        step(f + 1, std::integral_constant<int, 1>(), here, next);
+        here = next;
     }
+    // a lane's blocks of a row are 16 neighbouring columns; residuals of R rows travel at a time
+    static_assert(TN == 4 && TM % 4 == 0, "");
+    constexpr int R = 4;
+    typedef Columns<T, 16> Col;
+    const int col = first_col(nt0 + wn * TN, lane >> 4), left = a.n - col;
+    if (left <= 0) return;
+    typename Col::Run bias;
+    if (a.bias) bias = Col::load((const T *)a.bias + col, left, false);
+    with_act(a.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+        for (int i0 = 0; i0 < TM; i0 += R) {
+            const int row0 = (mt0 + wm * TM + i0) * 16 + (lane & 15);
+            typename Col::Run res[R];
+            if (a.res) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int tile = nt0 + wn * TN + j;
-            if (tile < a.ntiles)
-                finish4<T>(a, (mt0 + wm * TM + i) * 16 + (lane & 15), first_col(tile, lane >> 4), acc[i][j]);
+                for (int i = 0; i < R; ++i)
+                    if (row0 + 16 * i < a.m)
+                        res[i] = Col::load((const T *)a.res + (int64_t)(row0 + 16 * i) * a.ldres + col, left, a.vec);
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                typename Col::Sum v;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    v[c] = acc[i0 + i][c / 4][c % 4];
+                    if (a.bias) v[c] += (float)bias[c];
+                    if (a.res) v[c] += (float)res[i][c];
+                }
+                if (row0 + 16 * i < a.m)
+                    Col::template store<decltype(act)::value>((T *)a.y + (int64_t)(row0 + 16 * i) * a.ldy + col, left, a.vec, v);
+            }
         }
+    });
 }
 
 // One thread per 16 bytes of the packed weights, and of a fragment of zeros behind them.
@@ -272,7 +422,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T *__restrict__ 
     }
 }
 
-// x as fragments [M/16][kf][64][16 bytes], zeros behind its rows and columns.
+// x as granules [M/16][kf/2][2 KB], zeros behind its rows and columns; one thread per 16 bytes.
 template <class T>
 __global__ __launch_bounds__(256) void linear_pack_x_kernel(const T *__restrict__ x, u32x4 *__restrict__ out, int m, int k,
                                                             int64_t ldx, int64_t kf, int64_t total) {
@@ -280,10 +430,9 @@ __global__ __launch_bounds__(256) void linear_pack_x_kernel(const T *__restrict_
     typedef typename Bits<T>::type B;
     const B *xb = reinterpret_cast<const B *>(x);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int lane = (int)(i & 63);
-        const int64_t frag = i >> 6;
-        const int64_t tile = frag / kf, f = frag - tile * kf;
-        const int64_t row = tile * 16 + (lane & 15), k0 = f * kFrag<T> + (lane >> 4) * E;
+        const int in = (int)(i & 127), r = in >> 3;
+        const int64_t granule = i >> 7, tile = granule / (kf / 2), g = granule - tile * (kf / 2);
+        const int64_t row = tile * 16 + r, k0 = g * 2 * kFrag<T> + ((in & 7) ^ (r >> 1)) * E;
         u32x4 v = {0, 0, 0, 0};
         if (row < m) {
 #pragma unroll
@@ -308,8 +457,8 @@ void launch_stream(const LinearArgs &a, bool xp, hipStream_t st) {
 template <class T, int BM, int BN, int WVM, int WVN>
 void launch_tile(const LinearArgs &a, bool xp, hipStream_t st) {
     const int mb = (a.m + BM - 1) / BM, nb = (a.ntiles * 16 + BN - 1) / BN;
-    if (xp) linear_tile_kernel<T, BM, BN, WVM, WVN, true><<<mb * nb, 64 * WVM * WVN, 0, st>>>(a, mb);
-    else linear_tile_kernel<T, BM, BN, WVM, WVN, false><<<mb * nb, 64 * WVM * WVN, 0, st>>>(a, mb);
+    if (xp) linear_tile_kernel<T, BM, BN, WVM, WVN, true><<<mb * nb, 64 * WVM * WVN, 0, st>>>(a, mb, nb);
+    else linear_tile_kernel<T, BM, BN, WVM, WVN, false><<<mb * nb, 64 * WVM * WVN, 0, st>>>(a, mb, nb);
 }
 
 } // namespace
@@ -349,8 +498,8 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
     a.act = d->act;
     a.kf = (int32_t)frags(d);
     a.ntiles = (int32_t)n_tiles(d);
-    const size_t run = 4 * (size_t)dtype_bytes(d->dtype);
-    a.vec = (uintptr_t)y % run == 0 && d->ldy % 4 == 0 && (!res || ((uintptr_t)res % run == 0 && d->ldres % 4 == 0));
+    const int per = 16 / dtype_bytes(d->dtype);
+    a.vec = aligned16(y) && d->ldy % per == 0 && (!res || (aligned16(res) && d->ldres % per == 0));
     const bool xp = x_loose(d);
     const int64_t wgs = (int64_t)((d->m + 63) / 64) * (a.ntiles / 4);
     if (wgs > INT32_MAX / 4 || (d->m + 15) / 16 > 65535 * 4) return SPINN_HIP_EUNSUPPORTED;
