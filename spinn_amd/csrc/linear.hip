@@ -222,26 +222,68 @@ __device__ __forceinline__ void stage_ready() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-// BM x BN of y per workgroup of WVM x WVN waves. LDS holds three granules of x and four fragments of w along K:
-// while fragment f is computed, the reads of f + 1 go to registers (x's as each is used up), and
-// f + 2 .. f + 4 are on their way from memory. One barrier per fragment.
-template <class T, int BM, int BN, int WVM, int WVN, bool XP>
-__global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs a, int mblocks, int nblocks) {
+// A lane's sums of TM rows of blocks, 16 neighbouring columns of a row each, to y.
+template <class T, int TM>
+__device__ __forceinline__ void finish_rows(const LinearArgs &a, int row0, int col, const f32x4 (&acc)[TM][4]) {
+    typedef Columns<T, 16> Col;
+    constexpr int R = TM < 4 ? TM : 4; // rows whose residuals travel at a time
+    static_assert(TM % R == 0, "");
+    const int left = a.n - col;
+    if (left <= 0) return;
+    typename Col::Run bias;
+    if (a.bias) bias = Col::load((const T *)a.bias + col, left, false);
+    with_act(a.act, [&](auto act) {
+#pragma unroll
+        for (int i0 = 0; i0 < TM; i0 += R) {
+            const int row = row0 + 16 * i0;
+            typename Col::Run res[R];
+            if (a.res) {
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+                    if (row + 16 * i < a.m)
+                        res[i] = Col::load((const T *)a.res + (int64_t)(row + 16 * i) * a.ldres + col, left, a.vec);
+            }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                typename Col::Sum v;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    v[c] = acc[i0 + i][c / 4][c % 4];
+                    if (a.bias) v[c] += (float)bias[c];
+                    if (a.res) v[c] += (float)res[i][c];
+                }
+                if (row + 16 * i < a.m)
+                    Col::template store<decltype(act)::value>((T *)a.y + (int64_t)(row + 16 * i) * a.ldy + col, left, a.vec, v);
+            }
+        }
+    });
+}
+
+// BM x BN of y per workgroup of WVM x WVN waves, wave tiles 64 columns wide. LDS holds WF fragments of w along K
+// and WF / 2 + 1 granules of x: while fragment f is computed, the reads of f + 1 go to registers (x's
+// as each is used up), and f + 2 .. f + WF are on their way from memory. One barrier per fragment.
+// `splits` > 1: a workgroup takes its share of K and leaves its sums in part[split][tile][block][lane].
+template <class T, int BM, int BN, int WVM, int WVN, int WF, bool XP>
+__global__ __launch_bounds__(64 * WVM * WVN, 2) void linear_tile_kernel(LinearArgs a, int mblocks, int nblocks, int splits,
+                                                                     f32x4 *part) {
     constexpr int E = 16 / (int)sizeof(T);
     constexpr int NW = WVM * WVN;
-    constexpr int TM = BM / WVM / 16, TN = BN / WVN / 16;  // a wave's blocks
+    constexpr int TM = BM / WVM / 16, TN = BN / WVN / 16;   // a wave's blocks
     constexpr int PX = BM / 16 * 2 / NW, PW = BN / 16 / NW; // a wave's 1 KB copies of a granule and of a fragment
-    static_assert(BM / 16 * 2 % NW == 0 && BN / 16 % NW == 0, "");
+    static_assert(BM / 16 * 2 % NW == 0 && BN / 16 % NW == 0 && TN == 4 && (WF & (WF - 1)) == 0, "");
+    constexpr int GX = WF / 2 + 1;
     constexpr int kX = BM / 16 * kGranule, kW = BN / 16 * kFragBytes;
-    __shared__ __attribute__((aligned(16))) char lds[3 * kX + 4 * kW];
-    char *const ldw = lds + 3 * kX;
+    __shared__ __attribute__((aligned(16))) char lds[GX * kX + WF * kW];
+    char *const ldw = lds + GX * kX;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // workgroup b runs on XCD b % 8: an XCD takes neighbouring tiles, columns of 4 tiles high, so that
     // its CUs share rows of x and of w in its L2
-    int bm, bn;
+    int bm, bn, split, id;
     {
-        const int tiles = mblocks * nblocks, q = tiles / 8, r = tiles % 8, x = blockIdx.x % 8;
-        const int id = x * q + min(x, r) + (int)blockIdx.x / 8;
+        const int tiles = mblocks * nblocks, total = tiles * splits, q = total / 8, r = total % 8, x = blockIdx.x % 8;
+        id = x * q + min(x, r) + (int)blockIdx.x / 8;
+        split = id / tiles;
+        id -= split * tiles;
         constexpr int G = 4;
         const int group = id / (G * nblocks), high = min(G, mblocks - group * G);
         const int in = id - group * G * nblocks;
@@ -249,17 +291,20 @@ __global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs 
         bn = in / high;
     }
     const int mt0 = bm * (BM / 16), nt0 = bn * (BN / 16);
+    // this split's granules along K
+    const int g0 = (int)((int64_t)(a.kf / 2) * split / splits), g1 = (int)((int64_t)(a.kf / 2) * (split + 1) / splits);
+    const int kf = 2 * (g1 - g0); // at least 2
 
     // copy p of a granule: eight rows, lane l run l % 8 of row l / 8 as it lies in LDS
     const char *xs[PX];
-    int run[PX]; // first k of the lane's run in a granule
+    int run[PX]; // first k of the lane's run in granule 0
 #pragma unroll
     for (int p = 0; p < PX; ++p) {
         const int c = wave * PX + p, r = (c & 1) * 8 + (lane >> 3);
-        run[p] = ((lane & 7) ^ (r >> 1)) * E;
+        run[p] = g0 * 2 * kFrag<T> + ((lane & 7) ^ (r >> 1)) * E;
         if constexpr (XP) {
             const int mt = min(mt0 + (c >> 1), (a.m - 1) >> 4);
-            xs[p] = (const char *)a.x + (int64_t)mt * a.kf * kFragBytes + (c & 1) * kFragBytes + lane * 16;
+            xs[p] = (const char *)a.x + ((int64_t)mt * a.kf + 2 * g0) * kFragBytes + (c & 1) * kFragBytes + lane * 16;
         } else {
             const int row = min((mt0 + (c >> 1)) * 16 + r, a.m - 1);
             xs[p] = (const char *)((const T *)a.x + (int64_t)row * a.ldx + run[p]);
@@ -269,12 +314,12 @@ __global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs 
 #pragma unroll
     for (int p = 0; p < PW; ++p) {
         const int nt = min(nt0 + wave * PW + p, a.ntiles - 1);
-        ws[p] = a.w + (int64_t)nt * a.kf * kFragBytes + lane * 16;
+        ws[p] = a.w + ((int64_t)nt * a.kf + 2 * g0) * kFragBytes + lane * 16;
     }
     const char *zeros = a.w + (int64_t)a.ntiles * a.kf * kFragBytes;
-    auto fetch_x = [&](int g, int place) { // granule g
+    auto fetch_x = [&](int g, int place, bool whole) { // granule g of the split's; whole: it does not pass the rows' end
         char *to = lds + place * kX + wave * PX * kFragBytes;
-        if (XP || (g + 1) * 2 * kFrag<T> <= a.k) {
+        if (XP || whole || (g0 + g + 1) * 2 * kFrag<T> <= a.k) {
 #pragma unroll
             for (int p = 0; p < PX; ++p) copy_to_lds(xs[p] + (int64_t)g * (XP ? kGranule : 128), to + p * kFragBytes);
         } else { // the runs behind a row's end come from the packed weights' zeros
@@ -284,7 +329,7 @@ __global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs 
         }
     };
     auto fetch_w = [&](int f) {
-        char *to = ldw + (f & 3) * kW + wave * PW * kFragBytes;
+        char *to = ldw + (f & (WF - 1)) * kW + wave * PW * kFragBytes;
 #pragma unroll
         for (int p = 0; p < PW; ++p) copy_to_lds(ws[p] + (int64_t)f * kFragBytes, to + p * kFragBytes);
     };
@@ -296,33 +341,34 @@ __global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs 
     f32x4 acc[TM][TN] = {};
     u32x4 x[TM], w[2][TN];
 
-    const int kf = a.kf; // even
-    fetch_x(0, 0);
-    fetch_w(0);
-    if (kf > 2) fetch_x(1, 1);
-    fetch_w(1);
-    if (kf > 2) fetch_w(2);
-    if (kf > 4) fetch_x(2, 2);
-    if (kf > 2) fetch_w(3);
-    if (kf > 4) stage_ready<2 * PX + 3 * PW>();
+    // In the order of the steps before the first: x of a granule, then w, every odd step a granule.
+    fetch_x(0, 0, false);
+#pragma unroll
+    for (int s = 0; s < WF; ++s) {
+        if (s % 2 && s + 1 < kf) fetch_x((s + 1) / 2, (s + 1) / 2, false);
+        if (s < kf) fetch_w(s);
+    }
+    if (kf > WF) stage_ready<WF / 2 * PX + (WF - 1) * PW>();
     else stage_ready<0>();
 #pragma unroll
     for (int j = 0; j < TN; ++j) w[0][j] = read(lw + j * kFragBytes);
 #pragma unroll
     for (int i = 0; i < TM; ++i) x[i] = read(lx[0] + i * kGranule);
-    // One fragment f, half = f % 2. x's granule is in place `here`, the next one in `next`; every wave has read fragment f, so
-    // its place takes f + 4, and an odd one's granule the third after it.
-    auto step = [&](int f, auto half_, int here, int next) {
+    // One fragment f, half = f % 2. x's granule is in place `here`, the one after it in `next`; every wave has read fragment
+    // f, so its place takes f + WF, and an odd one's granule the GX-th after it.
+    // steady: all that a step asks for is there, and not the last granule (no branches in the loop)
+    auto step = [&](int f, auto half_, auto steady_, int here, int next) {
         constexpr int half = decltype(half_)::value;
-        const bool more = f + 1 < kf;
-        // copies since fragment f + 1 was asked for: w of f + 2, f + 3, and one granule of x
-        if (f + 4 < kf) stage_ready<PX + 2 * PW>();
+        constexpr bool steady = decltype(steady_)::value;
+        const bool more = steady || f + 1 < kf;
+        // copies since fragment f + 1 was asked for: w of f + 2 .. f + WF - 1, and a granule for every two
+        if (steady || f + WF < kf) stage_ready<(WF - 2) / 2 * PX + (WF - 2) * PW>();
         else if (more) stage_ready<0>();
-        if (half && f + 5 < kf) fetch_x(f / 2 + 3, here);
-        if (f + 4 < kf) fetch_w(f + 4);
+        if (half && (steady || f + WF + 1 < kf)) fetch_x(f / 2 + GX, here, steady);
+        if (steady || f + WF < kf) fetch_w(f + WF);
         const char *px = half ? lx[0] + next * kX : lx[1] + here * kX;
         if (more) {
-            const char *pw = lw + ((f + 1) & 3) * kW;
+            const char *pw = lw + ((f + 1) & (WF - 1)) * kW;
 #pragma unroll
             for (int j = 0; j < TN; ++j) w[!half][j] = read(pw + j * kFragBytes);
         }
@@ -353,45 +399,48 @@ __global__ __launch_bounds__(64 * WVM * WVN) void linear_tile_kernel(LinearArgs 
             }
         }
     };
-    for (int f = 0, here = 0; f < kf; f += 2) {
-        const int next = here == 2 ? 0 : here + 1;
-        step(f, std::integral_constant<int, 0>(), here, next);
-        step(f + 1, std::integral_constant<int, 1>(), here, next);
+    int f = 0, here = 0;
+    auto pair = [&](auto steady) {
+        const int next = here == GX - 1 ? 0 : here + 1;
+        step(f, std::integral_constant<int, 0>(), steady, here, next);
+        step(f + 1, std::integral_constant<int, 1>(), steady, here, next);
         here = next;
+        f += 2;
+    };
+    while (f + WF + 4 < kf) pair(std::true_type());
+    while (f < kf) pair(std::false_type());
+    if (splits > 1) {
+        f32x4 *to = part + (((int64_t)split * mblocks * nblocks + id) * NW + wave) * (TM * TN) * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) to[(i * TN + j) * 64] = acc[i][j];
+        return;
     }
-    // a lane's blocks of a row are 16 neighbouring columns; residuals of R rows travel at a time
-    static_assert(TN == 4 && TM % 4 == 0, "");
-    constexpr int R = 4;
-    typedef Columns<T, 16> Col;
-    const int col = first_col(nt0 + wn * TN, lane >> 4), left = a.n - col;
-    if (left <= 0) return;
-    typename Col::Run bias;
-    if (a.bias) bias = Col::load((const T *)a.bias + col, left, false);
-    with_act(a.act, [&](auto act) {
+    finish_rows<T, TM>(a, (mt0 + wm * TM) * 16 + (lane & 15), first_col(nt0 + wn * TN, lane >> 4), acc);
+}
+
+// The splits' sums of one row of blocks of a wave's tile, added in split order. One wave each.
+template <class T, int BM, int BN, int WVM, int WVN>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int mblocks, int nblocks, int splits,
+                                                          const f32x4 *part) {
+    constexpr int NW = WVM * WVN, TM = BM / WVM / 16;
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); // (tile, wave, block row)
+    const int64_t tiles = (int64_t)mblocks * nblocks;
+    if (unit >= tiles * NW * TM) return;
+    const int id = (int)(unit / (NW * TM)), wave = (int)(unit / TM % NW), i = (int)(unit % TM);
+    constexpr int G = 4;
+    const int group = id / (G * nblocks), high = min(G, mblocks - group * G), in = id - group * G * nblocks;
+    const int bm = group * G + in % high, bn = in / high;
+    f32x4 acc[1][4] = {};
+    const f32x4 *from = part + unit * 4 * 64 + lane;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s)
 #pragma unroll
-        for (int i0 = 0; i0 < TM; i0 += R) {
-            const int row0 = (mt0 + wm * TM + i0) * 16 + (lane & 15);
-            typename Col::Run res[R];
-            if (a.res) {
-#pragma unroll
-                for (int i = 0; i < R; ++i)
-                    if (row0 + 16 * i < a.m)
-                        res[i] = Col::load((const T *)a.res + (int64_t)(row0 + 16 * i) * a.ldres + col, left, a.vec);
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                typename Col::Sum v;
-#pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    v[c] = acc[i0 + i][c / 4][c % 4];
-                    if (a.bias) v[c] += (float)bias[c];
-                    if (a.res) v[c] += (float)res[i][c];
-                }
-                if (row0 + 16 * i < a.m)
-                    Col::template store<decltype(act)::value>((T *)a.y + (int64_t)(row0 + 16 * i) * a.ldy + col, left, a.vec, v);
-            }
-        }
-    });
+        for (int j = 0; j < 4; ++j) acc[0][j] += from[(s * tiles * NW * TM * 4 + j) * 64];
+    finish_rows<T, 1>(a, (bm * (BM / 16) + wave % WVM * TM + i) * 16 + (lane & 15),
+                      first_col(bn * (BN / 16) + wave / WVM * 4, lane >> 4), acc);
 }
 
 // One thread per 16 bytes of the packed weights, and of a fragment of zeros behind them.
@@ -454,12 +503,58 @@ void launch_stream(const LinearArgs &a, bool xp, hipStream_t st) {
     else linear_stream_kernel<T, MT, NT, NW, false><<<grid, 64 * NW, 0, st>>>(a);
 }
 
-template <class T, int BM, int BN, int WVM, int WVN>
-void launch_tile(const LinearArgs &a, bool xp, hipStream_t st) {
+template <class T, int BM, int BN, int WVM, int WVN, int WF>
+void launch_tile(const LinearArgs &a, bool xp, int splits, void *part, hipStream_t st) {
     const int mb = (a.m + BM - 1) / BM, nb = (a.ntiles * 16 + BN - 1) / BN;
-    if (xp) linear_tile_kernel<T, BM, BN, WVM, WVN, true><<<mb * nb, 64 * WVM * WVN, 0, st>>>(a, mb, nb);
-    else linear_tile_kernel<T, BM, BN, WVM, WVN, false><<<mb * nb, 64 * WVM * WVN, 0, st>>>(a, mb, nb);
+    const unsigned grid = (unsigned)(mb * nb * splits);
+    if (xp) linear_tile_kernel<T, BM, BN, WVM, WVN, WF, true><<<grid, 64 * WVM * WVN, 0, st>>>(a, mb, nb, splits, (f32x4 *)part);
+    else linear_tile_kernel<T, BM, BN, WVM, WVN, WF, false><<<grid, 64 * WVM * WVN, 0, st>>>(a, mb, nb, splits, (f32x4 *)part);
+    if (splits > 1)
+        linear_join_kernel<T, BM, BN, WVM, WVN><<<(unsigned)(((int64_t)mb * nb * (BM * BN / 1024) + 3) / 4), 256, 0, st>>>(
+            a, mb, nb, splits, (const f32x4 *)part);
 }
+
+// Which kernel a layer runs on.
+struct Choice {
+    enum { kStream, kTile64, kTile128, kTile256 } kind;
+    int mt, nt;  // kStream: blocks of 16 rows and columns per workgroup
+    int splits;  // kTile64: along K
+};
+// From measurements over m = 1..4096, n, k = 64..16384 (fp32 and bf16; us at k = 4096 unless stated):
+//  * up to 64 rows, and grids too short to fill the device at a short K: the stream kernel, on the largest blocks that
+//    still leave a workgroup per CU (64 x 4096: 2 x 2 blocks 11.7, 4 x 2 18.8, 1 x 2 14.0; 64 x 16384: 4 x 4
+//    36, 2 x 2 53; 512 x 1024 at k = 1024: 7.1 against 11.1 and more on tiles); up to 16 rows 1 x 1 with 16 waves
+//    (1 x 4096 7.1, 1 x 2 blocks 8.7);
+//  * 256 x 256 tiles from one per CU (4096 x 4096: 124; 2048 x 4096, half as many: 92 against 75 on 128 x 128);
+//  * 128 x 128 from more than one per CU (2048 x 4096: 75 against 97 on 64 x 128; 1024 x 4096, exactly one: 51 against 46);
+//  * 64 x 128 otherwise, K split where that leaves CUs idle (256 x 4096: 29 whole, 22 in two; 128 x 4096: 28, 16 in
+//    four; 200 x 1024 at k = 16384: 92, 23 in eight), parts of at least 16 fragments.
+Choice choose(const SpinnHipLinearDesc *d) {
+    const int64_t cus = device_cu_count(), mt = m_tiles(d), nt = n_tiles(d), kf = frags(d);
+    auto grid = [&](int64_t rows, int64_t cols) { return ((mt + rows - 1) / rows) * ((nt + cols - 1) / cols); };
+    Choice c{Choice::kStream, 1, 1, 1};
+    if (mt <= 1) return c;
+    const int64_t tiles = grid(4, 8);
+    if (mt <= 4 || (tiles < cus && kf < 64)) {
+        static const int blocks[][2] = {{4, 4}, {4, 2}, {2, 4}, {2, 2}, {1, 2}};
+        for (auto &b : blocks)
+            if ((b[0] <= mt || b[0] < 2 * mt) && grid(b[0], b[1]) >= cus) {
+                c.mt = b[0];
+                c.nt = b[1];
+                return c;
+            }
+        return c;
+    }
+    if (grid(16, 16) >= cus) c.kind = Choice::kTile256;
+    else if (grid(8, 8) > cus) c.kind = Choice::kTile128;
+    else {
+        c.kind = Choice::kTile64;
+        c.splits = (int)std::max<int64_t>(1, std::min(cus / tiles, kf / 16));
+    }
+    return c;
+}
+
+size_t x_bytes(const SpinnHipLinearDesc *d) { return x_loose(d) ? (size_t)(m_tiles(d) * frags(d)) * kFragBytes : 0; }
 
 } // namespace
 
@@ -468,7 +563,9 @@ size_t linear_packed_bytes(const SpinnHipLinearDesc *d) {
 }
 
 size_t linear_workspace_bytes(const SpinnHipLinearDesc *d) {
-    return x_loose(d) ? (size_t)(m_tiles(d) * frags(d)) * kFragBytes : 0;
+    const Choice c = choose(d);
+    const size_t tiles = (size_t)((m_tiles(d) + 3) / 4) * ((n_tiles(d) + 7) / 8);
+    return x_bytes(d) + (c.kind == Choice::kTile64 && c.splits > 1 ? tiles * c.splits * 64 * 128 * 4 : 0);
 }
 
 int linear_pack(const SpinnHipLinearDesc *d, const void *w, void *packed, hipStream_t st) {
@@ -501,8 +598,12 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
     const int per = 16 / dtype_bytes(d->dtype);
     a.vec = aligned16(y) && d->ldy % per == 0 && (!res || (aligned16(res) && d->ldres % per == 0));
     const bool xp = x_loose(d);
-    const int64_t wgs = (int64_t)((d->m + 63) / 64) * (a.ntiles / 4);
-    if (wgs > INT32_MAX / 4 || (d->m + 15) / 16 > 65535 * 4) return SPINN_HIP_EUNSUPPORTED;
+    const Choice c = choose(d);
+    const int64_t tiles = ((m_tiles(d) + 3) / 4) * ((n_tiles(d) + 7) / 8);
+    const bool deep = tiles * c.splits <= device_cu_count();
+    // (grids of at most 2^31 workgroups and 65535 rows of them)
+    if (tiles > INT32_MAX / 2 || (c.kind == Choice::kStream && (m_tiles(d) + c.mt - 1) / c.mt > 65535))
+        return SPINN_HIP_EUNSUPPORTED;
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
         if (xp) {
@@ -513,15 +614,23 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
             if (rc) return rc;
             a.x = ws;
         }
-        const int cus = device_cu_count();
-        const int64_t big = (int64_t)((d->m + 255) / 256) * ((a.ntiles + 15) / 16);
-        const int64_t mid = (int64_t)((d->m + 127) / 128) * ((a.ntiles + 7) / 8);
-        if (d->m <= 16) launch_stream<T, 1, 1, 8>(a, xp, st);
-        else if (d->m <= 32) launch_stream<T, 2, 1, 8>(a, xp, st);
-        else if (d->m <= 64) launch_stream<T, 4, 1, 8>(a, xp, st);
-        else if (big >= cus) launch_tile<T, 256, 256, 2, 4>(a, xp, st);
-        else if (mid >= cus / 2) launch_tile<T, 128, 128, 2, 2>(a, xp, st);
-        else launch_stream<T, 4, 4, 4>(a, xp, st);
+        char *part = (char *)ws + x_bytes(d);
+        switch (c.kind) {
+        case Choice::kTile256: launch_tile<T, 256, 256, 2, 4, 4>(a, xp, 1, nullptr, st); break;
+        case Choice::kTile128: launch_tile<T, 128, 128, 2, 2, 4>(a, xp, 1, nullptr, st); break;
+        case Choice::kTile64: // one workgroup per CU can have all of its LDS
+            if (deep) launch_tile<T, 64, 128, 2, 2, 8>(a, xp, c.splits, part, st);
+            else launch_tile<T, 64, 128, 2, 2, 4>(a, xp, c.splits, part, st);
+            break;
+        case Choice::kStream:
+            if (c.mt == 4 && c.nt == 4) launch_stream<T, 4, 4, 4>(a, xp, st);
+            else if (c.mt == 4) launch_stream<T, 4, 2, 8>(a, xp, st);
+            else if (c.mt == 2 && c.nt == 4) launch_stream<T, 2, 4, 4>(a, xp, st);
+            else if (c.mt == 2) launch_stream<T, 2, 2, 8>(a, xp, st);
+            else if (c.nt == 2) launch_stream<T, 1, 2, 8>(a, xp, st);
+            else launch_stream<T, 1, 1, 16>(a, xp, st);
+            break;
+        }
         return check_launch();
     });
 }
