@@ -3,8 +3,7 @@
 // Weights are packed once into MFMA operand fragments, [N/16][K/kFrag][64 lanes][16 bytes] with
 // zeros around, so that a wave reads 1 KB of them with one load and feeds a matrix instruction
 // as they come. The weights are the A operand (its rows are the accumulators' rows), x is the
-// B operand; tile t of four holds columns 64 G + 16 g + 4 t + i, g = l/16, so that a lane's
-// accumulators over the four tiles are 16 neighbouring columns of one row of y.
+// B operand; which columns of 64 a tile holds is chosen for the stores of y (first_col).
 //
 //  * few rows (single tokens): the weights are read once and bound it. linear_stream_kernel: tiles of
 //    16 MT x 16 NT, K spread over a workgroup's waves, operands straight from memory into
@@ -111,8 +110,17 @@ struct Columns {
     }
 };
 
-// First column of the four that accumulator block `tile` of a lane with l/16 = g holds.
-__device__ __forceinline__ int first_col(int tile, int g) { return (tile >> 2) * 64 + 16 * g + 4 * (tile & 3); }
+// Columns that accumulator block `tile` of a lane with l/16 = g holds: four from here on. Of 64 columns the
+// blocks tile % 4 together are 16-byte runs, run q of lane group g at q 4 C + g C (C columns a run), so that the
+// four lanes of a row store 64 neighbouring bytes at a time.
+template <class T>
+constexpr int kRunCols = 16 / (int)sizeof(T);
+template <class T>
+__device__ __forceinline__ int first_col(int tile, int g) {
+    constexpr int C = kRunCols<T>, B = C / 4; // blocks per run
+    const int t = tile & 3;
+    return (tile >> 2) * 64 + (t / B) * 4 * C + g * C + 4 * (t % B);
+}
 
 // x goes to LDS in granules of 16 rows by two fragments, 128 bytes (a cache line) of every row: row r's eight
 // 16-byte runs at 128 r, run c in place c ^ (r / 2), so that the 16 lanes that read run c of 16 rows at once
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
     for (int k = 0; k < B; ++k) {
         const int b = wave + k * NW, tile = t0 + b % NT;
         rows[k] = (m0 + b / NT) * 16 + (lane & 15);
-        cols[k] = first_col(tile, lane >> 4);
+        cols[k] = first_col<T>(tile, lane >> 4);
         left[k] = b < MT * NT && tile < a.ntiles && rows[k] < a.m ? a.n - cols[k] : 0;
         if (left[k] > 0) {
             if (a.bias) bias[k] = Col::load((const T *)a.bias + cols[k], left[k], false);
@@ -222,38 +230,49 @@ __device__ __forceinline__ void stage_ready() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-// A lane's sums of TM rows of blocks, 16 neighbouring columns of a row each, to y.
+// A lane's sums of TM rows of blocks, four 16-column blocks each (from a multiple of 64 on), to y.
 template <class T, int TM>
-__device__ __forceinline__ void finish_rows(const LinearArgs &a, int row0, int col, const f32x4 (&acc)[TM][4]) {
-    typedef Columns<T, 16> Col;
+__device__ __forceinline__ void finish_rows(const LinearArgs &a, int row0, int tile, int g, const f32x4 (&acc)[TM][4]) {
+    constexpr int C = kRunCols<T>, Q = 16 / C; // Q runs of C columns
+    typedef Columns<T, C> Col;
     constexpr int R = TM < 4 ? TM : 4; // rows whose residuals travel at a time
     static_assert(TM % R == 0, "");
-    const int left = a.n - col;
-    if (left <= 0) return;
-    typename Col::Run bias;
-    if (a.bias) bias = Col::load((const T *)a.bias + col, left, false);
+    const int col = first_col<T>(tile, g); // run q: 4 C q behind it
+    if (col >= a.n) return;
+    typename Col::Run bias[Q];
+    if (a.bias) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) bias[q] = Col::load((const T *)a.bias + col + q * 4 * C, a.n - col - q * 4 * C, false);
+    }
     with_act(a.act, [&](auto act) {
 #pragma unroll
         for (int i0 = 0; i0 < TM; i0 += R) {
             const int row = row0 + 16 * i0;
-            typename Col::Run res[R];
+            typename Col::Run res[R][Q];
             if (a.res) {
 #pragma unroll
                 for (int i = 0; i < R; ++i)
                     if (row + 16 * i < a.m)
-                        res[i] = Col::load((const T *)a.res + (int64_t)(row + 16 * i) * a.ldres + col, left, a.vec);
+#pragma unroll
+                        for (int q = 0; q < Q; ++q)
+                            res[i][q] = Col::load((const T *)a.res + (int64_t)(row + 16 * i) * a.ldres + col + q * 4 * C,
+                                                  a.n - col - q * 4 * C, a.vec);
             }
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                typename Col::Sum v;
+                if (row + 16 * i >= a.m) continue;
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    v[c] = acc[i0 + i][c / 4][c % 4];
-                    if (a.bias) v[c] += (float)bias[c];
-                    if (a.res) v[c] += (float)res[i][c];
+                for (int q = 0; q < Q; ++q) {
+                    typename Col::Sum v;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        v[c] = acc[i0 + i][q * (C / 4) + c / 4][c % 4];
+                        if (a.bias) v[c] += (float)bias[q][c];
+                        if (a.res) v[c] += (float)res[i][q][c];
+                    }
+                    Col::template store<decltype(act)::value>((T *)a.y + (int64_t)(row + 16 * i) * a.ldy + col + q * 4 * C,
+                                                              a.n - col - q * 4 * C, a.vec, v);
                 }
-                if (row + 16 * i < a.m)
-                    Col::template store<decltype(act)::value>((T *)a.y + (int64_t)(row + 16 * i) * a.ldy + col, left, a.vec, v);
             }
         }
     });
@@ -263,8 +282,9 @@ __device__ __forceinline__ void finish_rows(const LinearArgs &a, int row0, int c
 // and WF / 2 + 1 granules of x: while fragment f is computed, the reads of f + 1 go to registers (x's
 // as each is used up), and f + 2 .. f + WF are on their way from memory. One barrier per fragment.
 // `splits` > 1: a workgroup takes its share of K and leaves its sums in part[split][tile][block][lane].
+constexpr int tile_lds(int BM, int BN, int WF) { return (WF / 2 + 1) * (BM / 16) * kGranule + WF * (BN / 16) * kFragBytes; }
 template <class T, int BM, int BN, int WVM, int WVN, int WF, bool XP>
-__global__ __launch_bounds__(64 * WVM * WVN, 2) void linear_tile_kernel(LinearArgs a, int mblocks, int nblocks, int splits,
+__global__ __launch_bounds__(64 * WVM * WVN, WVM * WVN == 8 || 2 * tile_lds(BM, BN, WF) <= 160 * 1024 ? 2 : 1) void linear_tile_kernel(LinearArgs a, int mblocks, int nblocks, int splits,
                                                                      f32x4 *part) {
     constexpr int E = 16 / (int)sizeof(T);
     constexpr int NW = WVM * WVN;
@@ -273,7 +293,7 @@ __global__ __launch_bounds__(64 * WVM * WVN, 2) void linear_tile_kernel(LinearAr
     static_assert(BM / 16 * 2 % NW == 0 && BN / 16 % NW == 0 && TN == 4 && (WF & (WF - 1)) == 0, "");
     constexpr int GX = WF / 2 + 1;
     constexpr int kX = BM / 16 * kGranule, kW = BN / 16 * kFragBytes;
-    __shared__ __attribute__((aligned(16))) char lds[GX * kX + WF * kW];
+    __shared__ __attribute__((aligned(16))) char lds[tile_lds(BM, BN, WF)];
     char *const ldw = lds + GX * kX;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // workgroup b runs on XCD b % 8: an XCD takes neighbouring tiles, columns of 4 tiles high, so that
@@ -417,7 +437,7 @@ __global__ __launch_bounds__(64 * WVM * WVN, 2) void linear_tile_kernel(LinearAr
             for (int j = 0; j < TN; ++j) to[(i * TN + j) * 64] = acc[i][j];
         return;
     }
-    finish_rows<T, TM>(a, (mt0 + wm * TM) * 16 + (lane & 15), first_col(nt0 + wn * TN, lane >> 4), acc);
+    finish_rows<T, TM>(a, (mt0 + wm * TM) * 16 + (lane & 15), nt0 + wn * TN, lane >> 4, acc);
 }
 
 // The splits' sums of one row of blocks of a wave's tile, added in split order. One wave each.
@@ -440,7 +460,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a, int mblo
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[0][j] += from[(s * tiles * NW * TM * 4 + j) * 64];
     finish_rows<T, 1>(a, (bm * (BM / 16) + wave % WVM * TM + i) * 16 + (lane & 15),
-                      first_col(bn * (BN / 16) + wave / WVM * 4, lane >> 4), acc);
+                      bn * (BN / 16) + wave / WVM * 4, lane >> 4, acc);
 }
 
 // One thread per 16 bytes of the packed weights, and of a fragment of zeros behind them.
@@ -455,7 +475,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T *__restrict__ 
         const int64_t frag = i >> 6;
         const int64_t tile = frag / kf, f = frag - tile * kf;
         const int r = lane & 15;
-        const int64_t col = (tile >> 2) * 64 + 16 * (r >> 2) + 4 * (tile & 3) + (r & 3);
+        const int64_t col = (tile >> 2) * 64 + first_col<T>((int)(tile & 3), r >> 2) + (r & 3);
         const int64_t k0 = f * kFrag<T> + (lane >> 4) * E;
         u32x4 v = {0, 0, 0, 0};
         if (i < total && col < n) {
