@@ -95,6 +95,17 @@ def test_attention_lengths(hip, torch_gpu, dtype, slots):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("slots,dim,page", [(129, 64, 16), (250, 128, 16), (256, 80, 5), (500, 64, 16), (512, 128, 48), (513, 64, 16)])
+def test_attention_short_sequences(hip, torch_gpu, dtype, slots, dim, page):
+    """Sequences that fit one workgroup's waves, masked, ragged and empty ones among them."""
+    g = gen(slots)
+    c = Cache(g, dtype, 5, 2, dim, page, slots)
+    mask = (torch.rand(5, c.max_pages * page, generator=g) < 0.8).to(torch.uint8)
+    mask[3] = 0
+    attend(hip, c, [slots, slots // 2, 1, 100, 0], heads=8, mask=mask, accumulate=True, max_len=slots)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
 @pytest.mark.parametrize("page", [16, 5])
 def test_attention_masks_and_empty_rows(hip, torch_gpu, dtype, page):
     """Padding, scattered holes, rows that the mask empties, lengths of zero, below zero and past max_len;
