@@ -94,6 +94,21 @@ def test_attention_lengths(hip, torch_gpu, dtype, slots):
     attend(hip, c, [slots], heads=2, accumulate=True, seed=slots)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("seqs,kv,heads,slots", [(70, 1, 2, 900), (130, 3, 3, 700), (1, 5, 10, 3000), (3, 2, 34, 1500), (600, 1, 1, 600)])
+def test_attention_ragged_batches(hip, torch_gpu, dtype, seqs, kv, heads, slots):
+    """Lengths from nothing to all of it, in no order: rows that lie in one workgroup's share, that several share, and
+    shares of several rows; fewer steps than workgroups; more sequences than a wave looks at."""
+    g = gen(seqs)
+    c = Cache(g, dtype, seqs, kv, 16, 16, slots)
+    lengths = (torch.rand(seqs, generator=g) ** 4 * slots).int().tolist()
+    lengths[0], lengths[-1] = slots, (0 if seqs > 1 else slots)
+    attend(hip, c, lengths, heads=heads, accumulate=True)
+    if seqs > 1:
+        attend(hip, c, [0] * (seqs - 1) + [5], heads=heads, accumulate=True, seed=1)
+        attend(hip, c, [0] * seqs, heads=heads, accumulate=True, seed=2)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
 @pytest.mark.parametrize("slots,dim,page", [(129, 64, 16), (250, 128, 16), (256, 80, 5), (500, 64, 16), (512, 128, 48), (513, 64, 16)])
 def test_attention_short_sequences(hip, torch_gpu, dtype, slots, dim, page):
