@@ -98,7 +98,7 @@ int spinn_hip_linear(const SpinnHipLinearDesc *d, const void *x, const void *pac
                      const void *residual, void *y, void *workspace, size_t workspace_bytes, void *stream) {
     if (!linear_ok(d)) return SPINN_HIP_EINVAL;
     if (d->m == 0) return SPINN_HIP_OK;
-    if (!x || !packed_w || !y) return SPINN_HIP_EINVAL;
+    if (!x || !packed_w || !y || y == x) return SPINN_HIP_EINVAL;
     const SpinnHipLinearDesc f = linear_full(d);
     const size_t e = dtype_bytes(f.dtype);
     if (!multiple_of(x, f.x_unaligned ? e : 16) || !aligned16(packed_w) || !multiple_of(bias, e) ||

@@ -44,21 +44,23 @@ def test_linear_arguments(native):
     d = linear_desc(native)
     call = lambda *a, d=d: L.spinn_hip_linear(C.byref(d), *a, None)
     assert L.spinn_hip_linear(None, P, P, None, None, P, None, 0, None) == EINVAL
-    for a in ((None, P, None, None, P), (P, None, None, None, P), (P, P, None, None, None), (ODD, P, None, None, P),
-              (C.c_void_p(4098), P, None, None, P), (P, C.c_void_p(4104), None, None, P), (P, P, ODD, None, P),
-              (P, P, None, ODD, P), (P, P, None, None, ODD)):
+    Q = C.c_void_p(8192)
+    for a in ((None, P, None, None, Q), (P, None, None, None, Q), (P, P, None, None, None), (ODD, P, None, None, Q),
+              (C.c_void_p(4098), P, None, None, Q), (P, C.c_void_p(4104), None, None, Q), (P, P, ODD, None, Q),
+              (P, P, None, ODD, Q), (P, P, None, None, ODD)):
         assert call(*a, None, 0) == EINVAL
+    assert call(P, P, None, None, P, None, 0) == EINVAL  # over its own input
     # over its own residual, with another stride
-    assert call(P, P, None, P, P, None, 0, d=linear_desc(native, ldy=72)) == EINVAL
+    assert call(P, P, None, Q, Q, None, 0, d=linear_desc(native, ldy=72)) == EINVAL
     assert call(None, None, None, None, None, None, 0, d=linear_desc(native, m=0)) == 0
     # rows that are no whole 16-byte runs ask for workspace
     for kw in (dict(k=60), dict(ldx=65), dict(x_unaligned=1)):
         d2 = linear_desc(native, **kw)
         size = L.spinn_hip_linear_workspace_size(C.byref(d2))
         assert size > 0
-        assert call(P, P, None, None, P, None, 0, d=d2) == EWORKSPACE
-        assert call(P, P, None, None, P, P, size - 1, d=d2) == EWORKSPACE
-        assert call(P, P, None, None, P, C.c_void_p(4104), size, d=d2) == EWORKSPACE
+        assert call(P, P, None, None, Q, None, 0, d=d2) == EWORKSPACE
+        assert call(P, P, None, None, Q, P, size - 1, d=d2) == EWORKSPACE
+        assert call(P, P, None, None, Q, C.c_void_p(4104), size, d=d2) == EWORKSPACE
     # packed weights hold every weight, whatever m and the layout
     for kw in (dict(), dict(n=65), dict(k=1), dict(dtype=F32), dict(m=4000), dict(trans_w=0)):
         d2 = linear_desc(native, **kw)

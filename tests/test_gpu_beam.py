@@ -51,6 +51,13 @@ def test_select_sizes(hip, torch_gpu, dtype, b, w, v, k):
     select(hip, dtype, *make(v + k, dtype, b, w, v), k)
 
 
+@pytest.mark.parametrize("b,w,v,k", [(8, 16, 40001, 128), (1, 64, 200001, 20), (8, 16, 40000, 24), (8, 16, 40000, 25)])
+def test_select_long_lists(hip, torch_gpu, b, w, v, k):
+    """The longest candidate lists on chip, more lists than the joining workgroup has lanes, and both sides of the
+    chunk length that goes by k."""
+    select(hip, F16, *make(v + k, F16, b, w, v), k)
+
+
 def test_select_many_chunks(hip, torch_gpu):
     """Rows cut into chunks of every length: by the rows' number, few or many workgroups."""
     for b in (1, 16, 64):
