@@ -69,10 +69,45 @@ __device__ __forceinline__ u32x4 load_edge(const T *p, int left) {
     return r;
 }
 
-// T: element; DP: head_dim padded to 64, 128 or 256; VEC: rows are whole 16-byte runs;
+// N elements from d0 on of a row of `dim` >= N, zeros behind its end, from rows of any alignment: one load, which at the
+// row's end starts early enough to stay inside, and a shift (17 sequences of 12724 to 28547 slots, 8 heads of 33,
+// bf16: 266 us, element by element 756).
+template <class T, int N>
+__device__ __forceinline__ void load_loose(const T *row, int d0, int dim, uint32_t (&to)[N * sizeof(T) / 4]) {
+    constexpr int W = N * sizeof(T) / 4;
+    typedef uint32_t Words __attribute__((ext_vector_type(W)));
+    typedef Words Loose __attribute__((aligned(sizeof(T))));
+    const int at = min(d0, dim - N), skip = (d0 - at) * (int)sizeof(T) * 8; // bits of elements before d0
+    const Words w = *reinterpret_cast<const Loose *>(row + at);
+    if constexpr (W == 2) {
+        const uint64_t v = __builtin_bit_cast(uint64_t, w);
+        const uint64_t r = skip < 64 ? v >> skip : 0ull;
+        to[0] = (uint32_t)r;
+        to[1] = (uint32_t)(r >> 32);
+    } else {
+        static_assert(W == 4, "");
+        const uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+        const int s = skip & 63;
+        const uint64_t both = s ? lo >> s | hi << (64 - s) : lo, top = hi >> s;
+        const uint64_t r0 = skip < 64 ? both : (skip < 128 ? top : 0ull), r1 = skip < 64 ? top : 0ull;
+        to[0] = (uint32_t)r0;
+        to[1] = (uint32_t)(r0 >> 32);
+        to[2] = (uint32_t)r1;
+        to[3] = (uint32_t)(r1 >> 32);
+    }
+}
+
+// How rows of the cache are read.
+enum Rows {
+    kRuns,  // they are whole, aligned 16-byte runs
+    kLoose, // of any length from 16 bytes on and any alignment: load_loose
+    kShort  // shorter: load_edge
+};
+
+// T: element; DP: head_dim padded to 64, 128 or 256; ROWS: how rows are read;
 // UNI: pages are multiples of 16 slots, so that each half tile lies in one page.
 // kWaves: 4, or 8 for a short sequence in one workgroup.
-template <class T, int DP, bool VEC, bool UNI, int kWaves>
+template <class T, int DP, Rows ROWS, bool UNI, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
     constexpr int E = 16 / (int)sizeof(T);    // elements per 16 bytes
     constexpr int KC = DP / kFrag<T>;         // fragments of a row of K or Q
@@ -114,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             const int d0 = c * kFrag<T> + g * E;
-            if (VEC && a.q_runs) q[c] = n < nh && d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
+            if (a.q_runs) q[c] = n < nh && d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
             else q[c] = load_edge<T>(qp + d0, n < nh ? a.dim - d0 : 0);
         }
     }
@@ -163,8 +198,13 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 const int d0 = c * kFrag<T> + g * E;
-                if constexpr (VEC) kr[h][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(kp + d0) : (u32x4){0, 0, 0, 0};
-                else kr[h][c] = load_edge<T>(kp + d0, a.dim - d0);
+                if constexpr (ROWS == kRuns) kr[h][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(kp + d0) : (u32x4){0, 0, 0, 0};
+                else if constexpr (ROWS == kShort) kr[h][c] = load_edge<T>(kp + d0, a.dim - d0);
+                else {
+                    uint32_t w[4];
+                    load_loose<T, E>(kp, d0, a.dim, w);
+                    kr[h][c] = (u32x4){w[0], w[1], w[2], w[3]};
+                }
             }
         }
     };
@@ -187,7 +227,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
                     if (mask) shown[4 * h + j] = mask[slot]; // read where it is needed
                 }
                 uint32_t(&to)[VW] = vr[4 * h + j];
-                if constexpr (VEC) {
+                if constexpr (ROWS == kRuns) {
                     // in 16-byte runs (8 where a lane's share is 8); a row ends between runs
                     constexpr int R = VB >= 16 ? 16 : VB;
 #pragma unroll
@@ -204,11 +244,18 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
                         }
                     }
                 } else {
+                    constexpr int N = DPL < E ? DPL : E; // elements per load
 #pragma unroll
-                    for (int r = 0; r < (VB + 15) / 16; ++r) {
-                        const u32x4 w = load_edge<T>(vp + r * E, min(a.dim - n * DPL - r * E, DPL - r * E));
+                    for (int r = 0; r < DPL / N; ++r) {
+                        uint32_t w[N * sizeof(T) / 4];
+                        if constexpr (ROWS == kLoose) load_loose<T, N>(vp - n * DPL, n * DPL + r * N, a.dim, w);
+                        else {
+                            const u32x4 e = load_edge<T>(vp + r * N, min(a.dim - n * DPL - r * N, N));
 #pragma unroll
-                        for (int i = 0; i < (VW < 4 ? VW : 4); ++i) to[4 * r + i] = w[i];
+                            for (int i = 0; i < N * (int)sizeof(T) / 4; ++i) w[i] = e[i];
+                        }
+#pragma unroll
+                        for (int i = 0; i < N * (int)sizeof(T) / 4; ++i) to[r * (N * (int)sizeof(T) / 4) + i] = w[i];
                     }
                 }
             }
@@ -524,11 +571,13 @@ Plan plan(const SpinnHipKvAttentionDesc *d) {
 }
 
 template <class T, int DP, int W>
-void launch_attend(const AttendArgs &a, bool vec, bool uni, dim3 grid, hipStream_t st) {
+void launch_attend(const AttendArgs &a, Rows rows, bool uni, dim3 grid, hipStream_t st) {
     const size_t lds = (size_t)W * std::min(a.group, kHeadTile) * (DP + 1) * sizeof(float);
-    if (vec && uni) kv_attend_kernel<T, DP, true, true, W><<<grid, 64 * W, lds, st>>>(a);
-    else if (vec) kv_attend_kernel<T, DP, true, false, W><<<grid, 64 * W, lds, st>>>(a);
-    else kv_attend_kernel<T, DP, false, false, W><<<grid, 64 * W, lds, st>>>(a);
+    if (rows == kRuns && uni) kv_attend_kernel<T, DP, kRuns, true, W><<<grid, 64 * W, lds, st>>>(a);
+    else if (rows == kRuns) kv_attend_kernel<T, DP, kRuns, false, W><<<grid, 64 * W, lds, st>>>(a);
+    else if (rows == kLoose && uni) kv_attend_kernel<T, DP, kLoose, true, W><<<grid, 64 * W, lds, st>>>(a);
+    else if (rows == kLoose) kv_attend_kernel<T, DP, kLoose, false, W><<<grid, 64 * W, lds, st>>>(a);
+    else if constexpr (DP == 64) kv_attend_kernel<T, DP, kShort, false, W><<<grid, 64 * W, lds, st>>>(a);
 }
 
 } // namespace
@@ -597,12 +646,13 @@ int kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k,
         const int e = 16 / (int)sizeof(T);
         const bool vec = kv.head_dim % e == 0 && kv.page_stride % e == 0 && kv.head_stride % e == 0 &&
                          kv.slot_stride % e == 0 && aligned16(k) && aligned16(v);
+        const Rows rows = vec ? kRuns : (kv.head_dim >= e ? kLoose : kShort);
         const bool uni = kv.page_size % 16 == 0;
         a.q_runs = kv.head_dim % e == 0 && d->q_stride % e == 0 && aligned16(q);
         const dim3 grid((unsigned)blocks);
-        if (kv.head_dim <= 64) p.waves == 8 ? launch_attend<T, 64, 8>(a, vec, uni, grid, st) : launch_attend<T, 64, 4>(a, vec, uni, grid, st);
-        else if (kv.head_dim <= 128) p.waves == 8 ? launch_attend<T, 128, 8>(a, vec, uni, grid, st) : launch_attend<T, 128, 4>(a, vec, uni, grid, st);
-        else launch_attend<T, 256, 4>(a, vec, uni, grid, st);
+        if (kv.head_dim <= 64) p.waves == 8 ? launch_attend<T, 64, 8>(a, rows, uni, grid, st) : launch_attend<T, 64, 4>(a, rows, uni, grid, st);
+        else if (kv.head_dim <= 128) p.waves == 8 ? launch_attend<T, 128, 8>(a, rows, uni, grid, st) : launch_attend<T, 128, 4>(a, rows, uni, grid, st);
+        else launch_attend<T, 256, 4>(a, rows, uni, grid, st);
         return check_launch();
     });
     if (rc || join_blocks + acc_blocks == 0) return rc;

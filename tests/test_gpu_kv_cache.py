@@ -58,7 +58,7 @@ def attend(N, c, lengths, heads, scale=None, mask=None, accumulate=False, seed=0
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
-@pytest.mark.parametrize("dim", [1, 20, 32, 33, 64, 80, 96, 128, 160, 256])
+@pytest.mark.parametrize("dim", [1, 3, 4, 5, 7, 8, 9, 20, 32, 33, 64, 80, 96, 100, 127, 128, 129, 160, 251, 256])
 def test_attention_dims(hip, torch_gpu, dtype, dim):
     c = Cache(gen(dim), dtype, 3, 2, dim, 16, 100)
     attend(hip, c, [100, 1, 37], heads=4, accumulate=True)
