@@ -417,7 +417,7 @@ int spinn_hip_beam_select(const SpinnHipBeamDesc *d, const void *logits, const f
 /* Rows of beam states after their parents: for every state, batch item b and j < k, row b*k + j of
  * dst = row b*beams + parents[b*k + j] of src (the first row_bytes of it). A parent outside
  * [0, beams) leaves its row of dst as it was. Strides are bytes; dst overlaps no src. Up to
- * SPINN_HIP_MAX_BLOCKS states in one launch. */
+ * SPINN_HIP_MAX_BLOCKS states in one launch, of up to 2^22 rows on either side. */
 typedef struct {
     const void *src;
     void *dst;

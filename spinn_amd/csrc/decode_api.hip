@@ -190,9 +190,9 @@ int spinn_hip_beam_reorder(const SpinnHipBeamState *states, int n_states, int32_
                            const int32_t *parents, void *stream) {
     if (n_states < 0 || n_states > SPINN_HIP_MAX_BLOCKS || batch < 0 || beams <= 0 || k <= 0) return SPINN_HIP_EINVAL;
     if (n_states > 0 && !states) return SPINN_HIP_EINVAL;
-    constexpr int64_t kRows = (int64_t)1 << 22; // rows of dst: one grid row each
-    if ((int64_t)batch * k > kRows || (int64_t)batch * beams > (int64_t)INT32_MAX) return SPINN_HIP_EINVAL;
-    constexpr int64_t kFar = (int64_t)1 << 38;
+    constexpr int64_t kRows = (int64_t)1 << 22; // rows of dst (one grid row each) and of src
+    if ((int64_t)batch * k > kRows || (int64_t)batch * beams > kRows) return SPINN_HIP_EINVAL;
+    constexpr int64_t kFar = (int64_t)1 << 38; // ends of tensors within 61 bits
     for (int i = 0; i < n_states; ++i) {
         const SpinnHipBeamState &s = states[i];
         if (s.row_bytes < 0 || s.src_stride < s.row_bytes || s.dst_stride < s.row_bytes) return SPINN_HIP_EINVAL;

@@ -187,4 +187,8 @@ def test_reorder_arguments(native):
     assert call([ok], parents=None) == EINVAL
     assert call([ok], batch=-1) == EINVAL and call([ok], beams=0) == EINVAL and call([ok], k=0) == EINVAL
     assert call([ok] * 17) == EINVAL and call([ok], n=-1) == EINVAL
+    # sizes whose ends would not fit 64 bits
+    far = N.BeamState(A, B, 64, 1 << 38, 1 << 38)
+    assert call([far], batch=1 << 21, beams=4, k=1) == EINVAL and call([far], batch=1 << 21, k=4) == EINVAL
+    assert call([N.BeamState(A, B, 64, (1 << 38) + 64, 64)]) == EINVAL
     assert call([], n=0) == 0 and call([ok], batch=0) == 0
