@@ -6,8 +6,12 @@
 // first candidates together, from registers: a lower bound for the k-th comes from the lanes' own
 // maxima, and the few elements that pass it are ranked by counting. The second launch joins a
 // batch item's chunks, merging their ordered lists by their heads.
-// Bound: memory, each logit read once; short rows by the latency of two launches.
+// Bound: memory, each logit read once, and as much again the vector units' work on it (a conversion, a maximum
+// and an exponential each), which overlaps with other workgroups' reading only as far as registers let them be there.
+// 32 x 8 beams of 128000 bf16, k = 8: chunks 23 us (2.8 TB/s), join 10.5; 4 beams of 32000 fp32: 5.2 and 6.5, two
+// launches' latency.
 #include "decode.h"
+#include <type_traits>
 
 namespace spinn {
 namespace {
@@ -16,8 +20,9 @@ constexpr int kBeamThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // fp32 to an unsigned number of the same order, both zeros equal; NaN as -inf, +inf as the largest finite.
+// (By the bits: the maximum of a signalling NaN and a number is a NaN, and a bf16 one becomes an fp32 one.)
 __device__ __forceinline__ float clean(float v) {
-    return fminf(fmaxf(v, -INFINITY), 3.402823466e38f); // fmaxf of a NaN is its other operand
+    return (__builtin_bit_cast(uint32_t, v) & 0x7fffffffu) > 0x7f800000u ? -INFINITY : fminf(v, 3.402823466e38f);
 }
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -107,7 +112,8 @@ __host__ __device__ constexpr int beam_lanes(int k) { return 2 * k + 16 < kBeamT
 // Elements per thread of a chunk of kBeamThreads * EPT.
 template <class T, int EPT, bool VEC>
 __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
-    constexpr int E = 16 / (int)sizeof(T);
+    typedef typename Bits<T>::type B;
+    constexpr int E = 16 / (int)sizeof(T), P = 4 / (int)sizeof(T); // elements of a run and of a word
     const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *x = (const T *)a.logits + (int64_t)row * a.stride;
@@ -132,37 +138,62 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
     }
     // runs of E elements, a workgroup's runs side by side: equal logits then spread over the threads.
     // What lies behind the row is -inf like a hidden token, and comes after all tokens.
-    float v[EPT];
+    // They stay as they are in memory and each pass converts them again: 85 registers and five workgroups on a CU
+    // instead of 180 and two (25 -> 23 us over 32 x 8 beams of 128000, bf16).
+    uint32_t w[EPT / P];
     const int first = base + tid * E; // token of the first run
     auto token = [&](int i) { return first + (i / E) * kBeamThreads * E + i % E; };
     if constexpr (VEC) {
-        u32x4 w[EPT / E];
 #pragma unroll
         for (int r = 0; r < EPT / E; ++r) { // a row is whole runs
-            w[r] = (u32x4)(no_logits(T()));
-            if (token(r * E) < a.vocab) w[r] = *reinterpret_cast<const u32x4 *>(x + token(r * E));
+            u32x4 run = (u32x4)(no_logits(T()));
+            if (token(r * E) < a.vocab) run = *reinterpret_cast<const u32x4 *>(x + token(r * E));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[4 * r + i] = run[i];
         }
-#pragma unroll
-        for (int r = 0; r < EPT / E; ++r)
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[r * E + i] = (float)reinterpret_cast<const T *>(&w[r])[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) v[i] = token(i) < a.vocab ? (float)x[token(i)] : -INFINITY;
+        for (int i = 0; i < EPT; i += P) {
+            w[i / P] = no_logits(T());
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+                if (token(i + j) < a.vocab) {
+                    const uint32_t one = (uint32_t) reinterpret_cast<const B *>(x)[token(i + j)];
+                    if constexpr (P == 1) w[i] = one;
+                    else w[i / P] = j ? (w[i / P] & 0xffffu) | one << 16 : (w[i / P] & 0xffff0000u) | one;
+                }
+        }
     }
+    auto logit = [&](int i) {
+        if constexpr (P == 1) return __builtin_bit_cast(float, w[i]);
+        else return (float)__builtin_bit_cast(T, (uint16_t)(w[i / P] >> (16 * (i % P))));
+    };
+    // (keeps the compiler from holding what it converted for the next pass)
+    auto again = [&]() {
+#pragma unroll
+        for (int i = 0; i < EPT / P; ++i) asm volatile("" : "+v"(w[i]));
+    };
     constexpr int kWaves = kBeamThreads / 64;
     __shared__ float wmax[kWaves], wfloor[kWaves];
     __shared__ double wsum[kWaves];
     __shared__ uint64_t bound;
     __shared__ int count, passing;
     extern __shared__ uint64_t list[]; // [beam_lanes(k) * EPT]
+    constexpr int R = EPT / 8; // groups of 8 elements, with their maxima
+    float top[R];
     const int q = (a.k + kWaves - 1) / kWaves;
     float best, floor, m;
     double sum;
-    for (;;) {
+    auto scan = [&](auto cleaned) {
+        auto value = [&](int i) { return decltype(cleaned)::value ? clean(logit(i)) : logit(i); };
         best = -INFINITY; // a NaN leaves it as it is
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) best = fmaxf(best, v[i]);
+        for (int r = 0; r < R; ++r) {
+            top[r] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top[r] = fmaxf(top[r], value(8 * r + i));
+            best = fmaxf(best, top[r]);
+        }
         // Of each wave the q-th largest lane maximum, 4 q >= k: at least q of its elements reach it, so k
         // of the chunk reach the least of the four (-inf, which all reach, where a chunk has fewer).
         float nth = -INFINITY, left = best;
@@ -192,6 +223,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
         }
         const uint64_t pass = __ballot(best >= floor);
         if (lane == 0 && pass) atomicAdd(&passing, __popcll(pass));
+        again();
 
         // share of the sum: exponentials in fp32, added in fp64, so that beams compare to about 1e-8
         sum = 0.0;
@@ -203,12 +235,13 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
                 for (int i = 0; i < EPT; i += 4) {
                     float part = 0.f;
 #pragma unroll
-                    for (int j = i; j < i + 4; ++j) part += __builtin_amdgcn_exp2f(fmaf(v[j], kLog2e, -shift));
+                    for (int j = i; j < i + 4; ++j) part += __builtin_amdgcn_exp2f(fmaf(value(j), kLog2e, -shift));
                     sum += (double)part;
                 }
                 sum *= (double)__builtin_amdgcn_exp2f(-lost);
             } else {
-                for (int i = 0; i < EPT; ++i) sum += (double)__builtin_amdgcn_exp2f((v[i] - m) * kLog2e);
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) sum += (double)__builtin_amdgcn_exp2f((value(i) - m) * kLog2e);
             }
         }
 #pragma unroll
@@ -218,33 +251,30 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
         sum = wsum[0];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) sum += wsum[w];
-        if (m < INFINITY && sum == sum) break;
-        // a NaN or +inf among the logits: once more without them
-#pragma unroll
-        for (int i = 0; i < EPT; ++i) v[i] = clean(v[i]);
+        again();
+    };
+    scan(std::false_type());
+    if (!(m > -INFINITY && m < INFINITY && sum == sum)) { // a NaN or +inf among the logits, or hardly any: once more without them
         __syncthreads();
+        scan(std::true_type());
     }
     if (floor > -INFINITY && passing <= beam_lanes(a.k)) {
-        int n = 0;
+        // (few groups have one)
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) n += v[i] >= floor;
-        if (n) {
-            int to = atomicAdd(&count, n);
+        for (int r = 0; r < R; ++r)
+            if (top[r] >= floor) {
 #pragma unroll
-            for (int i = 0; i < EPT; ++i)
-                if (v[i] >= floor) list[to++] = rank32(v[i], token(i));
-        }
+                for (int i = 8 * r; i < 8 * r + 8; ++i)
+                    if (logit(i) >= floor) list[atomicAdd(&count, 1)] = rank32(clean(logit(i)), token(i));
+            }
     } else {
         // One wave's part of the row is far above another's, or many logits are equal: the k-th of all lane
         // maxima instead, ties told apart by their tokens, from the waves' sorted ones (kept where the list
         // comes later). At most k lanes reach it.
         int at = 0;
 #pragma unroll
-        for (int i = EPT - 1; i >= 0; --i) {
-            v[i] = clean(v[i]);
-            at = v[i] == best ? token(i) : at;
-        }
-        const uint64_t mine = at < a.vocab ? rank32(best, at) : 0ull;
+        for (int i = EPT - 1; i >= 0; --i) at = clean(logit(i)) == best ? i : at;
+        const uint64_t mine = token(at) < a.vocab ? rank32(best, token(at)) : 0ull;
         const int most = a.k < 64 ? a.k : 64;
         uint64_t left = mine;
         for (int i = 0; i < most; ++i) {
@@ -258,12 +288,13 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
             for (int i = 0; i < kWaves * most; ++i) over += list[i] > mine;
         if (mine != 0 && over == a.k - 1) bound = mine;
         __syncthreads();
+        again();
         const uint64_t least = bound;
         if (mine != 0 && mine >= least) {
 #pragma unroll
             for (int i = 0; i < EPT; ++i)
                 if (token(i) < a.vocab) {
-                    const uint64_t u = rank32(v[i], token(i));
+                    const uint64_t u = rank32(clean(logit(i)), token(i));
                     if (u >= least) list[atomicAdd(&count, 1)] = u;
                 }
         }

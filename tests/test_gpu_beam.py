@@ -123,6 +123,25 @@ def test_select_huge_logits(hip, torch_gpu):
     select(hip, F32, x[:1], s[:1], 1)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("v", [8, 40, 999, 8000, 40000])
+def test_select_signalling_nans(hip, torch_gpu, dtype, v):
+    """NaN of every kind count as -inf: among ordinary logits, and in rows of a single other logit, which an ordinary
+    maximum with a signalling NaN loses."""
+    x, s = make(v, dtype, 2, 4, v)
+    bits = torch.int32 if dtype == F32 else torch.int16
+    quiet = {F32: 0x7fc00000, F16: 0x7e00, BF16: 0x7fc0}[dtype]
+    for i, nan in enumerate((quiet, quiet ^ (quiet & -quiet) | 1, -1, quiet - 1)):  # quiet, signalling, negative, signalling
+        lone = x[0, i].clone()
+        lone[:] = -math.inf
+        lone[v // 3] = -2.5
+        x[0, i] = lone
+        x[0, i].view(bits)[torch.arange(v) % 3 != (v // 3) % 3] = nan
+        x[1, i].view(bits)[torch.arange(v) % 5 < 2] = nan
+    assert x[0].isnan().any(1).all() and x[1].isnan().any(1).all()
+    select(hip, dtype, x, s, 8)
+
+
 @pytest.mark.parametrize("end", [0, 999])
 def test_select_finished(hip, torch_gpu, end):
     """Ended beams go on with the end token alone; all ended; ended and empty."""
