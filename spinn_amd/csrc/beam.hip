@@ -8,8 +8,8 @@
 // batch item's chunks, merging their ordered lists by their heads.
 // Bound: memory, each logit read once, and as much again the vector units' work on it (a conversion, a maximum
 // and an exponential each), which overlaps with other workgroups' reading only as far as registers let them be there.
-// 32 x 8 beams of 128000 bf16, k = 8: chunks 23 us (2.8 TB/s), join 10.5; 4 beams of 32000 fp32: 5.2 and 6.5, two
-// launches' latency.
+// 32 x 8 beams of 128000 bf16, k = 16: chunks 23 us (2.8 TB/s), join 10.5; 4 beams of 32000 fp32, k = 8: 5.2 and 6.5,
+// two launches' latency.
 #include "decode.h"
 #include <type_traits>
 

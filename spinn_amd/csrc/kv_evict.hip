@@ -10,6 +10,8 @@
 //    each numbering is one prefix sum; longer rows walk through memory in steps of 1024;
 //  * the rows are moved, 16 lanes per row of K and V.
 // Bound: the rows' moves by memory (256-byte rows at random), the selection by its dozen dependent steps.
+// 16 sequences of 3000 to 8000 slots, 8 heads of 128 bf16, cut to 2000: selection 13 us, moves 47 us (3.8 TB/s).
+// (Counts added up by a wave's ballots before they go to LDS: selection 36 us, the vector units of the one CU.)
 #include "decode.h"
 
 namespace spinn {
@@ -85,7 +87,7 @@ __device__ __forceinline__ void select_key(uint32_t &found, int &want, int *hist
         __syncthreads();
         count(high, found, shift, hist);
         __syncthreads();
-            // thread t: kPer bins from the top (in the last pass the highest of the 11 bits is one found before)
+        // thread t: kPer bins from the top (in the last pass the highest of the 11 bits is one found before)
         int c[kPer], sum = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
