@@ -5,7 +5,7 @@
 // in one pass with the running maximum m and sum: a tile of slots raises m to m', and what
 // was summed so far is scaled by exp(m - m'). Every row of the cache is read once, for all the
 // query heads of its kv head, so the bound is memory: 2 rows a slot against 4 * heads * head_dim flops.
-// 8 kv heads of 128, bf16: one sequence of 131001 slots 101 us (5.3 TB/s), 32 of 37 to 8000 128 us (4.1 TB/s: the
+// 8 kv heads of 128, bf16: one sequence of 131001 slots 101 us (5.3 TB/s), 32 of 37 to 8000 121 us (4.4 TB/s: the
 // last parts run alone, since the split goes by max_len). 16 x 1500..2000, 16 heads of 80 fp32, with
 // weights: 76 us, 7 of them the second launch.
 //
@@ -127,8 +127,20 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
     const int per = 8 * a.head_tiles, ht = (int)(blockIdx.x % per) >> 3;
     int b = (int)(blockIdx.x / per) * 8 + (int)(blockIdx.x & 7);
     if (b >= a.parts) return;
-    const int sp = b % a.splits;
-    b /= a.splits;
+    // Lengths differ, so a row's last parts are short or empty. Up to four parts: all rows' first ones, then the second
+    // ones, ..., so that what starts late is short (24 sequences of 100 to 8000 slots, 8 x 128 bf16: 88 us,
+    // row by row 110; 48 of 100 to 3000: 72, 86). More: row by row, turned so that no XCD has only last ones
+    // (8 of 100 to 60000: 198 us, unturned 200, first parts first 208; 16 of 100 to 16000: 123, 130, 125).
+    int sp;
+    if (a.splits <= 4) {
+        const int rows = a.seqs * a.kv_heads;
+        sp = b / rows;
+        b -= sp * rows;
+    } else {
+        sp = b % a.splits;
+        b /= a.splits;
+        sp = (sp + b / 2) % a.splits;
+    }
     const int kvh = b % a.kv_heads, seq = b / a.kv_heads;
     const int h0 = kvh * a.group + ht * kHeadTile;              // first query head of the tile
     const int nh = min(kHeadTile, a.group - ht * kHeadTile);    // query heads in it
