@@ -518,15 +518,14 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int join_blo
     }
 }
 
-// One workgroup per (token, kv head)-strided run of rows: threads over a token's elements.
-template <class T>
-__global__ __launch_bounds__(256) void kv_append_kernel(SpinnHipKvDesc d, int64_t tokens, const int32_t *seq,
-                                                        const int32_t *slot, const int32_t *position, const T *k,
-                                                        int64_t k_stride, const T *v, int64_t v_stride,
-                                                        const int32_t *table, T *k_pages, T *v_pages, float *acc,
+// Rows of `units` units of U, strides in units. One workgroup per token, threads over its rows of all heads.
+template <class U>
+__global__ __launch_bounds__(256) void kv_append_kernel(SpinnHipKvDesc d, int units, int64_t tokens, const int32_t *seq,
+                                                        const int32_t *slot, const int32_t *position, const U *k,
+                                                        int64_t k_stride, const U *v, int64_t v_stride,
+                                                        const int32_t *table, U *k_pages, U *v_pages, float *acc,
                                                         int32_t *pos, int64_t acc_stride) {
-    typedef typename Bits<T>::type B;
-    const int row = d.kv_heads * d.head_dim;
+    const int row = d.kv_heads * units;
     for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
         const int s = seq ? seq[t] : (int)t;
         const int at = slot[t];
@@ -537,10 +536,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(SpinnHipKvDesc d, int64_
         if ((unsigned)page >= (unsigned)d.n_pages) continue;
         const int64_t base = (int64_t)page * d.page_stride + (int64_t)(at - pi * d.page_size) * d.slot_stride;
         for (int i = threadIdx.x; i < row; i += blockDim.x) {
-            const int h = i / d.head_dim;
-            const int64_t to = base + (int64_t)h * d.head_stride + (i - h * d.head_dim);
-            reinterpret_cast<B *>(k_pages)[to] = reinterpret_cast<const B *>(k)[t * k_stride + i];
-            reinterpret_cast<B *>(v_pages)[to] = reinterpret_cast<const B *>(v)[t * v_stride + i];
+            const int h = i / units;
+            const int64_t to = base + (int64_t)h * d.head_stride + (i - h * units);
+            k_pages[to] = k[t * k_stride + i];
+            v_pages[to] = v[t * v_stride + i];
         }
         if (at < acc_stride)
             for (int h = threadIdx.x; h < d.kv_heads; h += blockDim.x) {
@@ -687,13 +686,26 @@ int kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k,
 int kv_append(const SpinnHipKvDesc *d, int64_t tokens, const int32_t *seq, const int32_t *slot, const int32_t *position,
               const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *table, void *k_pages,
               void *v_pages, float *acc, int32_t *pos, int64_t acc_stride, hipStream_t st) {
-    return with_dtype(d->dtype, [&](auto t) {
-        typedef decltype(t) T;
-        const unsigned grid = (unsigned)std::min<int64_t>(tokens, 65536);
-        kv_append_kernel<T><<<grid, 256, 0, st>>>(*d, tokens, seq, slot, position, (const T *)k, k_stride, (const T *)v,
-                                                  v_stride, table, (T *)k_pages, (T *)v_pages, acc, pos, acc_stride);
+    // in units of 16 bytes where rows are whole, aligned runs of them (16384 tokens of 8 x 128, bf16: 24 us, 5.7 TB/s;
+    // by elements 42)
+    const int e = dtype_bytes(d->dtype), per = 16 / e;
+    const bool vec = d->head_dim % per == 0 && d->page_stride % per == 0 && d->head_stride % per == 0 &&
+                     d->slot_stride % per == 0 && k_stride % per == 0 && v_stride % per == 0 && aligned16(k) && aligned16(v) &&
+                     aligned16(k_pages) && aligned16(v_pages);
+    const int unit = vec ? per : 1;
+    SpinnHipKvDesc u = *d;
+    u.page_stride /= unit;
+    u.head_stride /= unit;
+    u.slot_stride /= unit;
+    auto launch = [&](auto one) {
+        typedef decltype(one) U;
+        kv_append_kernel<U><<<(unsigned)std::min<int64_t>(tokens, 65536), 256, 0, st>>>(
+            u, d->head_dim / unit, tokens, seq, slot, position, (const U *)k, k_stride / unit, (const U *)v, v_stride / unit,
+            table, (U *)k_pages, (U *)v_pages, acc, pos, acc_stride);
         return check_launch();
-    });
+    };
+    if (vec) return launch(u32x4());
+    return e == 4 ? launch(uint32_t()) : launch(uint16_t());
 }
 
 } // namespace spinn

@@ -12,7 +12,13 @@ from tests.decodeops import (BF16, F16, F32, NAMES, TORCH, Cache, assert_close, 
 pytestmark = pytest.mark.gpu
 
 
-def attend(N, c, lengths, heads, scale=None, mask=None, accumulate=False, seed=0, max_len=None, qpad=0, opad=0, lse=True):
+def shifted(x, by):
+    """x's elements at an address `by` elements behind an aligned one."""
+    return torch.cat([x.new_zeros(by), x.flatten()])[by:].view(x.shape)
+
+
+def attend(N, c, lengths, heads, scale=None, mask=None, accumulate=False, seed=0, max_len=None, qpad=0, opad=0, lse=True,
+           shift=0):
     """One call and its comparison; rows around the outputs have to stay as they were."""
     L, g, t = N.lib(), gen(seed), TORCH[c.dtype]
     S, d, slots = c.seqs, c.dim, c.max_pages * c.page
@@ -26,6 +32,8 @@ def attend(N, c, lengths, heads, scale=None, mask=None, accumulate=False, seed=0
     acc = torch.rand(S, c.kv, slots, generator=g)
     accd, outd = acc.cuda(), torch.full((S, c.kv, slots), 777.0, device="cuda")
     kd, vd, td = c.k.cuda(), c.v.cuda(), c.table.cuda()
+    if shift:
+        qd, od, kd, vd = (shifted(x, shift) for x in (qd, od, kd, vd))
     ld = torch.tensor(lengths, dtype=torch.int32).cuda()
     md = None if mask is None else mask.cuda()
     desc = N.KvAttentionDesc(kv=c.desc(N), heads=heads, max_len=max_len, scale=scale, accumulate=int(accumulate),
@@ -175,6 +183,16 @@ def test_attention_layouts(hip, torch_gpu, dtype, layout, pad):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("dim,page", [(64, 16), (33, 5), (4, 16)])
+def test_attention_unaligned_bases(hip, torch_gpu, dtype, dim, page):
+    """Queries, cache and results that start at multiples of their element's size only."""
+    c = Cache(gen(dim + page), dtype, 3, 2, dim, page, 200)
+    even = attend(hip, c, [200, 0, 77], heads=6, accumulate=True, lse=True)
+    odd = attend(hip, c, [200, 0, 77], heads=6, accumulate=True, lse=True, shift=1)
+    assert odd.shape == even.shape
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
 def test_attention_one_slot_outweighs_the_rest(hip, torch_gpu, dtype):
     """One score 17 above thousands of equal ones: the rest together still weigh 2^-12 or so each way, which fp16
     weights would lose one by one."""
@@ -221,8 +239,8 @@ def test_attention_far_pages(hip, torch_gpu):
 # ---- append ----
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
-@pytest.mark.parametrize("dim,page,layout", [(64, 16, "head"), (33, 5, "slot")])
-def test_append(hip, torch_gpu, dtype, dim, page, layout):
+@pytest.mark.parametrize("dim,page,layout,pad", [(64, 16, "head", 2), (64, 16, "head", 8), (24, 5, "slot", 0), (33, 5, "slot", 2)])
+def test_append(hip, torch_gpu, dtype, dim, page, layout, pad):
     """Tokens of a ragged batch, out of the rows of a fused projection; those outside the cache or on a page that
     holds nothing are skipped, all else stays."""
     N, L, g = hip, hip.lib(), gen(dim)
@@ -232,7 +250,7 @@ def test_append(hip, torch_gpu, dtype, dim, page, layout):
     seq = torch.tensor([0, 0, 2, 1, 1, 3, -1, 0, 2, 2], dtype=torch.int32)
     slot = torch.tensor([0, 39, 7, 3, page, 1, 1, slots, -1, 20], dtype=torch.int32)
     position = torch.arange(100, 110, dtype=torch.int32)
-    qkv = randn(g, 10, 3 * row + 2, dtype=dtype)
+    qkv = randn(g, 10, 3 * row + pad, dtype=dtype)
     acc, pos = torch.rand(3, 2, slots, generator=g), torch.full((3, 2, slots), 9, dtype=torch.int32)
     k0, v0 = c.k.clone(), c.v.clone()
     wa, wp = acc.clone(), pos.clone()
@@ -248,16 +266,16 @@ def test_append(hip, torch_gpu, dtype, dim, page, layout):
     sd, od, pd, xd, td, kd, vd, ad, bd = dev
     e = qkv.element_size()
     d = c.desc(N)
-    N.check(L.spinn_hip_kv_append(C.byref(d), 10, ptr(sd), ptr(od), ptr(pd), C.c_void_p(xd.data_ptr() + row * e), 3 * row + 2,
-                                  C.c_void_p(xd.data_ptr() + 2 * row * e), 3 * row + 2, ptr(td), ptr(kd), ptr(vd), ptr(ad),
+    N.check(L.spinn_hip_kv_append(C.byref(d), 10, ptr(sd), ptr(od), ptr(pd), C.c_void_p(xd.data_ptr() + row * e), 3 * row + pad,
+                                  C.c_void_p(xd.data_ptr() + 2 * row * e), 3 * row + pad, ptr(td), ptr(kd), ptr(vd), ptr(ad),
                                   ptr(bd), slots, stream()), "append")
     torch.cuda.synchronize()
     assert torch.equal(kd.cpu(), k0) and torch.equal(vd.cpu(), v0)
     assert torch.equal(ad.cpu(), wa) and torch.equal(bd.cpu(), wp)
     # one token per sequence, positions and weights not kept
     slot = torch.tensor([2, 4, 11], dtype=torch.int32).cuda()
-    N.check(L.spinn_hip_kv_append(C.byref(d), 3, None, ptr(slot), None, C.c_void_p(xd.data_ptr() + row * e), 3 * row + 2,
-                                  C.c_void_p(xd.data_ptr() + 2 * row * e), 3 * row + 2, ptr(td), ptr(kd), ptr(vd), None, None,
+    N.check(L.spinn_hip_kv_append(C.byref(d), 3, None, ptr(slot), None, C.c_void_p(xd.data_ptr() + row * e), 3 * row + pad,
+                                  C.c_void_p(xd.data_ptr() + 2 * row * e), 3 * row + pad, ptr(td), ptr(kd), ptr(vd), None, None,
                                   0, stream()), "append")
     for s, i in enumerate((2, 4, 11)):
         p = int(c.table[s, i // page])
