@@ -281,8 +281,8 @@ enum {
  * `packed_w` alone afterwards. Rows of x, residual and y are ldx, ldres and ldy apart
  * (0 = dense: k, n, n). y may be the residual itself (same address and stride); otherwise
  * y overlaps no input.
- * x starts at a multiple of 16 bytes unless x_unaligned is set, which asks for workspace (as
- * rows that are no whole 16-byte runs do); strides are free up to 2^28. m = 0 is an empty batch.
+ * x starts at a multiple of 16 bytes unless x_unaligned is set, with which many rows ask for
+ * workspace (as rows that are no whole 16-byte runs do); strides are free up to 2^28. m = 0 is an empty batch.
  */
 typedef struct {
     int32_t m, n, k;

@@ -26,7 +26,7 @@ inline int64_t frags(const SpinnHipLinearDesc *d) { // along K, an even number
 }
 inline int64_t n_tiles(const SpinnHipLinearDesc *d) { return ((int64_t)d->n + 63) / 64 * 4; }
 inline int64_t m_tiles(const SpinnHipLinearDesc *d) { return ((int64_t)d->m + 15) / 16; }
-// x's rows are not whole 16-byte runs: they are laid out as fragments first
+// x's rows are not whole, aligned 16-byte runs
 inline bool x_loose(const SpinnHipLinearDesc *d) {
     const int e = 16 / dtype_bytes(d->dtype);
     return d->x_unaligned || d->ldx % e || d->k % e;
@@ -135,8 +135,7 @@ __device__ __forceinline__ int granule_at(int lane, int half) {
     return r * 128 + ((c ^ (r >> 1)) << 4);
 }
 
-// XP: x is laid out as granules.
-template <class T, int MT, int NT, int NW, bool XP>
+template <class T, int MT, int NT, int NW, Rows ROWS>
 __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
     constexpr int E = 16 / (int)sizeof(T);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -145,16 +144,11 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
         wp[j] = a.w + (int64_t)min(t0 + j, a.ntiles - 1) * a.kf * kFragBytes + lane * 16;
-    const char *xp[MT];
+    const T *xp[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        if constexpr (XP) {
-            const int mt = min(m0 + i, (a.m - 1) >> 4);
-            xp[i] = (const char *)a.x + (int64_t)mt * a.kf * kFragBytes;
-        } else {
-            const int row = min((m0 + i) * 16 + (lane & 15), a.m - 1);
-            xp[i] = (const char *)((const T *)a.x + (int64_t)row * a.ldx + (lane >> 4) * E);
-        }
+        if constexpr (ROWS == kLaidOut) xp[i] = (const T *)((const char *)a.x + (int64_t)min(m0 + i, (a.m - 1) >> 4) * a.kf * kFragBytes);
+        else xp[i] = (const T *)a.x + (int64_t)min((m0 + i) * 16 + (lane & 15), a.m - 1) * a.ldx + (ROWS == kRuns ? (lane >> 4) * E : 0);
     }
     f32x4 acc[MT][NT] = {};
     constexpr int U = MT * NT >= 8 ? 2 : 4;
@@ -167,10 +161,15 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
             for (int j = 0; j < NT; ++j) w[u][j] = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)f * kFragBytes);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if constexpr (XP) x[u][i] = *reinterpret_cast<const u32x4 *>(xp[i] + (int64_t)(f >> 1) * kGranule + granule_at(lane, f & 1));
+                const int k0 = f * kFrag<T> + (lane >> 4) * E;
+                if constexpr (ROWS == kLaidOut)
+                    x[u][i] = *reinterpret_cast<const u32x4 *>((const char *)xp[i] + (int64_t)(f >> 1) * kGranule + granule_at(lane, f & 1));
+                else if constexpr (ROWS == kRuns) x[u][i] = k0 < a.k ? *reinterpret_cast<const u32x4 *>(xp[i] + (int64_t)f * kFrag<T>) : (u32x4){0, 0, 0, 0};
+                else if constexpr (ROWS == kShort) x[u][i] = load_edge<T>(xp[i] + k0, a.k - k0);
                 else {
-                    const bool in = f * kFrag<T> + (lane >> 4) * E < a.k;
-                    x[u][i] = in ? *reinterpret_cast<const u32x4 *>(xp[i] + (int64_t)f * 64) : (u32x4){0, 0, 0, 0};
+                    uint32_t r[4];
+                    load_loose<T, E>(xp[i], k0, a.k, r);
+                    x[u][i] = (u32x4){r[0], r[1], r[2], r[3]};
                 }
             }
         }
@@ -520,10 +519,12 @@ __global__ __launch_bounds__(256) void linear_pack_x_kernel(const T *__restrict_
 }
 
 template <class T, int MT, int NT, int NW>
-void launch_stream(const LinearArgs &a, bool xp, hipStream_t st) {
+void launch_stream(const LinearArgs &a, Rows rows, hipStream_t st) {
     const dim3 grid((a.ntiles + NT - 1) / NT, (a.m + 16 * MT - 1) / (16 * MT));
-    if (xp) linear_stream_kernel<T, MT, NT, NW, true><<<grid, 64 * NW, 0, st>>>(a);
-    else linear_stream_kernel<T, MT, NT, NW, false><<<grid, 64 * NW, 0, st>>>(a);
+    if (rows == kRuns) linear_stream_kernel<T, MT, NT, NW, kRuns><<<grid, 64 * NW, 0, st>>>(a);
+    else if (rows == kLaidOut) linear_stream_kernel<T, MT, NT, NW, kLaidOut><<<grid, 64 * NW, 0, st>>>(a);
+    else if (rows == kLoose) linear_stream_kernel<T, MT, NT, NW, kLoose><<<grid, 64 * NW, 0, st>>>(a);
+    else linear_stream_kernel<T, MT, NT, NW, kShort><<<grid, 64 * NW, 0, st>>>(a);
 }
 
 template <class T, int BM, int BN, int WVM, int WVN, int WF>
@@ -577,7 +578,20 @@ Choice choose(const SpinnHipLinearDesc *d) {
     return c;
 }
 
-size_t x_bytes(const SpinnHipLinearDesc *d) { return x_loose(d) ? (size_t)(m_tiles(d) * frags(d)) * kFragBytes : 0; }
+// How a layer reads x. Rows that are no whole, aligned runs are laid out in the workspace by a launch of their own,
+// but the stream kernel reads them where they are while a workgroup's rows stay under 32 KB: its unaligned loads then
+// cost less than the launch (1 x 4096 x 4097 bf16: 10.8 -> 7.8 us, 427 x 131 x 275: 10.3 -> 7.6; 40 KB, 202 x 1758 x 632:
+// 10.4 -> 13.0; 131 KB, 16 x 4096 x 4097: 11.6 -> 16.8).
+Rows x_rows(const SpinnHipLinearDesc *d, const Choice &c) {
+    if (!x_loose(d)) return kRuns;
+    const int64_t bytes = (int64_t)d->k * dtype_bytes(d->dtype);
+    if (c.kind != Choice::kStream || std::min(d->m, 16 * c.mt) * bytes > 32768) return kLaidOut;
+    return bytes >= 16 ? kLoose : kShort;
+}
+
+size_t x_bytes(const SpinnHipLinearDesc *d, const Choice &c) {
+    return x_rows(d, c) == kLaidOut ? (size_t)(m_tiles(d) * frags(d)) * kFragBytes : 0;
+}
 
 } // namespace
 
@@ -588,7 +602,7 @@ size_t linear_packed_bytes(const SpinnHipLinearDesc *d) {
 size_t linear_workspace_bytes(const SpinnHipLinearDesc *d) {
     const Choice c = choose(d);
     const size_t tiles = (size_t)((m_tiles(d) + 3) / 4) * ((n_tiles(d) + 7) / 8);
-    return x_bytes(d) + (c.kind == Choice::kTile64 && c.splits > 1 ? tiles * c.splits * 64 * 128 * 4 : 0);
+    return x_bytes(d, c) + (c.kind == Choice::kTile64 && c.splits > 1 ? tiles * c.splits * 64 * 128 * 4 : 0);
 }
 
 int linear_pack(const SpinnHipLinearDesc *d, const void *w, void *packed, hipStream_t st) {
@@ -620,8 +634,9 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
     a.ntiles = (int32_t)n_tiles(d);
     const int per = 16 / dtype_bytes(d->dtype);
     a.vec = aligned16(y) && d->ldy % per == 0 && (!res || (aligned16(res) && d->ldres % per == 0));
-    const bool xp = x_loose(d);
     const Choice c = choose(d);
+    const Rows rows = x_rows(d, c);
+    const bool xp = rows == kLaidOut;
     const int64_t tiles = ((m_tiles(d) + 3) / 4) * ((n_tiles(d) + 7) / 8);
     const bool deep = tiles * c.splits <= device_cu_count();
     // (grids of at most 2^31 workgroups and 65535 rows of them)
@@ -637,7 +652,7 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
             if (rc) return rc;
             a.x = ws;
         }
-        char *part = (char *)ws + x_bytes(d);
+        char *part = (char *)ws + x_bytes(d, c);
         switch (c.kind) {
         case Choice::kTile256: launch_tile<T, 256, 256, 2, 4, 4>(a, xp, 1, nullptr, st); break;
         case Choice::kTile128: launch_tile<T, 128, 128, 2, 2, 4>(a, xp, 1, nullptr, st); break;
@@ -646,12 +661,12 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
             else launch_tile<T, 64, 128, 2, 2, 4>(a, xp, c.splits, part, st);
             break;
         case Choice::kStream:
-            if (c.mt == 4 && c.nt == 4) launch_stream<T, 4, 4, 4>(a, xp, st);
-            else if (c.mt == 4) launch_stream<T, 4, 2, 8>(a, xp, st);
-            else if (c.mt == 2 && c.nt == 4) launch_stream<T, 2, 4, 4>(a, xp, st);
-            else if (c.mt == 2) launch_stream<T, 2, 2, 8>(a, xp, st);
-            else if (c.nt == 2) launch_stream<T, 1, 2, 8>(a, xp, st);
-            else launch_stream<T, 1, 1, 16>(a, xp, st);
+            if (c.mt == 4 && c.nt == 4) launch_stream<T, 4, 4, 4>(a, rows, st);
+            else if (c.mt == 4) launch_stream<T, 4, 2, 8>(a, rows, st);
+            else if (c.mt == 2 && c.nt == 4) launch_stream<T, 2, 4, 4>(a, rows, st);
+            else if (c.mt == 2) launch_stream<T, 2, 2, 8>(a, rows, st);
+            else if (c.nt == 2) launch_stream<T, 1, 2, 8>(a, rows, st);
+            else launch_stream<T, 1, 1, 16>(a, rows, st);
             break;
         }
         return check_launch();

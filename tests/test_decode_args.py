@@ -53,9 +53,10 @@ def test_linear_arguments(native):
     # over its own residual, with another stride
     assert call(P, P, None, Q, Q, None, 0, d=linear_desc(native, ldy=72)) == EINVAL
     assert call(None, None, None, None, None, None, 0, d=linear_desc(native, m=0)) == 0
-    # rows that are no whole 16-byte runs ask for workspace
+    # many rows that are no whole 16-byte runs ask for workspace, few do not
     for kw in (dict(k=60), dict(ldx=65), dict(x_unaligned=1)):
-        d2 = linear_desc(native, **kw)
+        assert L.spinn_hip_linear_workspace_size(C.byref(linear_desc(native, **kw))) == 0
+        d2 = linear_desc(native, m=4000, n=4096, **kw)
         size = L.spinn_hip_linear_workspace_size(C.byref(d2))
         assert size > 0
         assert call(P, P, None, None, Q, None, 0, d=d2) == EWORKSPACE

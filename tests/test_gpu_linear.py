@@ -81,6 +81,14 @@ def test_linear_strides(hip, torch_gpu, dtype, m, padx, padr, pady, off):
     run(hip, dtype, m, 260, 128, res=True, bias=True, padx=padx, padr=padr, pady=pady, off=off)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("mnk", [(5, 70, 3), (40, 200, 7), (2, 50, 8), (1, 100, 16385), (16, 100, 4097), (9, 64, 1023), (33, 300, 2047),
+                                 (60, 4200, 301), (427, 131, 275)], ids=str)
+def test_linear_loose_rows(hip, torch_gpu, dtype, mnk):
+    """Few rows that are no whole runs: read where they are, up to the length from which they are laid out first."""
+    run(hip, dtype, *mnk, bias=True, padx=1, off=1)
+
+
 @pytest.mark.parametrize("m", [1, 200, 600])
 def test_linear_in_place(hip, torch_gpu, m):
     """y over its own residual, the residual stream of a network."""
