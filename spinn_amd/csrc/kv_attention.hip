@@ -5,9 +5,9 @@
 // in one pass with the running maximum m and sum: a tile of slots raises m to m', and what
 // was summed so far is scaled by exp(m - m'). Every row of the cache is read once, for all the
 // query heads of its kv head, so the bound is memory: 2 rows a slot against 4 * heads * head_dim flops.
-// 8 kv heads of 128, bf16: one sequence of 131001 slots 101 us (5.3 TB/s), 32 of 37 to 8000 121 us (4.4 TB/s: the
+// 8 kv heads of 128, bf16: one sequence of 131001 slots 101 us (5.3 TB/s), 32 of 37 to 8000 119 us (4.4 TB/s: the
 // last parts run alone, since the split goes by max_len). 16 x 1500..2000, 16 heads of 80 fp32, with
-// weights: 76 us, 7 of them the second launch.
+// weights: 75 us, 7 of them the second launch.
 //
 // The matrix cores then have time to spare (one new token fills few of a tile's 16 columns, and
 // at 5 TB/s they are still under 5 % busy), which decides the layout: nothing goes through LDS in the

@@ -498,23 +498,22 @@ template <class T>
 __global__ __launch_bounds__(256) void linear_pack_x_kernel(const T *__restrict__ x, u32x4 *__restrict__ out, int m, int k,
                                                             int64_t ldx, int64_t kf, int64_t total) {
     constexpr int E = 16 / (int)sizeof(T);
-    typedef typename Bits<T>::type B;
-    const B *xb = reinterpret_cast<const B *>(x);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int in = (int)(i & 127), r = in >> 3;
         const int64_t granule = i >> 7, tile = granule / (kf / 2), g = granule - tile * (kf / 2);
-        const int64_t row = tile * 16 + r, k0 = g * 2 * kFrag<T> + ((in & 7) ^ (r >> 1)) * E;
-        u32x4 v = {0, 0, 0, 0};
-        if (row < m) {
+        const int64_t row = tile * 16 + r;
+        const int k0 = (int)(g * 2 * kFrag<T>) + ((in & 7) ^ (r >> 1)) * E;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (row < m && k0 < k) {
+            if (k >= E) {
+                load_loose<T, E>(x + row * ldx, k0, k, w);
+            } else {
+                const u32x4 v = load_edge<T>(x + row * ldx + k0, k - k0);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (k0 + e < k) {
-                    const uint32_t b = xb[row * ldx + k0 + e];
-                    if constexpr (E == 4) v[e] = b;
-                    else v[e / 2] |= b << (16 * (e % 2));
-                }
+                for (int j = 0; j < 4; ++j) w[j] = v[j];
+            }
         }
-        out[i] = v;
+        out[i] = (u32x4){w[0], w[1], w[2], w[3]};
     }
 }
 
@@ -581,7 +580,7 @@ Choice choose(const SpinnHipLinearDesc *d) {
 // How a layer reads x. Rows that are no whole, aligned runs are laid out in the workspace by a launch of their own,
 // but the stream kernel reads them where they are while a workgroup's rows stay under 32 KB: its unaligned loads then
 // cost less than the launch (1 x 4096 x 4097 bf16: 10.8 -> 7.8 us, 427 x 131 x 275: 10.3 -> 7.6; 40 KB, 202 x 1758 x 632:
-// 10.4 -> 13.0; 131 KB, 16 x 4096 x 4097: 11.6 -> 16.8).
+// 9.9 -> 13.0; 131 KB, 16 x 4096 x 4097: 10.0 -> 16.8).
 Rows x_rows(const SpinnHipLinearDesc *d, const Choice &c) {
     if (!x_loose(d)) return kRuns;
     const int64_t bytes = (int64_t)d->k * dtype_bytes(d->dtype);
