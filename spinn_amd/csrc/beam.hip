@@ -368,12 +368,17 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a, 
         const float *cm = a.chunk_max + (int64_t)row * a.chunks;
         const double *cs = a.chunk_sum + (int64_t)row * a.chunks;
         const float sc = a.scores[row];
-        float m = -INFINITY;
-        for (int i = lane; i < a.chunks; i += 64) m = fmaxf(m, cm[i]);
+        // (a lane's first chunk at once, both its numbers)
+        const float m0 = lane < a.chunks ? cm[lane] : -INFINITY;
+        const double s0 = lane < a.chunks ? cs[lane] : 0.0;
+        float m = m0;
+        for (int i = lane + 64; i < a.chunks; i += 64) m = fmaxf(m, cm[i]);
         m = wave_fmax(m);
         double s = 0.0;
-        if (m != -INFINITY)
-            for (int i = lane; i < a.chunks; i += 64) s += cs[i] * exp((double)cm[i] - (double)m);
+        if (m != -INFINITY) {
+            s = s0 * exp((double)m0 - (double)m);
+            for (int i = lane + 64; i < a.chunks; i += 64) s += cs[i] * exp((double)cm[i] - (double)m);
+        }
 #pragma unroll
         for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
         if (lane == 0) {
