@@ -228,9 +228,11 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
         // share of the sum: exponentials in fp32, added in fp64, so that beams compare to about 1e-8
         sum = 0.0;
         if (m != -INFINITY) {
-            // exp(v - m) = 2^(v L - m L), in one rounding; what m L lost is a factor of the whole sum
+            // exp(v - m) = 2^(v L - m L), in one rounding; what m L lost is a factor of the whole sum. Half a step of m L is
+            // at most 1/16 below 2^20; from 128 on, one of the two would be infinite and the other zero. Beyond, v - m first:
+            // exact for the v that are anywhere near m.
             const float shift = m * kLog2e, lost = fmaf(m, kLog2e, -shift);
-            if (fabsf(m) < 1e30f) {
+            if (fabsf(m) < 1e6f) {
 #pragma unroll
                 for (int i = 0; i < EPT; i += 4) {
                     float part = 0.f;

@@ -123,6 +123,45 @@ def test_select_huge_logits(hip, torch_gpu):
     select(hip, F32, x[:1], s[:1], 1)
 
 
+def far_ref(logits, scores, k):
+    """beam_ref without finished beams, the logits' maximum taken off before the sum's logarithm: a key of 64 bits, at any
+    magnitude."""
+    x = logits.double()
+    key = scores.double()[:, :, None] + torch.log_softmax(x, 2)
+    val, at = torch.sort(key.flatten(1), dim=1, descending=True, stable=True)
+    return val[:, :k], (at[:, :k] // x.shape[2]).int(), (at[:, :k] % x.shape[2]).int()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("far", [9e5, 1e6, 1.1e6, 1e9, 4e9, 5e9])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_select_far_logits(hip, torch_gpu, dtype, far, sign):
+    """Finite logits far from the others, as programs hide tokens with: single ones, whole chunks, whole rows, beside an
+    ordinary beam."""
+    for b, v in ((1, 40000), (64, 20000)):  # chunks of 2048 tokens, and of the longest
+        x, s = make(int(far % 997) + v, dtype, b, 4, v)
+        hidden = torch.tensor(sign * far).to(TORCH[dtype])
+        x[:, 0, 100:110] = hidden
+        x[:, 1, 4096:20000] = hidden  # chunks between others (from 16384 on of the longest), and the row's end there
+        x[:, 2] = hidden
+        x[:, 2, 5] = hidden * (1 + sign * 2.0 ** -6)  # next to it
+        s[:] = torch.tensor([-1.0, -3.0, -5.0, -7.0])
+        k = 24
+        L, xd, sd = hip.lib(), x.cuda(), s.cuda()
+        d = hip.BeamDesc(dtype=dtype, batch=b, beams=4, vocab=v, k=k, end_token=0, logits_stride=v)
+        size = L.spinn_hip_beam_select_workspace_size(C.byref(d))
+        ws, os = workspace(size), torch.full((b, k), 777.0, device="cuda")
+        op, ot = (torch.full((b, k), 777, dtype=torch.int32, device="cuda") for _ in range(2))
+        hip.check(L.spinn_hip_beam_select(C.byref(d), ptr(xd), ptr(sd), None, ptr(os), ptr(op), ptr(ot), ptr(ws), size, stream()),
+                  "spinn_hip_beam_select")
+        key, parents, tokens = far_ref(x, s, k)
+        got = os.cpu().double()
+        assert torch.isfinite(got).all()
+        # as in select(): the sum of exponentials, and the result's rounding
+        assert ((got - key).abs() <= 2.0 ** -20 + 2.0 ** -23 * key.abs()).all(), (got - key).abs().max()
+        assert torch.equal(op.cpu(), parents) and torch.equal(ot.cpu(), tokens)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
 @pytest.mark.parametrize("v", [8, 40, 999, 8000, 40000])
 def test_select_signalling_nans(hip, torch_gpu, dtype, v):
