@@ -358,7 +358,8 @@ template <bool CACHED>
 __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a, int merging) {
     const int item = blockIdx.x, tid = threadIdx.x, waves = blockDim.x >> 6;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    __shared__ double lse[SPINN_HIP_BEAM_MAX], score[SPINN_HIP_BEAM_MAX];
+    // lse in two parts: beside a large maximum the sum's logarithm would be lost
+    __shared__ double most[SPINN_HIP_BEAM_MAX], log_sum[SPINN_HIP_BEAM_MAX], score[SPINN_HIP_BEAM_MAX];
     __shared__ uint64_t key_at[CACHED ? kJoinCached : 1], cand_at[CACHED ? kJoinCached : 1];
     extern __shared__ Rank merged[]; // [merging][k], where several waves merge
     const int lists = a.beams * a.chunks, total = lists * a.k, per_beam = a.chunks * a.k;
@@ -385,13 +386,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a, 
         for (int off = 32; off; off >>= 1) s += __shfl_xor(s, off);
         if (lane == 0) {
             score[b] = (double)clean(sc);
-            lse[b] = m == -INFINITY ? 0.0 : (double)m + log(s);
+            most[b] = m == -INFINITY ? 0.0 : (double)m;
+            log_sum[b] = m == -INFINITY ? 0.0 : log(s);
         }
     }
     __syncthreads();
     auto key_of = [&](uint64_t c, int b) {
         const float x = unordered((uint32_t)(c >> 32));
-        return c == 0 ? 0ull : ordered64(x == -INFINITY ? -INFINITY : score[b] + ((double)x - lse[b]));
+        return c == 0 ? 0ull : ordered64(x == -INFINITY ? -INFINITY : score[b] + (((double)x - most[b]) - log_sum[b]));
     };
     if constexpr (CACHED) {
         for (int i = tid; i < total; i += blockDim.x) key_at[i] = key_of(cand_at[i], i / per_beam);

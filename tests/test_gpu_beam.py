@@ -133,7 +133,7 @@ def far_ref(logits, scores, k):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
-@pytest.mark.parametrize("far", [9e5, 1e6, 1.1e6, 1e9, 4e9, 5e9])
+@pytest.mark.parametrize("far", [9e5, 1e6, 1.1e6, 1e9, 4e9, 5e9, 1e10, 1e12, 1e15, 1e20, 9e29, 2e30, 3e38])
 @pytest.mark.parametrize("sign", [-1, 1])
 def test_select_far_logits(hip, torch_gpu, dtype, far, sign):
     """Finite logits far from the others, as programs hide tokens with: single ones, whole chunks, whole rows, beside an
