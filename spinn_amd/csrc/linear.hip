@@ -11,7 +11,7 @@
 //    33 x 8192 x 2048 fp16: 8.5 us, 4.0 TB/s.
 //  * many rows: the matrix cores bound it. linear_tile_kernel: both operands through LDS, whole
 //    fragments copied there without passing registers, four of them along K. 4096 x 8192 x 4096 bf16:
-//    218 us, 1260 TFLOP/s; 1568 x 2048 x 512 fp32: 40 us, 82 TFLOP/s (400 tiles for 256 CUs).
+//    218 us, 1260 TFLOP/s; 1568 x 2048 x 512 fp32: 41 us, 80 TFLOP/s (400 tiles for 256 CUs).
 #include "decode.h"
 #include <type_traits>
 
@@ -32,15 +32,20 @@ inline bool x_loose(const SpinnHipLinearDesc *d) {
     return d->x_unaligned || d->ldx % e || d->k % e;
 }
 
-// v Phi(v) with erfc by Abramowitz and Stegun 7.1.26 (|error| < 1.5e-7 of 1, so under 1e-7 |v| here, against
-// 6e-8 |v| for a correctly rounded erf): a dozen instructions for the library's forty, in an epilogue
-// that is unrolled over up to 128 values.
+// v Phi(v), within 3 * 2^-24 |v| (a correctly rounded 1 + erf has 2) and, for v < 0, within (10 + v^2) 2^-24 of itself.
+// Up to 1.25, Phi(v) = 1/2 + v S(v^2); beyond, Phi(-a) = exp(-a^2 / 2) R(a), R(a) = exp(a^2 / 2) Phi(-a) = t P(t) for
+// t = 1 / (1 + a/2). S and P are polynomials fitted to them with the least relative error (1e-8 and 1.4e-8, up to
+// a = 14.6, where exp has left fp32). 26 instructions; an epilogue unrolls them over up to 128 values, and the whole of
+// 1568 x 2048 x 512 fp32 takes 41.1 us (40.2 with a seven-digit erfc of half the length).
 __device__ __forceinline__ float gelu_erf(float v) {
-    const float x = fabsf(v) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-    const float p = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
-    const float half = 0.5f * t * p * __builtin_amdgcn_exp2f(x * x * -1.4426950408889634f); // erfc(x) / 2
-    return v * (v < 0.f ? half : 1.f - half);
+    const float a = fabsf(v), w = v * v;
+    const float s = fmaf(fmaf(fmaf(fmaf(fmaf(-6.80949188e-06f, w, 1.11041125e-04f), w, -1.18383719e-03f), w, 9.97228269e-03f), w,
+                              -6.64902106e-02f), w, 3.98942262e-01f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.5f, a, 1.f));
+    const float p = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(-1.39945731e-01f, t, 4.05194312e-01f), t, -3.73826802e-01f), t, 2.40476951e-02f), t,
+                                        3.27784605e-02f), t, 1.51606306e-01f), t, 1.99343786e-01f), t, 1.99474499e-01f);
+    const float below = t * p * __builtin_amdgcn_exp2f(w * -0.72134752044448170f); // Phi(-a)
+    return v * (a < 1.25f ? fmaf(v, s, 0.5f) : (v < 0.f ? below : 1.f - below));
 }
 // v/2 (1 + tanh u) = v / (1 + exp(-2u))
 __device__ __forceinline__ float gelu_tanh(float v) {

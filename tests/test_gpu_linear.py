@@ -2,6 +2,7 @@
 
 The bound of each element is derived in tests/decodeops.py (linear_ref)."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -110,6 +111,41 @@ def test_linear_far_rows(hip, torch_gpu):
     assert L.spinn_hip_linear_workspace_size(C.byref(d)) == 0
     N.check(L.spinn_hip_linear(C.byref(d), ptr(x), ptr(packed), None, None, ptr(y), None, 0, stream()), "linear")
     assert_close(y, *linear_ref(xc, w, 1, None, None, 0, F32), "far rows")
+
+
+@pytest.mark.parametrize("act", [6, 7])
+def test_linear_gelu_accuracy(hip, torch_gpu, act):
+    """Both forms over a dense sweep, in fp32: the residual is the argument, x is zero.
+
+    erf form: Phi near 0 is 1/2 + v S with v S <= 0.4 within 2.2 roundings (polynomial and fit), its sum and the product:
+    under 3 * 2^-24 of |v|; further out Phi(-a) <= 0.11 within 10 roundings and the exponent's two of v^2 / 2: under
+    (10 + v^2) 2^-24 of itself, so that 1 - Phi(-a) and the product stay under 3 * 2^-24 again.
+    tanh form, v / (1 + e), e = exp(-2u): u within 6 roundings, so e within 12 |u| + 2, weighed by e / (1 + e), the sum 1, the
+    reciprocal 2 and the product 1. (1e-37: results below the least normal number.)"""
+    N, L = hip, hip.lib()
+    m, n, k = 512, 2048, 64
+    g = gen(act)
+    v = torch.linspace(-20, 20, m * n).view(m, n).clone()
+    v[:64] = torch.randn(64, n, generator=g) * 0.1
+    v[64:128] = torch.randn(64, n, generator=g) * 2
+    v[0, :8] = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e30, 3e38, 1.25, -1.25])
+    v[1, :2] = torch.tensor([-1e30, -3e38])
+    d = N.LinearDesc(m=m, n=n, k=k, dtype=F32, trans_w=1, act=act)
+    packed, xd, vd = linear_pack(N, d, torch.zeros(n, k, device="cuda")), torch.zeros(m, k, device="cuda"), v.cuda()
+    size = L.spinn_hip_linear_workspace_size(C.byref(d))
+    ws, y = workspace(size), torch.empty(m, n, device="cuda")
+    N.check(L.spinn_hip_linear(C.byref(d), ptr(xd), ptr(packed), None, ptr(vd), ptr(y), ptr(ws), size, stream()), "linear")
+    x, step = v.double(), 2.0 ** -24
+    if act == 6:
+        ref = x * 0.5 * torch.erfc(-x * 0.5 ** 0.5)
+        tol = 3 * step * x.abs()
+        tol = torch.where(x < 0, torch.minimum(tol, (10 + x * x) * step * ref.abs()), tol)
+    else:
+        u = (2 / math.pi) ** 0.5 * (x + 0.044715 * x ** 3)
+        share = torch.sigmoid(-2 * u)  # e / (1 + e)
+        ref = x * torch.sigmoid(2 * u)
+        tol = ref.abs() * step * (4 + (12 * u.abs() + 2) * share)
+    assert_close(y, ref, tol + 1e-37 * (1 + x.abs().clamp(max=100)), f"gelu {act}")
 
 
 def test_linear_values(hip, torch_gpu):
