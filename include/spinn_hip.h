@@ -329,7 +329,7 @@ typedef struct {
  * and `pos` [seqs, kv_heads, acc_stride] take 0 and position[t] (NULL: slot[t]) at that
  * slot in every head (slots from acc_stride on have none). A token whose sequence or slot
  * is outside the cache, or whose page holds nothing, is skipped entirely. Two tokens of
- * one call must not name the same slot. */
+ * one call must not name the same slot. kv_heads * head_dim <= 2^30. */
 int spinn_hip_kv_append(const SpinnHipKvDesc *d, int64_t tokens, const int32_t *seq, const int32_t *slot,
                         const int32_t *position, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
                         const int32_t *page_table, void *k_pages, void *v_pages, float *acc, int32_t *pos,

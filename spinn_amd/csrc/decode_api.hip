@@ -116,6 +116,7 @@ int spinn_hip_kv_append(const SpinnHipKvDesc *d, int64_t tokens, const int32_t *
     if (!kv_ok(d) || tokens < 0 || tokens > (1 << 28)) return SPINN_HIP_EINVAL;
     const int64_t row = (int64_t)d->kv_heads * d->head_dim;
     constexpr int64_t kFar = (int64_t)1 << 32;
+    if (row > (int64_t)1 << 30) return SPINN_HIP_EINVAL; // counted in 31 bits, a step of the workgroup behind its end too
     if (k_stride < row || v_stride < row || k_stride > kFar || v_stride > kFar) return SPINN_HIP_EINVAL;
     if (!seq && tokens > d->seqs) return SPINN_HIP_EINVAL;
     if ((acc || pos) && (acc_stride <= 0 || acc_stride > ((int64_t)1 << 40))) return SPINN_HIP_EINVAL;

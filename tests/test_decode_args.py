@@ -102,6 +102,15 @@ def test_append_arguments(native):
     assert call(tokens=5, seq=P, d=kv_desc(native, seqs=0)) == 0
 
 
+def test_append_rows_past_31_bits(native):
+    """A token's row of all heads is counted in 31 bits: longer ones are refused, not cut short."""
+    L = native.lib()
+    for kv_heads, head_dim in ((1 << 24, 256), (1 << 23, 256), ((1 << 22) + 1, 256)):
+        row = kv_heads * head_dim
+        kv = kv_desc(native, kv_heads=kv_heads, head_dim=head_dim, page_size=1, page_stride=row, head_stride=head_dim, slot_stride=head_dim)
+        assert L.spinn_hip_kv_append(C.byref(kv), 1, None, P, None, P, row, P, row, P, P, P, None, None, 0, None) == EINVAL
+
+
 def test_attention_arguments(native):
     L, N = native.lib(), native
 
