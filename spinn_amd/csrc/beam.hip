@@ -483,20 +483,22 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(BeamArgs a, 
 struct ReorderArgs {
     SpinnHipBeamState s[SPINN_HIP_MAX_BLOCKS];
 };
-// Units of U per row and state: a grid row of workgroups per destination row, the states side by side.
+// Units of U per row and state: `parts` shares of a destination row each, the states side by side; a workgroup takes
+// every gridDim.x-th share.
 template <class U>
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a, const int32_t *__restrict__ parents, int beams,
-                                                           int k, int parts, int rows) {
-    const int64_t blk = blockIdx.x;
-    const int part = (int)(blk % parts);
-    const int row = (int)(blk / parts % rows);
-    const SpinnHipBeamState &s = a.s[blk / parts / rows];
-    const int parent = parents[row];
-    if ((unsigned)parent >= (unsigned)beams) return;
-    const U *src = (const U *)((const char *)s.src + ((int64_t)(row / k) * beams + parent) * s.src_stride);
-    U *dst = (U *)((char *)s.dst + (int64_t)row * s.dst_stride);
-    const int64_t units = s.row_bytes / (int64_t)sizeof(U);
-    for (int64_t u = (int64_t)part * 256 + threadIdx.x; u < units; u += (int64_t)parts * 256) dst[u] = src[u];
+                                                           int k, int parts, int rows, int64_t shares) {
+    for (int64_t blk = blockIdx.x; blk < shares; blk += gridDim.x) {
+        const int part = (int)(blk % parts);
+        const int row = (int)(blk / parts % rows);
+        const SpinnHipBeamState &s = a.s[blk / parts / rows];
+        const int parent = parents[row];
+        if ((unsigned)parent >= (unsigned)beams) continue;
+        const U *src = (const U *)((const char *)s.src + ((int64_t)(row / k) * beams + parent) * s.src_stride);
+        U *dst = (U *)((char *)s.dst + (int64_t)row * s.dst_stride);
+        const int64_t units = s.row_bytes / (int64_t)sizeof(U);
+        for (int64_t u = (int64_t)part * 256 + threadIdx.x; u < units; u += (int64_t)parts * 256) dst[u] = src[u];
+    }
 }
 
 struct Plan {
@@ -593,11 +595,11 @@ int beam_reorder(const SpinnHipBeamState *states, int n, int batch, int beams, i
     const int rows = batch * k;
     // about 16 KB a workgroup, at most 64 workgroups a row
     const int parts = (int)std::min<int64_t>(64, (longest + 16383) / 16384);
-    if ((int64_t)rows * used * parts > INT32_MAX) return SPINN_HIP_EUNSUPPORTED;
-    const unsigned grid = (unsigned)((int64_t)rows * used * parts);
-    if (unit == 16) beam_reorder_kernel<u32x4><<<grid, 256, 0, st>>>(a, parents, beams, k, parts, rows);
-    else if (unit == 4) beam_reorder_kernel<uint32_t><<<grid, 256, 0, st>>>(a, parents, beams, k, parts, rows);
-    else beam_reorder_kernel<uint8_t><<<grid, 256, 0, st>>>(a, parents, beams, k, parts, rows);
+    const int64_t shares = (int64_t)rows * used * parts;
+    const unsigned grid = (unsigned)std::min<int64_t>(shares, 1 << 20); // (a launch has at most 2^32 threads)
+    if (unit == 16) beam_reorder_kernel<u32x4><<<grid, 256, 0, st>>>(a, parents, beams, k, parts, rows, shares);
+    else if (unit == 4) beam_reorder_kernel<uint32_t><<<grid, 256, 0, st>>>(a, parents, beams, k, parts, rows, shares);
+    else beam_reorder_kernel<uint8_t><<<grid, 256, 0, st>>>(a, parents, beams, k, parts, rows, shares);
     return check_launch();
 }
 

@@ -228,3 +228,19 @@ def test_reorder(hip, torch_gpu, row):
                 want[i * k + j, :row] = src[i * w + p, :row]
                 wtab[i * k + j] = tab[i * w + p]
     assert torch.equal(dst.cpu(), want) and torch.equal(dtab.cpu(), wtab)
+
+
+@pytest.mark.parametrize("states,batch,k", [(1, 1 << 20, 4), (5, 1 << 20, 4), (16, 1 << 18, 9)])
+def test_reorder_most_rows(hip, torch_gpu, states, batch, k):
+    """Up to 2^22 rows of up to 16 states, more shares than a launch has workgroups of 256 threads."""
+    N, L, w = hip, hip.lib(), 4
+    g = torch.Generator(device="cuda")
+    g.manual_seed(states)
+    parents = torch.randint(0, w, (batch, k), generator=g, device="cuda", dtype=torch.int32)
+    parents[::7, 1] = -1
+    src = [torch.randint(0, 1 << 30, (batch, w), generator=g, device="cuda", dtype=torch.int32) for _ in range(states)]
+    dst = [torch.full((batch, k), -5, device="cuda", dtype=torch.int32) for _ in range(states)]
+    table = (N.BeamState * states)(*[N.BeamState(ptr(s), ptr(d), 4, 4, 4) for s, d in zip(src, dst)])
+    N.check(L.spinn_hip_beam_reorder(table, states, batch, w, k, ptr(parents), stream()), "reorder")
+    for s, d in zip(src, dst):
+        assert torch.equal(d, torch.where(parents >= 0, s.gather(1, parents.clamp(min=0).long()), -5))
