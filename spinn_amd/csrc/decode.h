@@ -115,6 +115,9 @@ int with_dtype(int dtype, F f) {
     }
 }
 
+// A launch has at most 2^32 threads; one of more wraps without an error and leaves the rest undone.
+inline bool launch_fits(int64_t blocks, int64_t threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
+
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 inline size_t round16(size_t v) { return (v + 15) & ~(size_t)15; }
 

@@ -22,6 +22,7 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kPick = 1024;      // threads of a selecting workgroup, at most
 constexpr int kHeld = 8;         // keys that a thread holds in registers
 constexpr int kMovesPer = 64;    // moves per workgroup of the second launch
+constexpr int kMoveGroups = 1 << 20; // workgroups of it at once
 
 struct EvictArgs {
     const int32_t *table, *lengths, *next_pos, *pos;
@@ -270,10 +271,10 @@ __global__ __launch_bounds__(TH) void evict_pick_kernel(EvictArgs a) {
     if (tid == 0) a.n_moves[row] = moves;
 }
 
-// 16 lanes per move, `U` the unit of copying.
+// 16 lanes per move, `U` the unit of copying. `chunks` workgroups a row, from the first-th share of its moves on.
 template <class U>
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, U *k, U *v, int units, int chunks) {
-    const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a, U *k, U *v, int units, int chunks, int first) {
+    const int row = blockIdx.x / chunks, chunk = first + (int)blockIdx.x - row * chunks;
     const int seq = row / a.kv_heads, head = row - seq * a.kv_heads;
     if (chunk == 0 && head == 0 && threadIdx.x == 0) a.lengths_out[seq] = a.left[seq];
     const int n = a.n_moves[row];
@@ -368,8 +369,7 @@ int kv_evict(const SpinnHipKvEvictDesc *d, const int32_t *table, const int32_t *
     a.recent = d->recent;
     a.sinks = d->sinks;
     a.max_len = d->max_len;
-    const int chunks = std::max(1, (a.most + kMovesPer - 1) / kMovesPer);
-    if ((int64_t)rows * chunks > INT32_MAX) return SPINN_HIP_EUNSUPPORTED;
+    if (!launch_fits((int64_t)rows, kPick)) return SPINN_HIP_EUNSUPPORTED;
     a.runs = d->acc_stride % 4 == 0 && aligned16(acc) && aligned16(pos) && aligned16(acc_out) && aligned16(pos_out);
     if (d->max_len <= 256 * kHeld) evict_pick_kernel<256, true><<<(unsigned)rows, 256, 0, st>>>(a);
     else if (d->max_len <= kPick * kHeld) evict_pick_kernel<kPick, true><<<(unsigned)rows, kPick, 0, st>>>(a);
@@ -384,12 +384,18 @@ int kv_evict(const SpinnHipKvEvictDesc *d, const int32_t *table, const int32_t *
     a.page_stride = kv.page_stride / div;
     a.head_stride = kv.head_stride / div;
     a.slot_stride = kv.slot_stride / div;
-    const unsigned grid = (unsigned)(rows * chunks);
     const int units = kv.head_dim / div;
-    if (vec) evict_move_kernel<<<grid, 256, 0, st>>>(a, (u32x4 *)k, (u32x4 *)v, units, chunks);
-    else if (e == 4) evict_move_kernel<<<grid, 256, 0, st>>>(a, (uint32_t *)k, (uint32_t *)v, units, chunks);
-    else evict_move_kernel<<<grid, 256, 0, st>>>(a, (uint16_t *)k, (uint16_t *)v, units, chunks);
-    return check_launch();
+    // all shares of moves in one launch, unless that has too many workgroups
+    const int chunks = std::max(1, (a.most + kMovesPer - 1) / kMovesPer);
+    const int at_once = (int)std::max<int64_t>(1, std::min<int64_t>(chunks, kMoveGroups / (int64_t)rows));
+    for (int first = 0; first < chunks && !rc; first += at_once) {
+        const unsigned grid = (unsigned)(rows * at_once);
+        if (vec) evict_move_kernel<<<grid, 256, 0, st>>>(a, (u32x4 *)k, (u32x4 *)v, units, at_once, first);
+        else if (e == 4) evict_move_kernel<<<grid, 256, 0, st>>>(a, (uint32_t *)k, (uint32_t *)v, units, at_once, first);
+        else evict_move_kernel<<<grid, 256, 0, st>>>(a, (uint16_t *)k, (uint16_t *)v, units, at_once, first);
+        rc = check_launch();
+    }
+    return rc;
 }
 
 } // namespace spinn

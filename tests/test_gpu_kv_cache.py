@@ -368,6 +368,50 @@ def test_evict_equal_and_odd_weights(hip, torch_gpu):
     evict(hip, c, [-3, 201, 200, 199, 590, 300], acc, pos, [600, 580, 600, 610, -2 ** 31, 2 ** 31 - 1], 200, 64, 0)
 
 
+@pytest.mark.parametrize("seqs,max_len,budget", [(256, 9000, 4500), (2048, 131072, 65536)])
+def test_evict_many_rows_of_great_capacity(hip, torch_gpu, seqs, max_len, budget):
+    """Sizes of many long rows, of which few are in use: more shares of moves than one launch has workgroups of 256 threads.
+    The others are empty and their pages hold nothing."""
+    N, L, kv, page = hip, hip.lib(), 8, 16
+    used = [3, seqs - 2]
+    c = Cache(gen(seqs), F16, 2, kv, 8, page, max_len)
+    n, pages = max_len, c.max_pages
+    table = torch.full((seqs, pages), -1, dtype=torch.int32, device="cuda")
+    table[used] = c.table.cuda()
+    g = gen(1)
+    acc = torch.empty(seqs, kv, n, device="cuda")
+    pos = torch.empty(seqs, kv, n, dtype=torch.int32, device="cuda")
+    w, p = torch.exp(torch.randn(2, kv, n, generator=g)), torch.arange(n, dtype=torch.int32).expand(2, kv, n)
+    acc[used], pos[used] = w.cuda(), p.cuda()
+    lengths = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    lengths[used] = torch.tensor([n, n - 11], dtype=torch.int32).cuda()
+    desc = c.desc(N)
+    desc.seqs = seqs
+    d = N.KvEvictDesc(kv=desc, budget=budget, recent=100, sinks=4, max_len=n, acc_stride=n)
+    size = L.spinn_hip_kv_evict_workspace_size(C.byref(d))
+    ws, kd, vd, next_pos = torch.empty(size, dtype=torch.uint8, device="cuda"), c.k.cuda(), c.v.cuda(), lengths.clone()
+    N.check(L.spinn_hip_kv_evict(C.byref(d), ptr(table), ptr(lengths), ptr(next_pos), ptr(acc), ptr(pos), ptr(acc), ptr(pos),
+                                 ptr(lengths), ptr(kd), ptr(vd), ptr(ws), size, stream()), "evict")
+    assert lengths.tolist() == [budget if s in used else 0 for s in range(seqs)]
+    want = {id(t): t.clone() for t in (c.k, c.v)}
+    for s, length in enumerate((n, n - 11)):
+        key = w[s, :, :length].clone()
+        key[:, :4] = key[:, length - 100:] = math.inf
+        order = torch.sort(key, dim=1, descending=True, stable=True)[1]
+        for h in range(kv):
+            kept = torch.sort(order[h, :budget])[0]
+            to = torch.ones(budget, dtype=torch.bool)
+            to[kept[kept < budget]] = False
+            to, frm, source = torch.nonzero(to)[:, 0], kept[kept >= budget], torch.arange(budget)
+            source[to] = frm
+            assert torch.equal(acc[used[s], h, :budget].cpu(), w[s, h, source])
+            assert torch.equal(pos[used[s], h, :budget].cpu(), source.to(torch.int32))
+            for t in (c.k, c.v):
+                c.view(want[id(t)])[c.table[s, to // page].long(), h, to % page] = c.view(t)[c.table[s, frm // page].long(), h, frm % page]
+    for t, got in ((c.k, kd), (c.v, vd)):
+        assert torch.equal(got.cpu().nan_to_num(nan=-7.0), want[id(t)].nan_to_num(nan=-7.0))
+
+
 def test_evict_twice(hip, torch_gpu):
     """Evict, append, evict again: slots are out of order by then, and the positions carry on."""
     N, L = hip, hip.lib()
