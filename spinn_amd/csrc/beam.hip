@@ -555,7 +555,7 @@ int beam_select(const SpinnHipBeamDesc *d, const void *logits, const float *scor
     a.k = d->k;
     a.end = d->end_token;
     a.chunks = p.chunks;
-    if ((int64_t)a.batch * a.beams * a.chunks > INT32_MAX) return SPINN_HIP_EUNSUPPORTED;
+    if (!launch_fits((int64_t)a.batch * a.beams * a.chunks, kBeamThreads)) return SPINN_HIP_EUNSUPPORTED;
     const int rc = with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
         const int e = 16 / (int)sizeof(T);

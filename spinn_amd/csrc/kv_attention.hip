@@ -606,7 +606,7 @@ int kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, const void *k,
     const int acc_chunks = (d->max_len + kAccSlots - 1) / kAccSlots;
     const int64_t join_blocks = p.splits > 1 ? (int64_t)kv.seqs * d->heads : 0;
     const int64_t acc_blocks = d->accumulate ? (int64_t)kv.seqs * kv.kv_heads * acc_chunks : 0;
-    if (blocks > INT32_MAX || join_blocks + acc_blocks > INT32_MAX) return SPINN_HIP_EUNSUPPORTED;
+    if (!launch_fits(blocks, 64 * p.waves) || !launch_fits(join_blocks + acc_blocks, 256)) return SPINN_HIP_EUNSUPPORTED;
     const size_t hml = (size_t)a.group * 8;
     if (hml > 32768) return SPINN_HIP_EUNSUPPORTED;
     const int rc = with_dtype(kv.dtype, [&](auto t) {

@@ -523,23 +523,27 @@ __global__ __launch_bounds__(256) void linear_pack_x_kernel(const T *__restrict_
 }
 
 template <class T, int MT, int NT, int NW>
-void launch_stream(const LinearArgs &a, Rows rows, hipStream_t st) {
+int launch_stream(const LinearArgs &a, Rows rows, hipStream_t st) {
     const dim3 grid((a.ntiles + NT - 1) / NT, (a.m + 16 * MT - 1) / (16 * MT));
+    if (!launch_fits(grid.x, 64 * NW) || grid.y > 65535) return SPINN_HIP_EUNSUPPORTED;
     if (rows == kRuns) linear_stream_kernel<T, MT, NT, NW, kRuns><<<grid, 64 * NW, 0, st>>>(a);
     else if (rows == kLaidOut) linear_stream_kernel<T, MT, NT, NW, kLaidOut><<<grid, 64 * NW, 0, st>>>(a);
     else if (rows == kLoose) linear_stream_kernel<T, MT, NT, NW, kLoose><<<grid, 64 * NW, 0, st>>>(a);
     else linear_stream_kernel<T, MT, NT, NW, kShort><<<grid, 64 * NW, 0, st>>>(a);
+    return check_launch();
 }
 
 template <class T, int BM, int BN, int WVM, int WVN, int WF>
-void launch_tile(const LinearArgs &a, bool xp, int splits, void *part, hipStream_t st) {
+int launch_tile(const LinearArgs &a, bool xp, int splits, void *part, hipStream_t st) {
     const int mb = (a.m + BM - 1) / BM, nb = (a.ntiles * 16 + BN - 1) / BN;
+    if (!launch_fits((int64_t)mb * nb * splits, 64 * WVM * WVN)) return SPINN_HIP_EUNSUPPORTED;
     const unsigned grid = (unsigned)(mb * nb * splits);
     if (xp) linear_tile_kernel<T, BM, BN, WVM, WVN, WF, true><<<grid, 64 * WVM * WVN, 0, st>>>(a, mb, nb, splits, (f32x4 *)part);
     else linear_tile_kernel<T, BM, BN, WVM, WVN, WF, false><<<grid, 64 * WVM * WVN, 0, st>>>(a, mb, nb, splits, (f32x4 *)part);
     if (splits > 1)
         linear_join_kernel<T, BM, BN, WVM, WVN><<<(unsigned)(((int64_t)mb * nb * (BM * BN / 1024) + 3) / 4), 256, 0, st>>>(
             a, mb, nb, splits, (const f32x4 *)part);
+    return check_launch();
 }
 
 // Which kernel a layer runs on.
@@ -643,9 +647,6 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
     const bool xp = rows == kLaidOut;
     const int64_t tiles = ((m_tiles(d) + 3) / 4) * ((n_tiles(d) + 7) / 8);
     const bool deep = tiles * c.splits <= device_cu_count();
-    // (grids of at most 2^31 workgroups and 65535 rows of them)
-    if (tiles > INT32_MAX / 2 || (c.kind == Choice::kStream && (m_tiles(d) + c.mt - 1) / c.mt > 65535))
-        return SPINN_HIP_EUNSUPPORTED;
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
         if (xp) {
@@ -658,22 +659,19 @@ int linear_run(const SpinnHipLinearDesc *d, const void *x, const void *packed, c
         }
         char *part = (char *)ws + x_bytes(d, c);
         switch (c.kind) {
-        case Choice::kTile256: launch_tile<T, 256, 256, 2, 4, 4>(a, xp, 1, nullptr, st); break;
-        case Choice::kTile128: launch_tile<T, 128, 128, 2, 2, 4>(a, xp, 1, nullptr, st); break;
+        case Choice::kTile256: return launch_tile<T, 256, 256, 2, 4, 4>(a, xp, 1, nullptr, st);
+        case Choice::kTile128: return launch_tile<T, 128, 128, 2, 2, 4>(a, xp, 1, nullptr, st);
         case Choice::kTile64: // one workgroup per CU can have all of its LDS
-            if (deep) launch_tile<T, 64, 128, 2, 2, 8>(a, xp, c.splits, part, st);
-            else launch_tile<T, 64, 128, 2, 2, 4>(a, xp, c.splits, part, st);
-            break;
-        case Choice::kStream:
-            if (c.mt == 4 && c.nt == 4) launch_stream<T, 4, 4, 4>(a, rows, st);
-            else if (c.mt == 4) launch_stream<T, 4, 2, 8>(a, rows, st);
-            else if (c.mt == 2 && c.nt == 4) launch_stream<T, 2, 4, 4>(a, rows, st);
-            else if (c.mt == 2) launch_stream<T, 2, 2, 8>(a, rows, st);
-            else if (c.nt == 2) launch_stream<T, 1, 2, 8>(a, rows, st);
-            else launch_stream<T, 1, 1, 16>(a, rows, st);
-            break;
+            if (deep) return launch_tile<T, 64, 128, 2, 2, 8>(a, xp, c.splits, part, st);
+            return launch_tile<T, 64, 128, 2, 2, 4>(a, xp, c.splits, part, st);
+        default: break;
         }
-        return check_launch();
+        if (c.mt == 4 && c.nt == 4) return launch_stream<T, 4, 4, 4>(a, rows, st);
+        if (c.mt == 4) return launch_stream<T, 4, 2, 8>(a, rows, st);
+        if (c.mt == 2 && c.nt == 4) return launch_stream<T, 2, 4, 4>(a, rows, st);
+        if (c.mt == 2) return launch_stream<T, 2, 2, 8>(a, rows, st);
+        if (c.nt == 2) return launch_stream<T, 1, 2, 8>(a, rows, st);
+        return launch_stream<T, 1, 1, 16>(a, rows, st);
     });
 }
 

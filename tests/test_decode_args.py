@@ -9,6 +9,7 @@ from tests.decodeops import BF16, F16, F32
 P = C.c_void_p(4096)  # never dereferenced
 ODD = C.c_void_p(4097)
 EINVAL, EWORKSPACE = -1, -3
+EUNSUPPORTED = -2
 
 
 def linear_desc(N, **kw):
@@ -202,3 +203,20 @@ def test_reorder_arguments(native):
     assert call([far], batch=1 << 21, beams=4, k=1) == EINVAL and call([far], batch=1 << 21, k=4) == EINVAL
     assert call([N.BeamState(A, B, 64, (1 << 38) + 64, 64)]) == EINVAL
     assert call([], n=0) == 0 and call([ok], batch=0) == 0
+
+
+def test_launches_past_32_bits_of_threads(native):
+    """Grids of more than 2^32 threads, which the runtime would cut short without an error, are refused before anything runs."""
+    L, N = native.lib(), native
+    Q = C.c_void_p(8192)
+    for kw in (dict(m=1, n=1 << 27), dict(m=1 << 24, n=1 << 24, k=1024)):
+        d = linear_desc(N, **kw)
+        assert L.spinn_hip_linear(C.byref(d), P, P, None, None, Q, P, 1 << 62, None) == EUNSUPPORTED, kw
+    b = N.BeamDesc(dtype=F32, batch=1 << 19, beams=64, vocab=100, k=8, logits_stride=100)
+    assert L.spinn_hip_beam_select(C.byref(b), P, P, None, P, P, P, P, 1 << 62, None) == EUNSUPPORTED
+    kv = kv_desc(N, dtype=F32, seqs=1 << 14, kv_heads=8, head_dim=256, page_stride=1 << 16, head_stride=4096, slot_stride=256,
+                 max_pages=1 << 14)
+    a = N.KvAttentionDesc(kv=kv, heads=8, max_len=1 << 18, scale=1.0, q_stride=2048, o_stride=2048)
+    assert L.spinn_hip_kv_attention(C.byref(a), P, P, P, P, P, None, None, None, P, None, P, 1 << 62, None) == EUNSUPPORTED
+    e = N.KvEvictDesc(kv=kv_desc(N, seqs=1 << 20, kv_heads=8, page_stride=8192), budget=4, recent=1, sinks=1, max_len=16, acc_stride=64)
+    assert L.spinn_hip_kv_evict(C.byref(e), P, P, P, P, P, P, P, P, P, P, P, 1 << 62, None) == EUNSUPPORTED
