@@ -96,6 +96,73 @@ def test_linear_in_place(hip, torch_gpu, m):
     run(hip, BF16, m, 256, 192, res=True, bias=True, padr=8, in_place=True)
 
 
+# Layers that run on tiles of the matrix cores on a device of 256 CUs, K long enough for the loop's steady part: (m, n, k),
+# whether K is split (the sums then go through the workspace).
+TILES = [((130, 260, 2056), True), ((200, 1024, 4104), True),  # 64 x 128, split
+         ((70, 8200, 2056), False), ((1030, 1100, 4000), False), ((1568, 2048, 512), False),  # 64 x 128 whole, up to one per CU and more
+         ((2048, 4096, 1000), False), ((1100, 4300, 776), False),  # 128 x 128
+         ((4100, 4200, 520), False)]  # 256 x 256
+
+
+def tiles_on(N, dtype, m, n, k, split, x_unaligned=0):
+    """The workspace beside laid-out rows of x holds the parts of a split, 4 bytes of every element of its tiles each."""
+    d = N.LinearDesc(m=m, n=n, k=k, dtype=dtype, trans_w=1, x_unaligned=x_unaligned)
+    size = N.lib().spinn_hip_linear_workspace_size(C.byref(d))
+    e = TORCH[dtype].itemsize
+    laid = 0
+    if x_unaligned or k * e % 16:
+        laid = (m + 15) // 16 * 16 * -(-k * e // 128) * 128
+    part = (m + 63) // 64 * 64 * (-(-n // 128) * 128) * 4
+    assert size >= laid and (size - laid) % part == 0
+    assert (size - laid) // part >= 2 if split else size == laid
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("mnk,split", TILES, ids=str)
+def test_linear_tiles(hip, torch_gpu, dtype, mnk, split):
+    """Rows of whole runs; rows, columns and K end inside tiles, K one run into a granule."""
+    tiles_on(hip, dtype, *mnk, split)
+    run(hip, dtype, *mnk, bias=True, res=True, act=1)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("mnk,split", TILES, ids=str)
+def test_linear_tiles_loose_rows(hip, torch_gpu, dtype, mnk, split):
+    """x laid out in the workspace first; K ends one element into a granule, or one before its end."""
+    m, n, k = mnk
+    for k in (k // 64 * 64 + 1, k // 64 * 64 - 1):
+        tiles_on(hip, dtype, m, n, k, split, x_unaligned=1)
+        run(hip, dtype, m, n, k, bias=True, padx=2, off=1, trans_w=k & 2 and 1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("mnk,split", [t for t in TILES if t[0][0] in (200, 1568, 1100, 4100)], ids=str)
+@pytest.mark.parametrize("act,bias,res,in_place", [(0, False, False, False), (3, True, False, False), (6, False, True, True),
+                                                   (7, True, True, True)])
+def test_linear_tiles_epilogue(hip, torch_gpu, dtype, mnk, split, act, bias, res, in_place):
+    tiles_on(hip, dtype, *mnk, split)
+    run(hip, dtype, *mnk, act=act, bias=bias, res=res, padr=3 if in_place else 0, in_place=in_place)
+
+
+@pytest.mark.parametrize("mnk,split", TILES, ids=str)
+def test_linear_tiles_values(hip, torch_gpu, mnk, split):
+    """Infinities and NaN on tiles reach the outputs of their row and column alone, at the ends of rows, columns and K, too."""
+    N, L = hip, hip.lib()
+    m, n, k = mnk
+    g = gen(m)
+    x, w = randn(g, m, k, dtype=BF16).cuda(), randn(g, n, k, dtype=BF16, scale=0.125).cuda()
+    x[1, 5], x[m - 1, k - 1], x[m // 2, k // 2] = float("inf"), float("nan"), float("-inf")
+    w[n - 1, k - 1], w[7, 9] = float("inf"), float("nan")
+    d = N.LinearDesc(m=m, n=n, k=k, dtype=BF16, trans_w=1)
+    packed = linear_pack(N, d, w)
+    size = L.spinn_hip_linear_workspace_size(C.byref(d))
+    ws, y = workspace(size, 0xFF), torch.full((m, n), 777.0, device="cuda", dtype=torch.bfloat16)
+    N.check(L.spinn_hip_linear(C.byref(d), ptr(x), ptr(packed), None, None, ptr(y), ptr(ws), size, stream()), "linear")
+    ref = torch.mm(x.float(), w.float().t().contiguous())
+    assert torch.equal(y.isnan(), ref.isnan())
+    assert torch.equal(torch.where(y.isinf(), y.float(), 0.0), torch.where(ref.isinf(), ref, 0.0))
+
+
 def test_linear_far_rows(hip, torch_gpu):
     """Rows whose offsets pass 32 bits of bytes."""
     N, L = hip, hip.lib()
