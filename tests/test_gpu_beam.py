@@ -58,6 +58,21 @@ def test_select_long_lists(hip, torch_gpu, b, w, v, k):
     select(hip, F16, *make(v + k, F16, b, w, v), k)
 
 
+@pytest.mark.parametrize("v,k", [(300001, 20), (200001, 128)])
+@pytest.mark.parametrize("kind", ["ordinary", "equal", "few beams"])
+def test_select_more_lists_than_lanes(hip, torch_gpu, v, k, kind):
+    """64 beams of 19 and 25 chunks: more lists than the 1024 lanes of the joining workgroup, so that lanes have several."""
+    x, s = make(v + k, F16, 1, 64, v)
+    fin = torch.zeros(1, 64, dtype=torch.uint8)
+    if kind == "equal":
+        x = (torch.randint(0, 2, (1, 1, v), generator=gen(k)) * 0.5).half().expand(1, 64, v).contiguous()
+        s[:] = -torch.arange(64).div(16, rounding_mode="floor")
+    elif kind == "few beams":
+        s[0, torch.arange(64) % 5 > 0] = -math.inf
+        fin[0, ::10] = 1
+    select(hip, F16, x, s, k, finished=fin, end=v - 2)
+
+
 def test_select_many_chunks(hip, torch_gpu):
     """Rows cut into chunks of every length: by the rows' number, few or many workgroups."""
     for b in (1, 16, 64):
