@@ -299,20 +299,23 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
         }
 
         if constexpr (sizeof(T) == 2) {
-            // p as two 16-bit parts, the rounding and what it left: the product then carries p to
-            // 2^-16 and better, for one more pass of a unit that is idle. fp16 takes p times 2^14:
-            // its least number is 2^-24, which weights of a long sequence fall under.
-            uint32_t hi[2 * H], lo[2 * H];
+            // p as 16-bit parts, each the rounding of what those before it left, for more passes of a unit that is idle: three
+            // of bf16 hold all 24 bits, two of fp16 carry p to 2^-22. fp16 takes p times 2^14: its least number is 2^-24,
+            // which weights of a long sequence fall under.
+            constexpr int kParts = __is_same(T, __bf16) ? 3 : 2;
+            uint32_t part[kParts][2 * H];
 #pragma unroll
             for (int i = 0; i < 2 * H; ++i) {
-                hi[i] = lo[i] = 0;
+                float v[2] = {p[2 * i] * kPScale, p[2 * i + 1] * kPScale};
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float v = p[2 * i + e] * kPScale;
-                    const T r = (T)v;
-                    const T rest = (T)(v - (float)r);
-                    hi[i] |= (uint32_t) __builtin_bit_cast(uint16_t, r) << (16 * e);
-                    lo[i] |= (uint32_t) __builtin_bit_cast(uint16_t, rest) << (16 * e);
+                for (int w = 0; w < kParts; ++w) {
+                    part[w][i] = 0;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const T r = (T)v[e];
+                        v[e] -= (float)r;
+                        part[w][i] |= (uint32_t) __builtin_bit_cast(uint16_t, r) << (16 * e);
+                    }
                 }
             }
 #pragma unroll
@@ -322,8 +325,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_attend_kernel(AttendArgs a) {
                 for (int i = 0; i < 2 * H; ++i)
                     f[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c / 2], vr[2 * i][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
                 const u32x4 fv = {f[0], f[1], f[2], f[3]};
-                mfma_frag(acc[c], fv, (u32x4){hi[0], hi[1], hi[2], hi[3]}, T());
-                mfma_frag(acc[c], fv, (u32x4){lo[0], lo[1], lo[2], lo[3]}, T());
+#pragma unroll
+                for (int w = 0; w < kParts; ++w) mfma_frag(acc[c], fv, (u32x4){part[w][0], part[w][1], part[w][2], part[w][3]}, T());
             }
         } else {
 #pragma unroll

@@ -213,6 +213,36 @@ def test_attention_one_slot_outweighs_the_rest(hip, torch_gpu, dtype):
     assert_close(o, ref, tol, "o")
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 5), (256, 16)])
+def test_attention_weights_keep_all_bits(hip, torch_gpu, dim, page):
+    """Weights 1, p, 1 over values -h, 1, -l, where h + l are the first 16 bits of p in two bf16 numbers: what is left of p is
+    the result, below 2^-17. p is off by an exponential's 2^-23 (its argument, at most 0.2, by 2^-25), the three terms' sums and
+    their division by three roundings of numbers up to 1 each: 2^-22 of the denominator's 2 to 3 in all."""
+    N, L, n = hip, hip.lib(), 100
+    c = Cache(gen(dim), BF16, n, 1, dim, page, 16)
+    score = (torch.arange(1, n + 1).double() * 2.0 ** -9).bfloat16().double()
+    p = torch.exp(-score)
+    h = p.bfloat16().double()
+    l = (p - h).bfloat16().double()
+    for s in range(n):
+        for i, (key, value) in enumerate(((score[s], -h[s]), (0.0, 1.0), (score[s], -l[s]))):
+            at = int(c.table[s, i // page])
+            c.view(c.k)[at, 0, i % page] = 0
+            c.view(c.k)[at, 0, i % page, 0] = float(key)
+            c.view(c.v)[at, 0, i % page] = float(value)
+    q = torch.zeros(n, 1, dim)
+    q[:, 0, 0] = 1
+    d = N.KvAttentionDesc(kv=c.desc(N), heads=1, max_len=16, scale=1.0, q_stride=dim, o_stride=dim)
+    size = L.spinn_hip_kv_attention_workspace_size(C.byref(d))
+    ws, o = workspace(size), torch.empty(n, dim, dtype=torch.bfloat16, device="cuda")
+    qd, kd, vd, td, ld = q.bfloat16().cuda(), c.k.cuda(), c.v.cuda(), c.table.cuda(), torch.full((n,), 3, dtype=torch.int32).cuda()
+    N.check(L.spinn_hip_kv_attention(C.byref(d), ptr(qd), ptr(kd), ptr(vd), ptr(td), ptr(ld), None, None, None, ptr(o), None, ptr(ws),
+                                     size, stream()), "attention")
+    ref = ((p - h - l) / (2 + p))[:, None].expand(n, dim)
+    assert ref.abs().max() > 8 * 2.0 ** -23
+    assert_close(o, ref, 2.0 ** -22 / 2 + 2.0 ** -8 * ref.abs(), "what is left of p")
+
+
 def test_attention_far_pages(hip, torch_gpu):
     """Pages whose offsets pass 32 bits of elements."""
     N, lib = hip, hip.lib()
