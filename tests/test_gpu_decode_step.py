@@ -265,6 +265,54 @@ def test_step_in_a_graph(hip, torch_gpu, seqs):
             assert torch.equal(x, y), t
 
 
+def test_eviction_in_a_graph(hip, torch_gpu):
+    """Append, attention and eviction captured together, the lengths that eviction leaves on the device read by the next
+    replay's calls: every replay gives the eager calls' bits, with host work and synchronizations between."""
+    torch = torch_gpu
+    N, w = hip, Weights(6)
+    seqs, budget = 6, 200
+    make = lambda: Step(N, w, seqs, 16, 300, accumulate=True)
+    a, b = make(), make()  # a from a graph, b eagerly
+
+    def step(st):
+        d = N.KvEvictDesc(kv=st.kv, budget=budget, recent=20, sinks=2, max_len=st.slots, acc_stride=st.slots)
+        if not hasattr(st, "evict_ws"):
+            st.evict_ws = workspace(st.L.spinn_hip_kv_evict_workspace_size(C.byref(d)))
+        st.slot.copy_(st.lengths)
+        st.lengths += 1
+        st.position += 1
+        st.forward()
+        N.check(st.L.spinn_hip_kv_evict(C.byref(d), ptr(st.table), ptr(st.lengths), ptr(st.position), ptr(st.acc), ptr(st.pos),
+                                        ptr(st.acc), ptr(st.pos), ptr(st.lengths), ptr(st.k), ptr(st.v), ptr(st.evict_ws),
+                                        st.evict_ws.numel(), stream()), "evict")
+
+    step(a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(a)
+    start = torch.tensor([196, 199, 200, 250, 0, 100], dtype=torch.int32)
+    for st in (a, b):
+        g = gen(40)
+        st.k.copy_(torch.randn(st.k.shape, generator=g))
+        st.v.copy_(torch.randn(st.v.shape, generator=g))
+        st.acc.copy_(torch.rand(st.acc.shape, generator=g))
+        st.pos.copy_(torch.arange(st.slots, dtype=torch.int32).expand(st.pos.shape))
+        st.lengths.copy_(start)
+        st.position.copy_(start)
+    want = start.clone()
+    for t in range(8):
+        for st in (a, b):
+            st.h.copy_(torch.randn(seqs, D, generator=gen(50 + t)))
+        graph.replay()
+        step(b)
+        torch.cuda.synchronize()
+        want = torch.clamp(want + 1, max=budget)
+        assert torch.equal(a.lengths.cpu(), want), t
+        for x, y in zip((a.logits, a.o, a.k, a.v, a.acc, a.pos, a.lengths), (b.logits, b.o, b.k, b.v, b.acc, b.pos, b.lengths)):
+            assert torch.equal(x, y), t
+
+
 def test_steps_on_two_streams(hip, torch_gpu):
     """Two programs at once on streams of their own, with buffers of their own."""
     torch = torch_gpu
