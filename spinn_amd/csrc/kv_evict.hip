@@ -33,7 +33,7 @@ struct EvictArgs {
     int32_t *n_moves;   // [rows]
     int32_t *from, *to; // [rows][most]
     int64_t acc_stride, page_stride, head_stride, slot_stride;
-    int32_t seqs, kv_heads, dim, page_size, n_pages, max_pages, budget, recent, sinks, max_len, most;
+    int32_t kv_heads, page_size, n_pages, max_pages, budget, recent, sinks, max_len, most;
     int32_t runs; // rows of acc and pos, in and out, start at multiples of 16 bytes
 };
 
@@ -359,9 +359,7 @@ int kv_evict(const SpinnHipKvEvictDesc *d, const int32_t *table, const int32_t *
     w += round16(4 * rows * a.most);
     a.to = (int32_t *)w;
     a.acc_stride = d->acc_stride;
-    a.seqs = kv.seqs;
     a.kv_heads = kv.kv_heads;
-    a.dim = kv.head_dim;
     a.page_size = kv.page_size;
     a.n_pages = kv.n_pages;
     a.max_pages = kv.max_pages;
