@@ -372,7 +372,8 @@ int spinn_hip_kv_attention(const SpinnHipKvAttentionDesc *d, const void *q, cons
  * free. K and V rows move within the pages. acc_out and pos_out [seqs, kv_heads, acc_stride]
  * take the staying slots' values at their new places (each may be its input itself);
  * lengths_out[s] = min(n, budget) (may be lengths itself). What lies behind it stays
- * as it was. Sequences share no page that is moved within. next_pos[s] is the position
+ * as it was. Sequences share no page that is moved within. A staying slot whose old or new page
+ * holds nothing moves with its weight and position alone. next_pos[s] is the position
  * that the sequence's next token gets.
  */
 typedef struct {
@@ -396,7 +397,9 @@ int spinn_hip_kv_evict(const SpinnHipKvEvictDesc *d, const int32_t *page_table, 
  * rows of vocab, logits_stride apart]; scores fp32 [batch, beams], -inf = an empty beam.
  * A beam with finished[b] != 0 (uint8 [batch, beams], NULL = none) has one continuation, end_token
  * at its score; its other keys are -inf. NaN logits and scores count as -inf, +inf as the
- * largest finite fp32. Keys are compared in 64 bits (within a beam, the logits are).
+ * largest finite fp32. Within a beam the logits are compared. Keys are 64-bit numbers, but the sum in
+ * them is one of fp32 exponentials, within 2^-20 of itself (equal rows have equal sums): keys of
+ * different beams that are no further apart than that may come in either order.
  * out_scores fp32, out_parents and out_tokens int32 [batch, k].
  */
 typedef struct {

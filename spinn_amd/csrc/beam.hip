@@ -8,8 +8,8 @@
 // batch item's chunks, merging their ordered lists by their heads.
 // Bound: memory, each logit read once, and as much again the vector units' work on it (a conversion, a maximum
 // and an exponential each), which overlaps with other workgroups' reading only as far as registers let them be there.
-// 32 x 8 beams of 128000 bf16, k = 16: chunks 23 us (2.8 TB/s), join 10.5; 4 beams of 32000 fp32, k = 8: 5.2 and 6.5,
-// two launches' latency.
+// 32 x 8 beams of 128000 bf16, k = 16: chunks 23 us (2.8 TB/s), join 10.3; 4 beams of
+// 32000 fp32, k = 8: 5.1 and 6.2, two launches' latency.
 #include "decode.h"
 #include <type_traits>
 
@@ -225,7 +225,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(BeamArgs a) {
         if (lane == 0 && pass) atomicAdd(&passing, __popcll(pass));
         again();
 
-        // share of the sum: exponentials in fp32, added in fp64, so that beams compare to about 1e-8
+        // share of the sum: exponentials in fp32 (their arguments rounded once, 2^-24 of themselves, and one step of
+        // the exponential; four added in fp32), then fp64. Within 2^-20; over many alike terms the errors average to 1e-8
         sum = 0.0;
         if (m != -INFINITY) {
             // exp(v - m) = 2^(v L - m L), in one rounding; what m L lost is a factor of the whole sum. Half a step of m L is

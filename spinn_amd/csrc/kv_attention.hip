@@ -5,12 +5,12 @@
 // in one pass with the running maximum m and sum: a tile of slots raises m to m', and what
 // was summed so far is scaled by exp(m - m'). Every row of the cache is read once, for all the
 // query heads of its kv head, so the bound is memory: 2 rows a slot against 4 * heads * head_dim flops.
-// 8 kv heads of 128, bf16: one sequence of 131001 slots 101 us (5.3 TB/s), 32 of 37 to 8000 119 us (4.4 TB/s: the
+// 8 kv heads of 128, bf16: one sequence of 131001 slots 101 us (5.3 TB/s), 32 of 37 to 8000 122 us (4.3 TB/s: the
 // last parts run alone, since the split goes by max_len). 16 x 1500..2000, 16 heads of 80 fp32, with
 // weights: 75 us, 7 of them the second launch.
 //
 // The matrix cores then have time to spare (one new token fills few of a tile's 16 columns, and
-// at 5 TB/s they are still under 5 % busy), which decides the layout: nothing goes through LDS in the
+// at 5 TB/s they are still under 8 % busy), which decides the layout: nothing goes through LDS in the
 // loop. S^T = K Q^T has slots as rows, and lane (g = l/16, n = l%16) ends up with
 // head n, slots 4g..4g+3 of each half tile: exactly the elements that the second product wants
 // from it as its operand (contraction over slots may run in any order, so V's rows
@@ -43,7 +43,7 @@ struct AttendArgs {
     uint32_t page_mul, page_shift; // slot / page_size = slot * page_mul >> 32 + page_shift (page_mul 0: slot)
     int32_t q_runs;        // query rows are whole 16-byte runs
     int32_t part_row;      // dim rounded up to a multiple of 4
-    int32_t splits, chunk; // chunk: slots per split, a multiple of kTile * kWaves
+    int32_t splits, chunk; // chunk: slots per split, a multiple of kStep
     int32_t head_tiles, parts; // parts: seqs * kv_heads * splits
 };
 
