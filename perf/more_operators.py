@@ -363,7 +363,7 @@ def _plain_assign(st):
     ended, add = new == -1, new.clamp(min=0)
     ends = add.cumsum(0)
     starts = (ends - add).clamp(max=st["max_tokens"])
-    fits = (new >= -1) & (length + add <= page * row) & (ends <= st["max_tokens"])
+    fits = (new >= -1) & ((add == 0) | (length + add <= page * row) & (ends <= st["max_tokens"]))
     # pages of ended sequences go on top of the free ones, in the sequences' order
     back = torch.where(ended, held, 0)
     place = st["free_count"].long() + back.cumsum(0) - back
@@ -372,7 +372,7 @@ def _plain_assign(st):
     seat = torch.where(gives, place[:, None] + col, free.numel())
     free = torch.cat([free, free[:1]]).scatter(0, seat.flatten(), torch.where(gives, table, 0).flatten())[:-1]
     count = st["free_count"].long() + back.sum()
-    need = torch.where(fits & ~ended, ((length + add + page - 1) // page - held).clamp(min=0), 0)
+    need = torch.where(fits & (add > 0), ((length + add + page - 1) // page - held).clamp(min=0), 0)
     upto = need.cumsum(0)
     served = fits & ((need == 0) | (upto <= count))
     got = torch.where(served, need, 0)
