@@ -429,6 +429,142 @@ typedef struct {
 int spinn_hip_beam_reorder(const SpinnHipBeamState *states, int n_states, int32_t batch, int32_t beams, int32_t k,
                            const int32_t *parents, void *stream);
 
+/* ---- a prompt: pages for requests, rotary positions, attention, 8-bit linear layers ----
+ *
+ * What a network that generates needs before its first new token and around every step; types, strides, workspaces and
+ * graphs as in the section on a decoding step. */
+
+/*
+ * Pages for the next tokens of every sequence, and where each token goes. Sequence s has lengths[s] slots in a paged
+ * cache, held[s] pages (the first held[s] numbers of its row of page_table), and next_pos[s] as its next token's
+ * position (next_pos = NULL: its length). free_pages [n_pages] holds the free pages' numbers, the first *free_count of
+ * them. new_tokens[s] asks for that many tokens; -1 ends the sequence: its pages go back on top of the free ones, its
+ * length, position and pages become 0.
+ *   starts[s] = sum of max(new_tokens, 0) before s, starts[seqs] = all of them (each at most max_tokens);
+ *   token starts[s] + i goes to slot[..] = lengths[s] + i of seq[..] = s, at position[..] = next_pos[s] + i.
+ * First the ended sequences' pages come back, in the sequences' order; then a sequence of n > 0 tokens needs
+ * max(0, ceil((lengths[s] + n) / page_size) - held[s]) pages, and takes them off the top. It is served if its tokens fit its
+ * row of the table and, with those before it, max_tokens, and if it needs no page or all the pages that it and
+ * those before it need (of the sequences whose tokens fit) are there. served[s] = 1 for those, ended sequences and such without
+ * tokens, else 0 (also for new_tokens < -1): they stay as they are, and their tokens, like those from starts[seqs] on
+ * to max_tokens, get seq = slot = -1 and position = 0, which spinn_hip_kv_append skips.
+ * lengths_out, next_out, held_out and free_count_out may each be its input itself; other arrays overlap nowhere. The rest
+ * of page_table and free_pages stays as it was. Lengths and positions count as at least 0, held and *free_count
+ * as 0 to max_pages and n_pages; seqs = 0 returns at once.
+ */
+typedef struct {
+    int32_t seqs;       /* 0..SPINN_HIP_ASSIGN_MAX_SEQS */
+    int32_t page_size, n_pages, max_pages; /* as in SpinnHipKvDesc */
+    int32_t max_tokens; /* entries of seq, slot and position: 0..2^28 */
+    int32_t reserved;   /* 0 */
+} SpinnHipKvAssignDesc;
+#define SPINN_HIP_ASSIGN_MAX_SEQS 65536
+
+int spinn_hip_kv_assign(const SpinnHipKvAssignDesc *d, const int32_t *new_tokens, const int32_t *lengths,
+                        const int32_t *next_pos, const int32_t *held, const int32_t *free_count, int32_t *free_pages,
+                        int32_t *page_table, int32_t *lengths_out, int32_t *next_out, int32_t *held_out,
+                        int32_t *free_count_out, int32_t *starts, int32_t *served, int32_t *seq, int32_t *slot,
+                        int32_t *position, void *stream);
+
+/* How the frequencies f_i = base^(-2i / rot_dim) of spinn_hip_rope are stretched for contexts longer than the trained ones. */
+enum {
+    SPINN_ROPE_PLAIN = 0,
+    SPINN_ROPE_LINEAR = 1,   /* f_i / factor */
+    SPINN_ROPE_BY_PARTS = 2  /* r = trained f_i / 2 pi turns within the trained positions: f_i from `high` turns on,
+                                f_i / factor up to `low`, between them t f_i + (1 - t) f_i / factor, t = (r - low) / (high - low) */
+};
+
+/*
+ * Rotary positions: in the first rot_dim elements of every head the pair i, elements (2i, 2i + 1) if interleaved, else
+ * (i, i + rot_dim / 2), turns by the angle position[t] f_i:
+ *   y_a = magnitude (cos x_a - sin x_b), y_b = magnitude (sin x_a + cos x_b);
+ * the rest of a head is copied. Head h of token t is at x + t*x_stride + h*x_head_stride, y alike; y may be x itself (same strides),
+ * else they overlap nowhere. Angles are exact to 2^-32 of a turn at any position (negative ones turn back).
+ * The frequencies are laid out once by spinn_hip_rope_table (which reads rot_dim, scaling, base, factor, low, high and
+ * trained alone), 16-byte aligned, and read from `table` afterwards.
+ */
+typedef struct {
+    int32_t dtype;
+    int32_t heads;
+    int32_t head_dim;    /* 2..SPINN_HIP_ROPE_MAX_DIM */
+    int32_t rot_dim;     /* even, 2..head_dim */
+    int32_t interleaved;
+    int32_t scaling;     /* SPINN_ROPE_* */
+    float base;          /* > 0 */
+    float factor;        /* > 0; 1 where scaling is PLAIN */
+    float low, high;     /* BY_PARTS: low < high */
+    int32_t trained;     /* BY_PARTS: trained positions, > 0 */
+    float magnitude;     /* 1 = as it is */
+    int64_t x_stride, x_head_stride, y_stride, y_head_stride;
+} SpinnHipRopeDesc;
+#define SPINN_HIP_ROPE_MAX_DIM 512
+
+size_t spinn_hip_rope_table_size(const SpinnHipRopeDesc *d);
+int spinn_hip_rope_table(const SpinnHipRopeDesc *d, void *table, void *stream);
+int spinn_hip_rope(const SpinnHipRopeDesc *d, int64_t tokens, const int32_t *position, const void *table, const void *x,
+                   void *y, void *stream);
+
+/*
+ * Attention within packed sequences. Sequence s has the rows starts[s] .. starts[s+1] - 1 of q and o, and the rows
+ * kv_starts[s] .. of k and v (kv_starts = NULL: the same):
+ *   o[i,h] = sum_j p_j v_j, p = softmax over the visible j of scale * q[i,h].k_j,
+ * query head h reading kv head h / (heads / kv_heads). Of nk keys row i of nq sees all, or if `causal` those j <= i + nk - nq.
+ * A row that sees none gives o = 0 and lse = -inf. Rows of a sequence's keys and values are finite.
+ * starts and kv_starts [seqs + 1] are on the device, ascend, and are cut to [0, q_rows] and [0, kv_rows]; rows of o
+ * and lse outside every sequence stay as they were, and rows of k and v outside are not read.
+ * Rows of q and o hold heads * head_dim contiguous elements, those of k and v kv_heads * head_dim. lse [q_rows, heads]
+ * fp32 (NULL = not wanted): log of the softmax's denominator. o overlaps no input.
+ * Single tokens over a paged cache: spinn_hip_kv_attention.
+ */
+typedef struct {
+    int32_t dtype;
+    int32_t seqs;
+    int32_t heads, kv_heads; /* heads: multiple of kv_heads */
+    int32_t head_dim;        /* 1..SPINN_HIP_KV_MAX_DIM */
+    int32_t causal;
+    int32_t q_rows, kv_rows; /* rows of q, o and lse, and of k and v; the split and the workspace go by them */
+    float scale;             /* finite */
+    int32_t reserved;        /* 0 */
+    int64_t q_stride, k_stride, v_stride, o_stride; /* up to 2^24 */
+} SpinnHipPromptAttentionDesc;
+
+size_t spinn_hip_prompt_attention_workspace_size(const SpinnHipPromptAttentionDesc *d);
+int spinn_hip_prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const void *k, const void *v,
+                               const int32_t *starts, const int32_t *kv_starts, void *o, float *lse, void *workspace,
+                               size_t workspace_bytes, void *stream);
+
+/*
+ * Rows to 8-bit integers with a scale each: scale[i] = max_j |x[i,j]| / 127 in fp32, xq[i,j] = x[i,j] / scale[i] rounded
+ * to the nearest integer, ties to even (of the exact quotient; 0 where the scale is 0; within +-127). A row with a NaN or an
+ * infinity gets scale NaN and zeros. Rows are ldx and ldq apart; x needs its element's alignment, xq starts at a
+ * multiple of 16, ldq is one and at least k; xq[i, k .. k rounded up to 16) is filled with zeros.
+ */
+int spinn_hip_quantize_rows(int32_t dtype, int64_t rows, int32_t k, const void *x, int64_t ldx, int8_t *xq, int64_t ldq,
+                            float *scale, void *stream);
+
+/*
+ * spinn_hip_linear with x and w in 8-bit integers, scales for each row of x and each of the n channels:
+ *   y[i,j] = act( x_scale[i] w_scale[j] sum_k x[i,k] w(j,k) + bias[j] + residual[i,j] ).
+ * The sum is exact (32-bit integers, k <= SPINN_HIP_I8_MAX_K). w(j,k), bias, residual, y and the packed weights are as
+ * there; dtype is that of bias, residual and y. Rows of x start at multiples of 16 bytes (ldx too, 0 = k rounded up to 16) and
+ * hold k rounded up to 16 bytes that may be read; what is behind k does not count. y overlaps no input but the residual.
+ */
+typedef struct {
+    int32_t m, n, k;
+    int32_t dtype;       /* of bias, residual and y */
+    int32_t trans_w;
+    int32_t act;         /* SPINN_LINEAR_* */
+    int64_t ldx, ldres, ldy;
+} SpinnHipLinearI8Desc;
+#define SPINN_HIP_I8_MAX_K 131071
+
+size_t spinn_hip_linear_i8_packed_size(const SpinnHipLinearI8Desc *d);
+int spinn_hip_linear_i8_pack_weights(const SpinnHipLinearI8Desc *d, const int8_t *w, void *packed_w, void *stream);
+size_t spinn_hip_linear_i8_workspace_size(const SpinnHipLinearI8Desc *d);
+int spinn_hip_linear_i8(const SpinnHipLinearI8Desc *d, const int8_t *x, const float *x_scale, const void *packed_w,
+                        const float *w_scale, const void *bias, const void *residual, void *y, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
 /* ---- device, memory, stream, event and graph plumbing for the host runtime ---- */
 
 int spinn_hip_init(int device);

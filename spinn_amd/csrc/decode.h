@@ -1,11 +1,12 @@
-// decode.h - declarations and element types shared by the decoding-step operators
-// (linear.hip, kv_attention.hip, kv_evict.hip, beam.hip).
+// decode.h - declarations and element types shared by the operators of a decoding step and of a prompt (linear.hip,
+// linear_i8.hip, kv_attention.hip, kv_evict.hip, beam.hip, kv_assign.hip, rope.hip, prompt_attention.hip).
 #pragma once
 #include "spinn_hip_internal.h"
 
 namespace spinn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -13,7 +14,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // 16 bytes of a matrix operand per lane, a fragment of 16 rows or columns by kFrag<T> k:
 // lane l holds row l%16, k = (16 / sizeof(T)) * (l/16) + 0.. . For 16-bit types that is
-// one v_mfma_f32_16x16x32 operand; for fp32 element e of every lane feeds the e-th of four
+// one v_mfma_f32_16x16x32 operand, for 8-bit ones one v_mfma_i32_16x16x64; for fp32 element e of every lane feeds the e-th of four
 // v_mfma_f32_16x16x4_f32 (k = l/16 there: the four take k in another order, the same
 // for both operands). Accumulator element r of lane l is D[4*(l/16) + r][l%16].
 template <class T>
@@ -31,6 +32,9 @@ __device__ __forceinline__ void mfma_frag(f32x4 &c, u32x4 a, u32x4 b, _Float16) 
 __device__ __forceinline__ void mfma_frag(f32x4 &c, u32x4 a, u32x4 b, __bf16) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ void mfma_frag(i32x4 &c, u32x4 a, u32x4 b, int8_t) {
+    c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
 
 // The bits of an element, for copies and transposes.
 template <class T>
@@ -38,6 +42,10 @@ struct Bits;
 template <>
 struct Bits<float> {
     typedef uint32_t type;
+};
+template <>
+struct Bits<int8_t> {
+    typedef uint8_t type;
 };
 template <>
 struct Bits<_Float16> {
@@ -121,6 +129,9 @@ inline bool launch_fits(int64_t blocks, int64_t threads) { return blocks <= (int
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 inline size_t round16(size_t v) { return (v + 15) & ~(size_t)15; }
 
+inline bool multiple_of(const void *p, size_t n) { return ((uintptr_t)p % n) == 0; }
+inline bool workspace_ok(const void *ws, size_t bytes, size_t need) { return need == 0 || (ws && aligned16(ws) && bytes >= need); }
+
 // linear.hip
 size_t linear_packed_bytes(const SpinnHipLinearDesc *d);
 size_t linear_workspace_bytes(const SpinnHipLinearDesc *d);
@@ -149,5 +160,29 @@ int beam_select(const SpinnHipBeamDesc *d, const void *logits, const float *scor
                 float *out_scores, int32_t *out_parents, int32_t *out_tokens, void *ws, hipStream_t st);
 int beam_reorder(const SpinnHipBeamState *states, int n, int batch, int beams, int k, const int32_t *parents,
                  hipStream_t st);
+
+// kv_assign.hip
+int kv_assign(const SpinnHipKvAssignDesc *d, const int32_t *new_tokens, const int32_t *lengths, const int32_t *next,
+              const int32_t *held, const int32_t *free_count, int32_t *free_pages, int32_t *table, int32_t *lengths_out,
+              int32_t *next_out, int32_t *held_out, int32_t *free_count_out, int32_t *starts, int32_t *served, int32_t *seq,
+              int32_t *slot, int32_t *position, hipStream_t st);
+
+// rope.hip
+int rope_table(const SpinnHipRopeDesc *d, void *table, hipStream_t st);
+int rope_run(const SpinnHipRopeDesc *d, int64_t tokens, const int32_t *position, const void *table, const void *x, void *y,
+             hipStream_t st);
+
+// prompt_attention.hip
+size_t prompt_attention_workspace_bytes(const SpinnHipPromptAttentionDesc *d);
+int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const void *k, const void *v, const int32_t *starts,
+                     const int32_t *kv_starts, void *o, float *lse, void *ws, hipStream_t st);
+
+// linear_i8.hip
+int quantize_rows(int dtype, int64_t rows, int k, const void *x, int64_t ldx, int8_t *xq, int64_t ldq, float *scale, hipStream_t st);
+size_t linear_i8_packed_bytes(const SpinnHipLinearI8Desc *d);
+size_t linear_i8_workspace_bytes(const SpinnHipLinearI8Desc *d);
+int linear_i8_pack(const SpinnHipLinearI8Desc *d, const int8_t *w, void *packed, hipStream_t st);
+int linear_i8_run(const SpinnHipLinearI8Desc *d, const int8_t *x, const float *x_scale, const void *packed, const float *w_scale,
+                  const void *bias, const void *res, void *y, void *ws, hipStream_t st);
 
 } // namespace spinn

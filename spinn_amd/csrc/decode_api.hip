@@ -69,10 +69,6 @@ bool beam_ok(const SpinnHipBeamDesc *d) {
     return d->logits_stride >= d->vocab && d->logits_stride <= kFar;
 }
 
-bool multiple_of(const void *p, size_t n) { return ((uintptr_t)p % n) == 0; }
-
-bool workspace_ok(const void *ws, size_t bytes, size_t need) { return need == 0 || (ws && aligned16(ws) && bytes >= need); }
-
 } // namespace
 } // namespace spinn
 

@@ -1,0 +1,437 @@
+// prompt_attention.hip - attention within packed sequences: every row of a prompt over the rows that it sees.
+//
+// o_i = sum_j p_ij v_j, p = softmax over the visible j of scale q_i.k_j, in one pass over the keys with the running maximum and sum.
+// 4 head_dim flops a visible pair: the matrix cores bound it, and beside them the exponentials, one a pair.
+//
+// The rows of a tile are (token, query head of the group) pairs, so that all heads that share a kv head share its
+// tiles in LDS. S^T = K Q^T: an accumulator's column, so a lane, is one row of queries, its maximum and sum
+// are the lane's own and its partner's (lane ^ 32), and a mask is one number a lane. The products' elements that a lane
+// holds are exactly the operand that O^T = V^T P^T wants from it (contraction over keys may run in any order); V^T comes
+// out of LDS transposed by the read itself (16-bit types) or is read element by element (fp32).
+#include "decode.h"
+#include <cmath>
+#include <type_traits>
+
+namespace spinn {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The maximum that a row's weights are relative to may lag behind by 2^kLag, so that sums are rescaled seldom.
+constexpr float kLag = 8.f;
+
+struct PromptArgs {
+    const void *q, *k, *v;
+    void *o;
+    float *lse;
+    const int32_t *starts, *kv_starts;
+    int64_t q_stride, k_stride, v_stride, o_stride;
+    float scale2;      // |scale| log2 e
+    uint32_t flip;     // sign bits of two 16-bit elements or one fp32 where the scale is negative
+    int32_t seqs, heads, kv_heads, group, dim, causal, q_rows, kv_rows;
+    int32_t o_runs;    // rows of o take four elements at a time
+};
+
+// Which tile of which sequence is `item`.
+struct Place {
+    int seq, tile; // seq < 0: none
+};
+__device__ __forceinline__ int clamped(const int32_t *starts, int i, int rows) { return min(max(starts[i], 0), rows); }
+__device__ __forceinline__ int tiles_of(const PromptArgs &a, int s, int rows) {
+    if (s >= a.seqs) return 0;
+    const int n = max(clamped(a.starts, s + 1, a.q_rows) - clamped(a.starts, s, a.q_rows), 0) * a.group;
+    return (n + rows - 1) / rows;
+}
+// Up to 64 sequences: the tiles with the most before them in their sequences first (under a causal mask they have the most keys), so that
+// what starts last is short. More: sequence by sequence, each from its end.
+__device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int rows) {
+    const int lane = threadIdx.x & 63;
+    if (a.seqs <= 64) {
+        const int n = tiles_of(a, lane, rows);
+        int most = n;
+#pragma unroll
+        for (int d = 32; d; d >>= 1) most = max(most, __shfl_xor(most, d));
+        // above(L): tiles numbered above L in their sequences. The least L with above(L) <= item; none if item is behind all.
+        auto above = [&](int L) {
+            int sum = 0;
+            for (int s = 0; s < a.seqs; ++s) sum += max(__builtin_amdgcn_readlane(n, s) - 1 - L, 0);
+            return sum;
+        };
+        if (item >= above(-1)) return {-1, 0};
+        int lo = -1, hi = most - 1;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 63) / 64, L = min(lo + (lane + 1) * step, hi);
+            const int first = __ffsll((unsigned long long)__ballot(above(L) <= item)) - 1;
+            hi = min(lo + (first + 1) * step, hi);
+            lo += first * step;
+        }
+        const int in = item - above(hi);
+        const unsigned long long has = __ballot(n > hi);
+        const bool mine = n > hi && __popcll(has & ((1ull << lane) - 1)) == in;
+        return {__ffsll((unsigned long long)__ballot(mine)) - 1, hi};
+    }
+    int first = 0, left = a.seqs, before = 0;
+    while (true) { // 64 shares of the sequences left, until a share is one
+        const int each = (left + 63) / 64;
+        int n = 0;
+        for (int i = 0; i < each; ++i) {
+            const int s = lane * each + i;
+            if (s < left) n += tiles_of(a, first + s, rows);
+        }
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(upto, d);
+            if (lane >= d) upto += o;
+        }
+        const unsigned long long behind = __ballot(before + upto > item);
+        if (!behind) return {-1, 0};
+        const int w = __ffsll(behind) - 1;
+        before += __shfl(upto - n, w);
+        const int tiles = __shfl(n, w);
+        first += w * each;
+        left = min(each, left - w * each);
+        if (each == 1) return {first, tiles - 1 - (item - before)};
+    }
+}
+
+// How 16-byte runs of a row lie in LDS, so that lanes that read a column of them, and lanes that read pieces of four rows, meet all banks.
+template <class T, int DP>
+struct Tile {
+    static constexpr int E = 16 / (int)sizeof(T);
+    static constexpr int kRow = DP * (int)sizeof(T);  // bytes
+    static constexpr int kRuns = kRow / 16;
+    static constexpr int kPow2 = (kRuns & -kRuns) < 16 ? (kRuns & -kRuns) : 16; // runs that may change places among each other
+    __device__ __forceinline__ static int k_run(int row, int run) { return run ^ ((row / (16 / kPow2)) & (kPow2 - 1)); }
+    static constexpr int kBlocks = kRow / 64, kBlockPow2 = (kBlocks & -kBlocks) < 4 ? (kBlocks & -kBlocks) : 4;
+    __device__ __forceinline__ static int v_run(int row, int run) {
+        if constexpr (sizeof(T) == 2) return run ^ (((row / (4 / kBlockPow2)) & (kBlockPow2 - 1)) << 2);
+        else return DP % 64 == 0 ? run ^ (((row >> 2) & 1) << 3) : run;
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, _Float16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, __bf16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, float) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, (uint32_t)a[e]), __builtin_bit_cast(float, (uint32_t)b[e]), c, 0, 0, 0);
+    return c;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    T2 v;
+    v[0] = (T)a;
+    v[1] = (T)b;
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+__device__ __forceinline__ float other_half(float v) { // lane ^ 32's
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & 32) ? r[0] : r[1]));
+}
+
+__device__ __forceinline__ void async_run(const char *src, char *lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+// This wave's copies have landed and its LDS reads are done, and so are every other wave's.
+__device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// T: element; DP: head_dim padded to a multiple of 32; KB: keys of a tile; QB: blocks of 32 rows per wave;
+// RUNS: rows of q, k and v are whole, aligned 16-byte runs.
+template <class T, int DP, int KB, int QB, bool RUNS>
+__global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kernel(PromptArgs a) {
+    typedef Tile<T, DP> Lay;
+    constexpr int E = Lay::E, kRow = Lay::kRow, NC = kRow / 32; // NC: operand pieces of a row
+    constexpr int B = KB / 32, DB = DP / 32;
+    constexpr int BM = 128 * QB;
+    constexpr int kTile = KB * kRow;                     // bytes of a tile of K or V
+    constexpr int PI = kTile / 1024 / 4;                 // a wave's 1 KB copies of one
+    static_assert(kTile % 4096 == 0, "");
+    // fp16's weights are kept 2^7 higher: its least number is 2^-24, which many small ones together fall under
+    constexpr float kUp = __is_same(T, _Float16) ? 7.f : 0.f;
+    __shared__ __attribute__((aligned(16))) char lds[4 * kTile]; // K, V of the even tiles, then of the odd ones
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int kvh = (int)blockIdx.x % a.kv_heads, item = (int)blockIdx.x / a.kv_heads;
+    const Place at = find_place(a, item, BM);
+    const int seq = __builtin_amdgcn_readfirstlane(at.seq);
+    if (seq < 0) return;
+    const int q0 = clamped(a.starts, seq, a.q_rows), nq = clamped(a.starts, seq + 1, a.q_rows) - q0;
+    const int32_t *ks = a.kv_starts ? a.kv_starts : a.starts;
+    const int k0 = clamped(ks, seq, a.kv_rows), nk = max(clamped(ks, seq + 1, a.kv_rows) - k0, 0);
+    const int rows = nq * a.group, row0 = __builtin_amdgcn_readfirstlane(at.tile) * BM;
+    // rows beyond the last take part as copies of it
+    auto limit_of = [&](int row) { // keys that a row sees
+        return a.causal ? min(max(min(row, rows - 1) / a.group + nk - nq + 1, 0), nk) : nk;
+    };
+    const int wrow = row0 + wave * 32 * QB;
+    const int wave_min = limit_of(wrow), wave_max = limit_of(wrow + 32 * QB - 1), most = limit_of(row0 + BM - 1);
+    int limit[QB];
+    int head[QB], token[QB]; // of a lane's rows, the token from the sequence's first
+    u32x4 q[QB][NC];
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        const int row = wrow + 32 * i + n, r = min(row, rows - 1);
+        limit[i] = limit_of(row);
+        token[i] = r / a.group;
+        head[i] = kvh * a.group + (r - token[i] * a.group);
+        const T *qp = (const T *)a.q + (int64_t)(q0 + token[i]) * a.q_stride + (int64_t)head[i] * a.dim;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d0 = (2 * c + h) * E;
+            if constexpr (RUNS) q[i][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
+            else q[i][c] = load_edge<T>(qp + d0, a.dim - d0);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) q[i][c][w] ^= a.flip;
+        }
+    }
+
+    const char *kb = (const char *)((const T *)a.k + (int64_t)k0 * a.k_stride + (int64_t)kvh * a.dim);
+    const char *vb = (const char *)((const T *)a.v + (int64_t)k0 * a.v_stride + (int64_t)kvh * a.dim);
+    const uint32_t k_bytes = (uint32_t)(a.k_stride * (int)sizeof(T)), v_bytes = (uint32_t)(a.v_stride * (int)sizeof(T));
+    auto fetch = [&](int t, int buf) { // tile t; rows behind the last key are copies of it
+        const int left = nk - t * KB - 1; // last row of the tile that there is
+        const char *kt = kb + (int64_t)t * KB * k_bytes, *vt = vb + (int64_t)t * KB * v_bytes;
+        char *to = lds + buf * 2 * kTile + wave * PI * 1024;
+#pragma unroll
+        for (int p = 0; p < PI; ++p) {
+            const int off = (wave * PI + p) * 1024 + lane * 16, row = off / kRow, run = off % kRow / 16;
+            const int from = min(row, left);
+            const int kr = Lay::k_run(row, run), vr = Lay::v_run(row, run);
+            if constexpr (RUNS) {
+                if (kr * E < a.dim) async_run(kt + ((uint32_t)from * k_bytes + (uint32_t)kr * 16u), to + p * 1024);
+                if (vr * E < a.dim) async_run(vt + ((uint32_t)from * v_bytes + (uint32_t)vr * 16u), to + kTile + p * 1024);
+            } else {
+                const T *kp = (const T *)(kt + (int64_t)from * k_bytes), *vp = (const T *)(vt + (int64_t)from * v_bytes);
+                uint32_t kw[4], vw[4];
+                if (a.dim >= E) {
+                    load_loose<T, E>(kp, kr * E, a.dim, kw);
+                    load_loose<T, E>(vp, vr * E, a.dim, vw);
+                } else {
+                    const u32x4 x = load_edge<T>(kp + kr * E, a.dim - kr * E), y = load_edge<T>(vp + vr * E, a.dim - vr * E);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        kw[w] = x[w];
+                        vw[w] = y[w];
+                    }
+                }
+                *reinterpret_cast<u32x4 *>(to + p * 1024 + lane * 16) = (u32x4){kw[0], kw[1], kw[2], kw[3]};
+                *reinterpret_cast<u32x4 *>(to + kTile + p * 1024 + lane * 16) = (u32x4){vw[0], vw[1], vw[2], vw[3]};
+            }
+        }
+    };
+    if (RUNS && a.dim < DP) { // runs behind dim are never fetched; K's count as zeros
+        for (int i = threadIdx.x; i < 4 * kTile / 16; i += 256) reinterpret_cast<u32x4 *>(lds)[i] = (u32x4){0, 0, 0, 0};
+        __syncthreads();
+    }
+
+    // where a lane reads: K's row n (+ 32 a block), piece c; V's rows 4h + (lane % 16) / 4 (+ 8, + 16 cc, + 32 b), columns of block db
+    // (the swap of runs is among the first ones; the others follow at the same distances)
+    constexpr int NK = Lay::kPow2 / 2, NV = sizeof(T) == 2 ? Lay::kBlockPow2 : (DP % 64 == 0 ? 2 : 1);
+    int k_off[NK], v_off[NV];
+#pragma unroll
+    for (int c = 0; c < NK; ++c) k_off[c] = n * kRow + Lay::k_run(n, 2 * c + h) * 16;
+#pragma unroll
+    for (int d = 0; d < NV; ++d) {
+        if constexpr (sizeof(T) == 2) {
+            const int row = 4 * h + (lane & 15) / 4, run = 4 * d + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
+            v_off[d] = row * kRow + Lay::v_run(row, run) * 16 + (lane & 1) * 8;
+        } else {
+            const int row = 4 * h, run = 8 * d + n / 4;
+            v_off[d] = row * kRow + Lay::v_run(row, run) * 16 + (n & 3) * 4;
+        }
+    }
+
+    f32x16 o[QB][DB] = {};
+    float m[QB], l[QB]; // base 2; l: this lane's half of the keys
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+    }
+    const int tiles = (most + KB - 1) / KB;
+    if (tiles > 0) fetch(0, 0);
+    for (int t = 0; t < tiles; ++t) {
+        all_ready(); // tile t is there, and every wave is done with tile t - 1
+        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+        const int first = t * KB;
+        if (first >= wave_max) continue;
+        const char *kt = lds + (t & 1) * 2 * kTile, *vt = kt + kTile;
+
+        f32x16 s[QB][B] = {};
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const u32x4 kf = *reinterpret_cast<const u32x4 *>(kt + k_off[c % NK] + c / NK * NK * 32 + b * 32 * kRow);
+#pragma unroll
+                for (int i = 0; i < QB; ++i) s[i][b] = mfma32(kf, q[i][c], s[i][b], T());
+            }
+        if (first + KB > wave_min) {
+#pragma unroll
+            for (int i = 0; i < QB; ++i)
+#pragma unroll
+                for (int b = 0; b < B; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (first + 32 * b + 8 * (r / 4) + 4 * h + r % 4 >= limit[i]) s[i][b][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            float top = s[i][0][0];
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][b][r]);
+            top = fmaxf(top, other_half(top)) * a.scale2;
+            if (__any(top > m[i] + kLag)) {
+                const float to = fmaxf(m[i], top), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - to);
+                m[i] = to;
+                l[i] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[i][d] *= alpha;
+            }
+            const float base = m[i] == -INFINITY ? 0.f : m[i] - kUp;
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[i][b][r] = __builtin_amdgcn_exp2f(fmaf(s[i][b][r], a.scale2, -base));
+                    l[i] += s[i][b][r];
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if constexpr (sizeof(T) == 2) {
+                // weights enter the second product rounded once to T, as its operands have to be: off by half a step of T each, where
+                // the result is rounded by as much (their sum is taken of the unrounded ones)
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    u32x4 p[QB];
+#pragma unroll
+                    for (int i = 0; i < QB; ++i)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) p[i][w] = pack2<T>(s[i][b][8 * cc + 2 * w], s[i][b][8 * cc + 2 * w + 1]);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        typedef __attribute__((address_space(3))) s16x4 *Piece;
+                        const char *vp = vt + v_off[d % NV] + d / NV * NV * 64 + (32 * b + 16 * cc) * kRow;
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)vp);
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)(vp + 8 * kRow));
+                        const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
+                        const u32x4 vf = {wl[0], wl[1], wh[0], wh[1]};
+#pragma unroll
+                        for (int i = 0; i < QB; ++i) o[i][d] = mfma32(vf, p[i], o[i][d], T());
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const float vf = *reinterpret_cast<const float *>(vt + v_off[d % NV] + d / NV * NV * 128 + (32 * b + 8 * (r / 4) + r % 4) * kRow);
+#pragma unroll
+                        for (int i = 0; i < QB; ++i) o[i][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[i][b][r], o[i][d], 0, 0, 0);
+                    }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        const int row = wrow + 32 * i + n;
+        const float sum = l[i] + other_half(l[i]);
+        if (row >= rows) continue;
+        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+        const int64_t grow = q0 + token[i];
+        T *op = (T *)a.o + grow * a.o_stride + (int64_t)head[i] * a.dim;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int at4 = 32 * d + 8 * r4 + 4 * h;
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                T4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (T)(o[i][d][4 * r4 + e] * inv);
+                if (a.o_runs) {
+                    if (at4 < a.dim) *reinterpret_cast<T4 *>(op + at4) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at4 + e < a.dim) op[at4 + e] = v[e];
+                }
+            }
+        if (a.lse && h == 0) a.lse[grow * a.heads + head[i]] = sum == 0.f ? -INFINITY : (m[i] - kUp + __log2f(sum)) * kLn2;
+    }
+}
+
+template <class T, int DP, int KB, int QB>
+int launch(const PromptArgs &a, bool runs, hipStream_t st) {
+    constexpr int BM = 128 * QB;
+    const int64_t items = (int64_t)a.q_rows * a.group / BM + std::min(a.seqs, a.q_rows);
+    const int64_t grid = items * a.kv_heads;
+    if (!launch_fits(grid, 256)) return SPINN_HIP_EUNSUPPORTED;
+    if (runs) prompt_kernel<T, DP, KB, QB, true><<<(unsigned)grid, 256, 0, st>>>(a);
+    else prompt_kernel<T, DP, KB, QB, false><<<(unsigned)grid, 256, 0, st>>>(a);
+    return check_launch();
+}
+
+} // namespace
+
+size_t prompt_attention_workspace_bytes(const SpinnHipPromptAttentionDesc *) { return 0; }
+
+int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const void *k, const void *v, const int32_t *starts,
+                     const int32_t *kv_starts, void *o, float *lse, void *ws, hipStream_t st) {
+    (void)ws;
+    PromptArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.o = o;
+    a.lse = lse;
+    a.starts = starts;
+    a.kv_starts = kv_starts;
+    a.q_stride = d->q_stride;
+    a.k_stride = d->k_stride;
+    a.v_stride = d->v_stride;
+    a.o_stride = d->o_stride;
+    // a scale of (nearly) nothing still multiplies the -inf of hidden keys
+    a.scale2 = std::max(std::fabs(d->scale) * kLog2e, 1e-37f);
+    const int e = dtype_bytes(d->dtype);
+    a.flip = d->scale < 0 ? (e == 2 ? 0x80008000u : 0x80000000u) : 0u;
+    a.seqs = d->seqs;
+    a.heads = d->heads;
+    a.kv_heads = d->kv_heads;
+    a.group = d->heads / d->kv_heads;
+    a.dim = d->head_dim;
+    a.causal = d->causal;
+    a.q_rows = d->q_rows;
+    a.kv_rows = d->kv_rows;
+    const int per = 16 / e;
+    const bool runs = a.dim % per == 0 && (d->q_stride | d->k_stride | d->v_stride) % per == 0 && aligned16(q) && aligned16(k) && aligned16(v);
+    a.o_runs = a.dim % 4 == 0 && d->o_stride % 4 == 0 && multiple_of(o, 4 * e);
+    return with_dtype(d->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        constexpr int K = sizeof(T) == 2 ? 64 : 32;
+        if (a.dim <= 64) return launch<T, 64, K, 1>(a, runs, st);
+        if (a.dim <= 96) return launch<T, 96, K, 1>(a, runs, st);
+        if (a.dim <= 128) return launch<T, 128, K, 1>(a, runs, st);
+        return launch<T, 256, 32, 1>(a, runs, st);
+    });
+}
+
+} // namespace spinn

@@ -38,6 +38,8 @@ MAX_BLOCKS = 16
 TYPE_FLOAT32, TYPE_FLOAT16, TYPE_BFLOAT16 = 1, 10, 16  # ENNF_TYPE_*
 LINEAR_NONE, LINEAR_RELU, LINEAR_SILU, LINEAR_GELU, LINEAR_GELU_TANH = 0, 1, 3, 6, 7
 KV_MAX_DIM, BEAM_MAX, BEAM_MAX_K = 256, 64, 128
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BY_PARTS = 0, 1, 2
+ASSIGN_MAX_SEQS, ROPE_MAX_DIM, I8_MAX_K = 65536, 512, 131071
 
 
 class ConvDesc(C.Structure):
@@ -101,6 +103,28 @@ class BeamDesc(C.Structure):
 class BeamState(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("row_bytes", C.c_int64), ("src_stride", C.c_int64),
                 ("dst_stride", C.c_int64)]
+
+
+class KvAssignDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("seqs", "page_size", "n_pages", "max_pages", "max_tokens", "reserved")]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "heads", "head_dim", "rot_dim", "interleaved", "scaling")] + \
+               [(n, C.c_float) for n in ("base", "factor", "low", "high")] + \
+               [("trained", C.c_int32), ("magnitude", C.c_float)] + \
+               [(n, C.c_int64) for n in ("x_stride", "x_head_stride", "y_stride", "y_head_stride")]
+
+
+class PromptAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "seqs", "heads", "kv_heads", "head_dim", "causal", "q_rows", "kv_rows")] + \
+               [("scale", C.c_float), ("reserved", C.c_int32)] + \
+               [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "o_stride")]
+
+
+class LinearI8Desc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("m", "n", "k", "dtype", "trans_w", "act")] + \
+               [(n, C.c_int64) for n in ("ldx", "ldres", "ldy")]
 
 
 class SpinnTensor(C.Structure):
@@ -215,6 +239,18 @@ _SIGS = {
     "spinn_hip_beam_select": (C.c_int, [C.POINTER(BeamDesc)] + [C.c_void_p] * 7 + [C.c_size_t, C.c_void_p]),
     "spinn_hip_beam_reorder": (C.c_int, [C.POINTER(BeamState), C.c_int, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                          C.c_void_p]),
+    "spinn_hip_kv_assign": (C.c_int, [C.POINTER(KvAssignDesc)] + [C.c_void_p] * 17),
+    "spinn_hip_rope_table_size": (C.c_size_t, [C.POINTER(RopeDesc)]),
+    "spinn_hip_rope_table": (C.c_int, [C.POINTER(RopeDesc), C.c_void_p, C.c_void_p]),
+    "spinn_hip_rope": (C.c_int, [C.POINTER(RopeDesc), C.c_int64] + [C.c_void_p] * 5),
+    "spinn_hip_prompt_attention_workspace_size": (C.c_size_t, [C.POINTER(PromptAttentionDesc)]),
+    "spinn_hip_prompt_attention": (C.c_int, [C.POINTER(PromptAttentionDesc)] + [C.c_void_p] * 8 + [C.c_size_t, C.c_void_p]),
+    "spinn_hip_quantize_rows": (C.c_int, [C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                          C.c_void_p, C.c_void_p]),
+    "spinn_hip_linear_i8_packed_size": (C.c_size_t, [C.POINTER(LinearI8Desc)]),
+    "spinn_hip_linear_i8_pack_weights": (C.c_int, [C.POINTER(LinearI8Desc), C.c_void_p, C.c_void_p, C.c_void_p]),
+    "spinn_hip_linear_i8_workspace_size": (C.c_size_t, [C.POINTER(LinearI8Desc)]),
+    "spinn_hip_linear_i8": (C.c_int, [C.POINTER(LinearI8Desc)] + [C.c_void_p] * 8 + [C.c_size_t, C.c_void_p]),
     "spinn_hip_init": (C.c_int, [C.c_int]),
     "spinn_hip_device_count": (C.c_int, [C.POINTER(C.c_int)]),
     "spinn_hip_malloc": (C.c_int, [C.POINTER(C.c_void_p), C.c_size_t]),
