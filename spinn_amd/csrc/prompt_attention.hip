@@ -32,46 +32,48 @@ struct PromptArgs {
     float scale2;      // |scale| log2 e
     uint32_t flip;     // sign bits of two 16-bit elements or one fp32 where the scale is negative
     int32_t seqs, heads, kv_heads, group, dim, causal, q_rows, kv_rows;
-    int32_t o_runs;    // rows of o take four elements at a time
+    uint32_t group_mul, group_shift; // row / group = row * group_mul >> 32 + group_shift (group_mul 0: row)
+    int32_t o_runs;    // rows of o are whole, aligned 16-byte runs
 };
 
-// Which tile of which sequence is `item`.
+__device__ __forceinline__ int token_of(const PromptArgs &a, int row) {
+    return a.group_mul ? (int)(__umulhi((uint32_t)row, a.group_mul) >> a.group_shift) : row;
+}
+
+// Which tile of which sequence is `item`, and the sequence's rows.
 struct Place {
-    int seq, tile; // seq < 0: none
+    int tile; // < 0: none
+    int q0, nq, k0, nk;
 };
 __device__ __forceinline__ int clamped(const int32_t *starts, int i, int rows) { return min(max(starts[i], 0), rows); }
-__device__ __forceinline__ int tiles_of(const PromptArgs &a, int s, int rows) {
-    if (s >= a.seqs) return 0;
-    const int n = max(clamped(a.starts, s + 1, a.q_rows) - clamped(a.starts, s, a.q_rows), 0) * a.group;
-    return (n + rows - 1) / rows;
-}
-// Up to 64 sequences: the tiles with the most before them in their sequences first (under a causal mask they have the most keys), so that
-// what starts last is short. More: sequence by sequence, each from its end.
+// Sequence by sequence, so that what runs at a time shares keys in the L2 (24 sequences of 37 to 2000 rows: 406 us; all their last
+// tiles first, then the ones before them, 421), each from its end, where a causal mask leaves the most keys. Up to 64, one a
+// lane, the longest first, so that what starts last is short.
 __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int rows) {
     const int lane = threadIdx.x & 63;
+    const int32_t *ks = a.kv_starts ? a.kv_starts : a.starts;
     if (a.seqs <= 64) {
-        const int n = tiles_of(a, lane, rows);
-        int most = n;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) most = max(most, __shfl_xor(most, d));
-        // above(L): tiles numbered above L in their sequences. The least L with above(L) <= item; none if item is behind all.
-        auto above = [&](int L) {
-            int sum = 0;
-            for (int s = 0; s < a.seqs; ++s) sum += max(__builtin_amdgcn_readlane(n, s) - 1 - L, 0);
-            return sum;
-        };
-        if (item >= above(-1)) return {-1, 0};
-        int lo = -1, hi = most - 1;
-        while (hi - lo > 1) {
-            const int step = (hi - lo + 63) / 64, L = min(lo + (lane + 1) * step, hi);
-            const int first = __ffsll((unsigned long long)__ballot(above(L) <= item)) - 1;
-            hi = min(lo + (first + 1) * step, hi);
-            lo += first * step;
+        const int s = min(lane, a.seqs - 1);
+        const int q0 = clamped(a.starts, s, a.q_rows), q1 = clamped(a.starts, s + 1, a.q_rows);
+        const int k0 = clamped(ks, s, a.kv_rows), k1 = clamped(ks, s + 1, a.kv_rows);
+        const int n = lane < a.seqs ? (max(q1 - q0, 0) * a.group + rows - 1) / rows : 0;
+        // tiles of the sequences that come first: more tiles, or as many and an earlier lane
+        const uint64_t key = (uint64_t)n << 32 | (uint32_t)(64 - lane);
+        int before = 0;
+        if (a.seqs > 1) {
+#pragma unroll 8
+            for (int i = 0; i < ((a.seqs + 7) & ~7); ++i) { // lanes behind the last sequence have no tiles
+                const int o = __builtin_amdgcn_readlane(n, i);
+                before += ((uint64_t)(uint32_t)o << 32 | (uint32_t)(64 - i)) > key ? o : 0;
+            }
         }
-        const int in = item - above(hi);
-        const unsigned long long has = __ballot(n > hi);
-        const bool mine = n > hi && __popcll(has & ((1ull << lane) - 1)) == in;
-        return {__ffsll((unsigned long long)__ballot(mine)) - 1, hi};
+        const unsigned long long mine = __ballot(item >= before && item - before < n);
+        const int seq = __ffsll(mine) - 1;
+        if (seq < 0) return {-1, 0, 0, 0, 0};
+        const int tile = __builtin_amdgcn_readlane(n - 1 - (item - before), seq);
+        const int first = __builtin_amdgcn_readlane(q0, seq), kfirst = __builtin_amdgcn_readlane(k0, seq);
+        return {tile, first, __builtin_amdgcn_readlane(q1, seq) - first, kfirst,
+                max(__builtin_amdgcn_readlane(k1, seq) - kfirst, 0)};
     }
     int first = 0, left = a.seqs, before = 0;
     while (true) { // 64 shares of the sequences left, until a share is one
@@ -79,7 +81,8 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
         int n = 0;
         for (int i = 0; i < each; ++i) {
             const int s = lane * each + i;
-            if (s < left) n += tiles_of(a, first + s, rows);
+            if (s < left)
+                n += (max(clamped(a.starts, first + s + 1, a.q_rows) - clamped(a.starts, first + s, a.q_rows), 0) * a.group + rows - 1) / rows;
         }
         int upto = n;
 #pragma unroll
@@ -88,13 +91,16 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
             if (lane >= d) upto += o;
         }
         const unsigned long long behind = __ballot(before + upto > item);
-        if (!behind) return {-1, 0};
+        if (!behind) return {-1, 0, 0, 0, 0};
         const int w = __ffsll(behind) - 1;
-        before += __shfl(upto - n, w);
-        const int tiles = __shfl(n, w);
+        before += __builtin_amdgcn_readlane(upto - n, w);
         first += w * each;
         left = min(each, left - w * each);
-        if (each == 1) return {first, tiles - 1 - (item - before)};
+        if (each == 1) {
+            const int q0 = clamped(a.starts, first, a.q_rows), k0 = clamped(ks, first, a.kv_rows);
+            return {__builtin_amdgcn_readlane(n, w) - 1 - (item - before), q0, clamped(a.starts, first + 1, a.q_rows) - q0, k0,
+                    max(clamped(ks, first + 1, a.kv_rows) - k0, 0)};
+        }
     }
 }
 
@@ -141,9 +147,15 @@ __device__ __forceinline__ float other_half(float v) { // lane ^ 32's
     return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & 32) ? r[0] : r[1]));
 }
 
-__device__ __forceinline__ void async_run(const char *src, char *lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+// 16 bytes a lane from base + off to lds + 16 lane; all_ready() waits for it. In assembly, since the compiler would wait for all
+// of these before every transposing read of LDS that follows, whatever it reads (16000 rows: 2020 -> 1916 us).
+__device__ __forceinline__ void async_run(const char *base, uint32_t off, const char *lds) {
+    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void async_run(const char *from, const char *lds) { // from an address of its own each
+    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory", "m0");
 }
 
 // This wave's copies have landed and its LDS reads are done, and so are every other wave's.
@@ -167,53 +179,45 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
     const int n = lane & 31, h = lane >> 5;
     const int kvh = (int)blockIdx.x % a.kv_heads, item = (int)blockIdx.x / a.kv_heads;
     const Place at = find_place(a, item, BM);
-    const int seq = __builtin_amdgcn_readfirstlane(at.seq);
-    if (seq < 0) return;
-    const int q0 = clamped(a.starts, seq, a.q_rows), nq = clamped(a.starts, seq + 1, a.q_rows) - q0;
-    const int32_t *ks = a.kv_starts ? a.kv_starts : a.starts;
-    const int k0 = clamped(ks, seq, a.kv_rows), nk = max(clamped(ks, seq + 1, a.kv_rows) - k0, 0);
-    const int rows = nq * a.group, row0 = __builtin_amdgcn_readfirstlane(at.tile) * BM;
+    if (at.tile < 0) return;
+    const int q0 = at.q0, nq = at.nq, k0 = at.k0, nk = at.nk;
+    const int rows = nq * a.group, row0 = at.tile * BM;
     // rows beyond the last take part as copies of it
     auto limit_of = [&](int row) { // keys that a row sees
-        return a.causal ? min(max(min(row, rows - 1) / a.group + nk - nq + 1, 0), nk) : nk;
+        return a.causal ? min(max(token_of(a, min(row, rows - 1)) + nk - nq + 1, 0), nk) : nk;
     };
     const int wrow = row0 + wave * 32 * QB;
     const int wave_min = limit_of(wrow), wave_max = limit_of(wrow + 32 * QB - 1), most = limit_of(row0 + BM - 1);
-    int limit[QB];
-    int head[QB], token[QB]; // of a lane's rows, the token from the sequence's first
-    u32x4 q[QB][NC];
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        const int row = wrow + 32 * i + n, r = min(row, rows - 1);
-        limit[i] = limit_of(row);
-        token[i] = r / a.group;
-        head[i] = kvh * a.group + (r - token[i] * a.group);
-        const T *qp = (const T *)a.q + (int64_t)(q0 + token[i]) * a.q_stride + (int64_t)head[i] * a.dim;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int d0 = (2 * c + h) * E;
-            if constexpr (RUNS) q[i][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
-            else q[i][c] = load_edge<T>(qp + d0, a.dim - d0);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) q[i][c][w] ^= a.flip;
-        }
-    }
-
     const char *kb = (const char *)((const T *)a.k + (int64_t)k0 * a.k_stride + (int64_t)kvh * a.dim);
     const char *vb = (const char *)((const T *)a.v + (int64_t)k0 * a.v_stride + (int64_t)kvh * a.dim);
     const uint32_t k_bytes = (uint32_t)(a.k_stride * (int)sizeof(T)), v_bytes = (uint32_t)(a.v_stride * (int)sizeof(T));
+    uint32_t k_from[PI], v_from[PI]; // bytes from a whole tile's first row to a lane's runs
+#pragma unroll
+    for (int p = 0; p < PI; ++p) {
+        const int at = (wave * PI + p) * 1024 + lane * 16, row = at / kRow, run = at % kRow / 16;
+        k_from[p] = (uint32_t)row * k_bytes + (uint32_t)Lay::k_run(row, run) * 16u;
+        v_from[p] = (uint32_t)row * v_bytes + (uint32_t)Lay::v_run(row, run) * 16u;
+    }
     auto fetch = [&](int t, int buf) { // tile t; rows behind the last key are copies of it
         const int left = nk - t * KB - 1; // last row of the tile that there is
         const char *kt = kb + (int64_t)t * KB * k_bytes, *vt = vb + (int64_t)t * KB * v_bytes;
         char *to = lds + buf * 2 * kTile + wave * PI * 1024;
+        if (RUNS && left >= KB - 1 && a.dim == DP) {
+#pragma unroll
+            for (int p = 0; p < PI; ++p) {
+                async_run(kt, k_from[p], to + p * 1024);
+                async_run(vt, v_from[p], to + kTile + p * 1024);
+            }
+            return;
+        }
 #pragma unroll
         for (int p = 0; p < PI; ++p) {
             const int off = (wave * PI + p) * 1024 + lane * 16, row = off / kRow, run = off % kRow / 16;
-            const int from = min(row, left);
+            const int over = max(row - left, 0), from = row - over;
             const int kr = Lay::k_run(row, run), vr = Lay::v_run(row, run);
             if constexpr (RUNS) {
-                if (kr * E < a.dim) async_run(kt + ((uint32_t)from * k_bytes + (uint32_t)kr * 16u), to + p * 1024);
-                if (vr * E < a.dim) async_run(vt + ((uint32_t)from * v_bytes + (uint32_t)vr * 16u), to + kTile + p * 1024);
+                if (kr * E < a.dim) async_run(kt, k_from[p] - (uint32_t)over * k_bytes, to + p * 1024);
+                if (vr * E < a.dim) async_run(vt, v_from[p] - (uint32_t)over * v_bytes, to + kTile + p * 1024);
             } else {
                 const T *kp = (const T *)(kt + (int64_t)from * k_bytes), *vp = (const T *)(vt + (int64_t)from * v_bytes);
                 uint32_t kw[4], vw[4];
@@ -236,6 +240,46 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
     if (RUNS && a.dim < DP) { // runs behind dim are never fetched; K's count as zeros
         for (int i = threadIdx.x; i < 4 * kTile / 16; i += 256) reinterpret_cast<u32x4 *>(lds)[i] = (u32x4){0, 0, 0, 0};
         __syncthreads();
+    }
+
+    const int tiles = (most + KB - 1) / KB;
+    if (tiles > 0) fetch(0, 0);
+    // Q's rows come through the odd tiles' place where they fit, whole lines at a time, a wave's own ones (24 sequences of 500 rows,
+    // 32 heads of 128: 89.6 us, straight to registers 91.1; heads of 64 gain nothing, 155 and 151 at 1000 rows)
+    constexpr bool kStageQ = RUNS && DP > 64 && BM * kRow <= 2 * kTile;
+    if constexpr (kStageQ) {
+        constexpr int PQ = 32 * QB * kRow / 1024;
+        char *to = lds + 2 * kTile + wave * PQ * 1024;
+#pragma unroll
+        for (int p = 0; p < PQ; ++p) {
+            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = Lay::k_run(r, off % kRow / 16);
+            const int row = min(row0 + r, rows - 1), tok = token_of(a, row);
+            const T *from = (const T *)a.q + (int64_t)(q0 + tok) * a.q_stride + (int64_t)(kvh * a.group + row - tok * a.group) * a.dim + run * E;
+            if (run * E < a.dim) async_run((const char *)from, to + p * 1024);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+
+    int limit[QB];
+    int head[QB], token[QB]; // of a lane's rows, the token from the sequence's first
+    u32x4 q[QB][NC];
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        const int row = wrow + 32 * i + n, r = min(row, rows - 1);
+        limit[i] = limit_of(row);
+        token[i] = token_of(a, r);
+        head[i] = kvh * a.group + (r - token[i] * a.group);
+        const T *qp = (const T *)a.q + (int64_t)(q0 + token[i]) * a.q_stride + (int64_t)head[i] * a.dim;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d0 = (2 * c + h) * E;
+            if constexpr (kStageQ)
+                q[i][c] = *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, 2 * c + h) * 16);
+            else if constexpr (RUNS) q[i][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
+            else q[i][c] = load_edge<T>(qp + d0, a.dim - d0);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) q[i][c][w] ^= a.flip;
+        }
     }
 
     // where a lane reads: K's row n (+ 32 a block), piece c; V's rows 4h + (lane % 16) / 4 (+ 8, + 16 cc, + 32 b), columns of block db
@@ -262,8 +306,6 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         m[i] = -INFINITY;
         l[i] = 0.f;
     }
-    const int tiles = (most + KB - 1) / KB;
-    if (tiles > 0) fetch(0, 0);
     for (int t = 0; t < tiles; ++t) {
         all_ready(); // tile t is there, and every wave is done with tile t - 1
         if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
@@ -272,14 +314,23 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         const char *kt = lds + (t & 1) * 2 * kTile, *vt = kt + kTile;
 
         f32x16 s[QB][B] = {};
+        // pieces of K's rows are read kAhead products before they are needed
+        constexpr int kAhead = NC < 8 ? NC : 8;
+        auto read_k = [&](int j) { return *reinterpret_cast<const u32x4 *>(kt + k_off[j % NC % NK] + j % NC / NK * NK * 32 + j / NC * 32 * kRow); };
+        u32x4 kf[kAhead];
 #pragma unroll
-        for (int b = 0; b < B; ++b)
+        for (int j = 0; j < kAhead; ++j) kf[j] = read_k(j);
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const u32x4 kf = *reinterpret_cast<const u32x4 *>(kt + k_off[c % NK] + c / NK * NK * 32 + b * 32 * kRow);
+        for (int j = 0; j < B * NC; ++j) {
 #pragma unroll
-                for (int i = 0; i < QB; ++i) s[i][b] = mfma32(kf, q[i][c], s[i][b], T());
+            for (int i = 0; i < QB; ++i) s[i][j / NC] = mfma32(kf[j % kAhead], q[i][j % NC], s[i][j / NC], T());
+            __builtin_amdgcn_sched_group_barrier(0x8, QB * (sizeof(T) == 2 ? 1 : 4), 0);
+            if (j + kAhead < B * NC) {
+                kf[j % kAhead] = read_k(j + kAhead);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
+        }
         if (first + KB > wave_min) {
 #pragma unroll
             for (int i = 0; i < QB; ++i)
@@ -350,11 +401,11 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         }
     }
 
+    __syncthreads(); // the tiles' place takes o's
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
         const int row = wrow + 32 * i + n;
         const float sum = l[i] + other_half(l[i]);
-        if (row >= rows) continue;
         const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
         const int64_t grow = q0 + token[i];
         T *op = (T *)a.o + grow * a.o_stride + (int64_t)head[i] * a.dim;
@@ -367,15 +418,26 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
                 T4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = (T)(o[i][d][4 * r4 + e] * inv);
-                if (a.o_runs) {
-                    if (at4 < a.dim) *reinterpret_cast<T4 *>(op + at4) = v;
+                if (a.o_runs) { // rows of whole runs go through LDS, so that a store takes whole lines
+                    const int run = at4 / E;
+                    *reinterpret_cast<T4 *>(lds + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, run) * 16 + at4 % E * (int)sizeof(T)) = v;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (at4 + e < a.dim) op[at4 + e] = v[e];
+                        if (at4 + e < a.dim && row < rows) op[at4 + e] = v[e];
                 }
             }
-        if (a.lse && h == 0) a.lse[grow * a.heads + head[i]] = sum == 0.f ? -INFINITY : (m[i] - kUp + __log2f(sum)) * kLn2;
+        if (a.lse && h == 0 && row < rows) a.lse[grow * a.heads + head[i]] = sum == 0.f ? -INFINITY : (m[i] - kUp + __log2f(sum)) * kLn2;
+    }
+    if (a.o_runs) {
+        constexpr int PO = 32 * QB * kRow / 1024;
+#pragma unroll
+        for (int p = 0; p < PO; ++p) {
+            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = off % kRow / 16, row = row0 + r, tok = token_of(a, row);
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + r * kRow + Lay::k_run(r, run) * 16);
+            T *op = (T *)a.o + (int64_t)(q0 + tok) * a.o_stride + (int64_t)(kvh * a.group + row - tok * a.group) * a.dim + run * E;
+            if (row < rows && run * E < a.dim) *reinterpret_cast<u32x4 *>(op) = v;
+        }
     }
 }
 
@@ -419,11 +481,15 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.group = d->heads / d->kv_heads;
     a.dim = d->head_dim;
     a.causal = d->causal;
+    if (a.group > 1) { // exact for rows under 2^31
+        while ((2u << a.group_shift) < (uint32_t)a.group) ++a.group_shift;
+        a.group_mul = (uint32_t)(((1ull << (32 + a.group_shift)) + a.group - 1) / a.group);
+    }
     a.q_rows = d->q_rows;
     a.kv_rows = d->kv_rows;
     const int per = 16 / e;
     const bool runs = a.dim % per == 0 && (d->q_stride | d->k_stride | d->v_stride) % per == 0 && aligned16(q) && aligned16(k) && aligned16(v);
-    a.o_runs = a.dim % 4 == 0 && d->o_stride % 4 == 0 && multiple_of(o, 4 * e);
+    a.o_runs = a.dim % per == 0 && d->o_stride % per == 0 && aligned16(o);
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
         constexpr int K = sizeof(T) == 2 ? 64 : 32;
