@@ -4,7 +4,8 @@
 // needed; then the pages' numbers are copied between the stack of free ones and the rows of the table, and each token
 // finds its sequence by a search among the starts. Nothing here has work to speak of: dependent steps bound it. The
 // sums are one workgroup's, 1024 sequences at a time; few tokens are placed by it, too, in the same launch, many by a
-// second one, which needs all the starts.
+// second one, which needs all the starts. 64 sequences of one token: a launch (7.6 us a call); 500, of which 50 bring prompts of
+// up to 8000 tokens and 25 end: 22 us, 5 of them the second launch's.
 #include "decode.h"
 
 namespace spinn {
@@ -44,25 +45,68 @@ __device__ __forceinline__ uint32_t scan(uint32_t v, uint32_t *parts, uint32_t &
     return wave ? sum(before, __shfl(p, wave - 1)) : before;
 }
 
-// Largest i in [lo, hi) with v[i] <= t, v ascending, v[lo] <= t.
-__device__ __forceinline__ int last_upto(const int32_t *v, int lo, int hi, int t) {
+// Largest i in [lo, hi) with v(i) <= t, v ascending, v(lo) <= t.
+template <class V>
+__device__ __forceinline__ int last_upto(V v, int lo, int hi, int t) {
     while (hi - lo > 1) {
         const int mid = lo + (hi - lo) / 2;
-        if (v[mid] <= t) lo = mid;
+        if (v(mid) <= t) lo = mid;
         else hi = mid;
     }
     return lo;
 }
 // The same for a t that all lanes share: 64 places a step.
-__device__ __forceinline__ int wave_last_upto(const int32_t *v, int lo, int hi, int t) {
+template <class V>
+__device__ __forceinline__ int wave_last_upto(V v, int lo, int hi, int t) {
     const int lane = threadIdx.x & 63;
     while (hi - lo > 1) {
         const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-        const int n = __popcll(__ballot(at < hi && v[at] <= t));
+        const int n = __popcll(__ballot(at < hi && v(at) <= t));
         lo += (n - 1) * step;
         hi = min(hi, lo + step);
     }
     return lo;
+}
+// The same for t = first.. +63, one a lane, up to `last` (the lanes behind it get its place): one search where they all share a place,
+// as a long prompt's tokens do.
+template <class V>
+__device__ __forceinline__ int lanes_last_upto(V v, int hi, int first, int last) {
+    const int lo = wave_last_upto(v, 0, hi, first), end = min(first + 63, last);
+    if (lo + 1 >= hi || v(lo + 1) > end) return lo;
+    return last_upto(v, lo, wave_last_upto(v, lo, hi, end) + 1, min(first + (int)(threadIdx.x & 63), last));
+}
+
+// Page numbers 0 .. n - 1, each of the sequence (of 1024) that `offset` places it in, from one list to another. A wave has a stretch
+// of them and goes on from the sequence that it is in; those of four rounds are asked for before the first is written (12600 pages
+// there and back, one round after the other with a search each: 17 us, so 10).
+template <class V, class From, class To>
+__device__ __forceinline__ void move_pages(V offset, int n, From from, To to) {
+    constexpr int R = 4, kWaves = kThreads / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int each = ((n + kWaves - 1) / kWaves + 63) & ~63, end = min(n, (wave + 1) * each);
+    int first = wave * each;
+    if (first >= end) return;
+    int at = wave_last_upto(offset, 0, kThreads, first);
+    for (; first < end; first += 64 * R) {
+        int32_t page[R];
+        int owner[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = first + 64 * r, last = min(i + 63, end - 1);
+            owner[r] = at;
+            if (i < end && at + 1 < kThreads && __builtin_amdgcn_readfirstlane(offset(at + 1)) <= last) {
+                const int to_at = wave_last_upto(offset, at, kThreads, last);
+                owner[r] = last_upto(offset, at, to_at + 1, min(i + lane, last));
+                at = to_at;
+            }
+            page[r] = from(min(i + lane, n - 1), owner[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = first + 64 * r + lane;
+            if (i < end) to(i, owner[r], page[r]);
+        }
+    }
 }
 
 // Tokens first.. +63, one a lane: all lanes of a wave together.
@@ -70,10 +114,8 @@ __device__ __forceinline__ void place_tokens(const AssignArgs &a, int first, int
     const int t = first + (int)(threadIdx.x & 63);
     int seq = -1, slot = -1, position = 0;
     if (first < total) {
-        const int s0 = wave_last_upto(a.starts, 0, a.seqs, first);
-        const int s1 = a.starts[s0 + 1] > min(first + 63, total - 1) ? s0 : wave_last_upto(a.starts, s0, a.seqs, min(first + 63, total - 1));
+        const int s = lanes_last_upto([&](int i) { return a.starts[i]; }, a.seqs, first, total - 1);
         if (t < total) {
-            const int s = last_upto(a.starts, s0, s1 + 1, t);
             if (a.served[s]) {
                 const int left = a.starts[s + 1] - t; // tokens to its end
                 seq = s;
@@ -93,6 +135,7 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(AssignArgs a, int p
     __shared__ uint32_t before[kThreads + 1], parts[2][kThreads / 64], s_taken;
     __shared__ int32_t s_held[kThreads];
     const int tid = threadIdx.x;
+    auto offset = [&](int i) { return (int)before[i]; };
     uint32_t count = (uint32_t)min(max(*a.free_count, 0), a.n_pages);
     if (tid == 0) s_taken = 0;
 
@@ -107,10 +150,8 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(AssignArgs a, int p
             if (tid == 0) before[kThreads] = total;
             __syncthreads();
             total = min(total, (uint32_t)a.n_pages - count);
-            for (uint32_t i = tid; i < total; i += kThreads) {
-                const int j = last_upto(reinterpret_cast<const int32_t *>(before), 0, kThreads, (int)i);
-                a.free_pages[count + i] = a.table[(int64_t)(base + j) * a.max_pages + (i - before[j])];
-            }
+            move_pages(offset, (int)total, [&](int i, int j) { return a.table[(int64_t)(base + j) * a.max_pages + (i - before[j])]; },
+                       [&](int i, int, int32_t page) { a.free_pages[count + i] = page; });
             count += total;
             __syncthreads();
         }
@@ -147,11 +188,11 @@ __global__ __launch_bounds__(kThreads) void kv_assign_kernel(AssignArgs a, int p
             a.held_out[s] = ended ? 0 : (int32_t)((uint32_t)held + got);
         }
         __syncthreads();
-        for (uint32_t i = tid; i < total_need && needed + i < count; i += kThreads) {
-            const int j = last_upto(reinterpret_cast<const int32_t *>(before), 0, kThreads, (int)i);
-            if (sum(needed, before[j + 1]) <= count)
-                a.table[(int64_t)(base + j) * a.max_pages + s_held[j] + (i - before[j])] = a.free_pages[count - 1 - (needed + i)];
-        }
+        const uint32_t most = needed < count ? min(total_need, count - needed) : 0u;
+        move_pages(offset, (int)most, [&](int i, int) { return a.free_pages[count - 1 - (needed + i)]; },
+                   [&](int i, int j, int32_t page) {
+                       if (sum(needed, before[j + 1]) <= count) a.table[(int64_t)(base + j) * a.max_pages + s_held[j] + (i - before[j])] = page;
+                   });
         tokens = sum(tokens, total);
         needed = sum(needed, total_need);
         __syncthreads();
