@@ -131,6 +131,56 @@ __device__ __forceinline__ int granule_at(int lane, int half) {
     return r * 128 + ((c ^ (r >> 1)) << 4);
 }
 
+// The waves' sums of a workgroup's MT x NT blocks (from block row m0 and tile t0 on), added in wave order, to y.
+template <class T, class O, int MT, int NT, int NW>
+__device__ __forceinline__ void join_waves(const LinearArgs &a, int m0, int t0, int wave, int lane, const Sums<T> (&acc)[MT][NT]) {
+    __shared__ Sums<T> part[NW][MT * NT][64];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+    // a wave finishes every NW-th block; what it adds is on its way while the others' sums come together
+    constexpr int B = (MT * NT + NW - 1) / NW;
+    typedef Columns<O, 4> Col;
+    typename Col::Run bias[B], res[B];
+    int rows[B], cols[B], left[B];
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+        const int b = wave + k * NW, tile = t0 + b % NT;
+        rows[k] = (m0 + b / NT) * 16 + (lane & 15);
+        cols[k] = first_col<T>(tile, lane >> 4);
+        left[k] = b < MT * NT && tile < a.ntiles && rows[k] < a.m ? a.n - cols[k] : 0;
+        if (left[k] > 0) {
+            if (a.bias) bias[k] = Col::load((const O *)a.bias + cols[k], left[k], false);
+            if (a.res) res[k] = Col::load((const O *)a.res + (int64_t)rows[k] * a.ldres + cols[k], left[k], a.vec);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < B; ++k)
+        if (left[k] > 0) {
+            const int b = wave + k * NW;
+            Sums<T> s = part[0][b][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) s += part[w][b][lane];
+            f32x4 v;
+            if constexpr (sizeof(T) == 1) {
+                const float sx = a.sx[rows[k]];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (float)s[i] * (i < left[k] ? a.sw[cols[k] + i] : 0.f) * sx;
+            } else {
+                v = s;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (a.bias) v[i] += (float)bias[k][i];
+                if (a.res) v[i] += (float)res[k][i];
+            }
+            O *y = (O *)a.y + (int64_t)rows[k] * a.ldy + cols[k];
+            with_act(a.act, [&](auto act) { Col::template store<decltype(act)::value>(y, left[k], a.vec, v); });
+        }
+}
+
 template <class T, class O, int MT, int NT, int NW, Rows ROWS>
 __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
     constexpr int E = 16 / (int)sizeof(T);
@@ -178,51 +228,7 @@ __global__ __launch_bounds__(64 * NW) void linear_stream_kernel(LinearArgs a) {
                     for (int j = 0; j < NT; ++j) mfma_frag(acc[i][j], w[u][j], x[u][i], T());
             }
     }
-    __shared__ Sums<T> part[NW][MT * NT][64];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
-    // a wave finishes every NW-th block; what it adds is on its way while the others' sums come together
-    constexpr int B = (MT * NT + NW - 1) / NW;
-    typedef Columns<O, 4> Col;
-    typename Col::Run bias[B], res[B];
-    int rows[B], cols[B], left[B];
-#pragma unroll
-    for (int k = 0; k < B; ++k) {
-        const int b = wave + k * NW, tile = t0 + b % NT;
-        rows[k] = (m0 + b / NT) * 16 + (lane & 15);
-        cols[k] = first_col<T>(tile, lane >> 4);
-        left[k] = b < MT * NT && tile < a.ntiles && rows[k] < a.m ? a.n - cols[k] : 0;
-        if (left[k] > 0) {
-            if (a.bias) bias[k] = Col::load((const O *)a.bias + cols[k], left[k], false);
-            if (a.res) res[k] = Col::load((const O *)a.res + (int64_t)rows[k] * a.ldres + cols[k], left[k], a.vec);
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < B; ++k)
-        if (left[k] > 0) {
-            const int b = wave + k * NW;
-            Sums<T> s = part[0][b][lane];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) s += part[w][b][lane];
-            f32x4 v;
-            if constexpr (sizeof(T) == 1) {
-                const float sx = a.sx[rows[k]];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = (float)s[i] * (i < left[k] ? a.sw[cols[k] + i] : 0.f) * sx;
-            } else {
-                v = s;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (a.bias) v[i] += (float)bias[k][i];
-                if (a.res) v[i] += (float)res[k][i];
-            }
-            O *y = (O *)a.y + (int64_t)rows[k] * a.ldy + cols[k];
-            with_act(a.act, [&](auto act) { Col::template store<decltype(act)::value>(y, left[k], a.vec, v); });
-        }
+    join_waves<T, O, MT, NT, NW>(a, m0, t0, wave, lane, acc);
 }
 
 __device__ __forceinline__ void copy_to_lds(const char *src, char *lds) {
@@ -512,8 +518,7 @@ template <class T, class O, int MT, int NT, int NW>
 int launch_stream(const LinearArgs &a, Rows rows, hipStream_t st) {
     const dim3 grid((a.ntiles + NT - 1) / NT, (a.m + 16 * MT - 1) / (16 * MT));
     if (!launch_fits(grid.x, 64 * NW) || grid.y > 65535) return SPINN_HIP_EUNSUPPORTED;
-    if constexpr (sizeof(T) == 1) linear_stream_kernel<T, O, MT, NT, NW, kRuns><<<grid, 64 * NW, 0, st>>>(a);
-    else if (rows == kRuns) linear_stream_kernel<T, O, MT, NT, NW, kRuns><<<grid, 64 * NW, 0, st>>>(a);
+    if (rows == kRuns) linear_stream_kernel<T, O, MT, NT, NW, kRuns><<<grid, 64 * NW, 0, st>>>(a);
     else if (rows == kLaidOut) linear_stream_kernel<T, O, MT, NT, NW, kLaidOut><<<grid, 64 * NW, 0, st>>>(a);
     else if (rows == kLoose) linear_stream_kernel<T, O, MT, NT, NW, kLoose><<<grid, 64 * NW, 0, st>>>(a);
     else linear_stream_kernel<T, O, MT, NT, NW, kShort><<<grid, 64 * NW, 0, st>>>(a);
@@ -577,20 +582,22 @@ inline Choice choose(int64_t mt, int64_t nt, int64_t kf) { // tiles of 16 rows a
     return c;
 }
 
-// The kernel of `c` for a layer. part: the splits' sums.
+// A layer on tiles. part: the splits' sums.
 template <class T, class O>
-int launch_linear(const LinearArgs &a, const Choice &c, Rows rows, void *part, hipStream_t st) {
-    const bool xp = rows == kLaidOut;
+int launch_tiles(const LinearArgs &a, const Choice &c, bool xp, void *part, hipStream_t st) {
     const int64_t tiles = (((int64_t)(a.m + 15) / 16 + 3) / 4) * ((a.ntiles + 7) / 8);
     const bool deep = tiles * c.splits <= device_cu_count();
-    switch (c.kind) {
-    case Choice::kTile256: return launch_tile<T, O, 256, 256, 2, 4, 4>(a, xp, 1, nullptr, st);
-    case Choice::kTile128: return launch_tile<T, O, 128, 128, 2, 2, 4>(a, xp, 1, nullptr, st);
-    case Choice::kTile64: // one workgroup per CU can have all of its LDS
-        if (deep) return launch_tile<T, O, 64, 128, 2, 2, 8>(a, xp, c.splits, part, st);
-        return launch_tile<T, O, 64, 128, 2, 2, 4>(a, xp, c.splits, part, st);
-    default: break;
-    }
+    if (c.kind == Choice::kTile256) return launch_tile<T, O, 256, 256, 2, 4, 4>(a, xp, 1, nullptr, st);
+    if (c.kind == Choice::kTile128) return launch_tile<T, O, 128, 128, 2, 2, 4>(a, xp, 1, nullptr, st);
+    // one workgroup per CU can have all of its LDS
+    if (deep) return launch_tile<T, O, 64, 128, 2, 2, 8>(a, xp, c.splits, part, st);
+    return launch_tile<T, O, 64, 128, 2, 2, 4>(a, xp, c.splits, part, st);
+}
+
+// The kernel of `c` for a layer.
+template <class T, class O>
+int launch_linear(const LinearArgs &a, const Choice &c, Rows rows, void *part, hipStream_t st) {
+    if (c.kind != Choice::kStream) return launch_tiles<T, O>(a, c, rows == kLaidOut, part, st);
     if (c.mt == 4 && c.nt == 4) return launch_stream<T, O, 4, 4, 4>(a, rows, st);
     if (c.mt == 4) return launch_stream<T, O, 4, 2, 8>(a, rows, st);
     if (c.mt == 2 && c.nt == 4) return launch_stream<T, O, 2, 4, 4>(a, rows, st);

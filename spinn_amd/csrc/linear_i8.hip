@@ -117,10 +117,103 @@ int launch_quantize(int64_t rows, int k, const void *x, int64_t ldx, int8_t *xq,
     return check_launch();
 }
 
+// Few rows: as linear_stream_kernel, with the next U fragments of a wave on their way while U are multiplied. What bounds it is what a CU takes in,
+// some 50 GB/s of weights and of rows (12.8 TB/s over all), whichever level of memory they come from: see choose().
+template <class O, int MT, int NT, int NW, int U>
+__global__ __launch_bounds__(64 * NW) void linear_i8_stream_kernel(LinearArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t0 = blockIdx.x * NT, m0 = blockIdx.y * MT;
+    const char *wp[NT], *xp[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) wp[j] = a.w + (int64_t)min(t0 + j, a.ntiles - 1) * a.kf * kFragBytes + lane * 16;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xp[i] = (const char *)a.x + (int64_t)min((m0 + i) * 16 + (lane & 15), a.m - 1) * a.ldx;
+    const int last = ((a.k + 15) & ~15) - 16; // what is behind a row meets zeros of w: any 16 bytes of it do
+    Sums<int8_t> acc[MT][NT] = {};
+    u32x4 w[2][U][NT], x[2][U][MT];
+    // a wave takes fragments in pairs: 128 bytes, a cache line, of every row of x
+    auto fragment = [](int u) { return u / 2 * 2 * NW + u % 2; };
+    auto fetch = [&](int f0, u32x4 (&wb)[U][NT], u32x4 (&xb)[U][MT]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int f = f0 + fragment(u);
+            if (f >= a.kf) break;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) wb[u][j] = *reinterpret_cast<const u32x4 *>(wp[j] + (int64_t)f * kFragBytes);
+            const int k0 = min(f * kFrag<int8_t> + (lane >> 4) * 16, last);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xb[u][i] = *reinterpret_cast<const u32x4 *>(xp[i] + k0);
+        }
+    };
+    auto multiply = [&](int f0, const u32x4 (&wb)[U][NT], const u32x4 (&xb)[U][MT]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (f0 + fragment(u) >= a.kf) break;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mfma_frag(acc[i][j], wb[u][j], xb[u][i], int8_t());
+        }
+    };
+    constexpr int S = NW * U;
+    fetch(2 * wave, w[0], x[0]);
+    for (int f = 2 * wave; f < a.kf; f += 2 * S) {
+        fetch(f + S, w[1], x[1]);
+        multiply(f, w[0], x[0]);
+        fetch(f + 2 * S, w[0], x[0]);
+        multiply(f + S, w[1], x[1]);
+    }
+    join_waves<int8_t, O, MT, NT, NW>(a, m0, t0, wave, lane, acc);
+}
+
+template <class O, int MT, int NT, int NW, int U>
+int launch_stream_i8(const LinearArgs &a, hipStream_t st) {
+    const dim3 grid((a.ntiles + NT - 1) / NT, (a.m + 16 * MT - 1) / (16 * MT));
+    if (!launch_fits(grid.x, 64 * NW) || grid.y > 65535) return SPINN_HIP_EUNSUPPORTED;
+    linear_i8_stream_kernel<O, MT, NT, NW, U><<<grid, 64 * NW, 0, st>>>(a);
+    return check_launch();
+}
+
 inline int64_t frags(const SpinnHipLinearI8Desc *d) { return ((int64_t)d->k + 127) / 128 * 2; }
 inline int64_t n_tiles(const SpinnHipLinearI8Desc *d) { return ((int64_t)d->n + 63) / 64 * 4; }
 inline int64_t m_tiles(const SpinnHipLinearI8Desc *d) { return ((int64_t)d->m + 15) / 16; }
-Choice choose(const SpinnHipLinearI8Desc *d) { return choose(m_tiles(d), n_tiles(d), frags(d)); }
+
+// Which kernel a layer runs on, by its time as measured over m = 1..2000, n = 1024..14336, k = 1024..16384 (us; f fragments of 64 along K,
+// 256 CUs, one workgroup of the stream kernel at a time on each):
+//  * stream kernel on MT x NT blocks: 2 + 0.02 f (MT + NT) a round of its grid (45 x 5120 x 8192: 1 x 4 blocks 16.2, 2 x 2
+//    18.4, 2 x 4 17.5, 4 x 4 25.0; 64 x 14336 x 4096: 18.8 on 4 x 4, 23.0 on 2 x 4, 36.6 on 1 x 4; 100 x 4096 x 4096: 8.7 on 2 x 4, 11.4 on
+//    1 x 4, 12.9 on 4 x 4; 8 x 14336 x 4096: 12.5 on 1 x 2, 14.9 on 1 x 1);
+//  * 64 x 128 tiles: 5.5 + 0.2 f / splits, 5 more where K is split, 5.5 + 0.18 f a round from more than one per CU (200 x 1024 x 16384:
+//    54.6 whole, 34.1 in two, 22.6 in four, the stream kernel 24.8; 500 x 1024 x 1024: 8.2, stream 5.0);
+//  * 128 x 128 tiles: 5.5 + 0.23 f up to one per CU (150 x 14336 x 4096: 24.0, 64 x 128 27.5, stream 38.1); beyond, and for
+//    256 x 256 from one per CU, as the other types.
+Choice choose(const SpinnHipLinearI8Desc *d) {
+    const int64_t cus = device_cu_count(), mt = m_tiles(d), nt = n_tiles(d), f = frags(d);
+    auto grid = [&](int64_t rows, int64_t cols) { return ((mt + rows - 1) / rows) * ((nt + cols - 1) / cols); };
+    auto rounds = [&](int64_t blocks) { return (blocks + cus - 1) / cus; };
+    if (grid(8, 8) > cus) return choose(mt, nt, f);
+    Choice c{Choice::kStream, 1, 1, 1};
+    double least = 1e30;
+    static const int blocks[][2] = {{1, 1}, {1, 2}, {1, 4}, {2, 2}, {2, 4}, {3, 2}, {3, 4}, {4, 2}, {4, 4}};
+    for (auto &b : blocks) {
+        const double t = (2 + 0.02 * f * (b[0] + b[1])) * rounds(grid(b[0], b[1]));
+        if (b[0] <= mt && t < least) {
+            least = t;
+            c.mt = b[0];
+            c.nt = b[1];
+        }
+    }
+    const int64_t tiles = grid(4, 8);
+    const int64_t splits = std::max<int64_t>(1, std::min(cus / tiles, f / 16));
+    const double whole = tiles <= cus ? 5.5 + 0.2 * f : 5.5 + 0.18 * f * rounds(tiles), parts = 10.5 + 0.2 * f / splits;
+    if (std::min(whole, parts) < least) {
+        least = std::min(whole, parts);
+        c.kind = Choice::kTile64;
+        c.splits = splits > 1 && parts < whole ? (int)splits : 1;
+    }
+    if (5.5 + 0.23 * f < least) c.kind = Choice::kTile128;
+    return c;
+}
 
 } // namespace
 
@@ -170,7 +263,21 @@ int linear_i8_run(const SpinnHipLinearI8Desc *d, const int8_t *x, const float *x
     const int per = 16 / dtype_bytes(d->dtype);
     a.vec = aligned16(y) && d->ldy % per == 0 && (!res || (aligned16(res) && d->ldres % per == 0));
     const Choice c = choose(d);
-    return with_dtype(d->dtype, [&](auto o) { return launch_linear<int8_t, decltype(o)>(a, c, kRuns, ws, st); });
+    return with_dtype(d->dtype, [&](auto o) {
+        typedef decltype(o) O;
+        if (c.kind != Choice::kStream) return launch_tiles<int8_t, O>(a, c, false, ws, st);
+        switch (c.mt * 10 + c.nt) {
+        case 44: return launch_stream_i8<O, 4, 4, 8, 2>(a, st);
+        case 34: return launch_stream_i8<O, 3, 4, 8, 2>(a, st);
+        case 24: return launch_stream_i8<O, 2, 4, 8, 2>(a, st);
+        case 42: return launch_stream_i8<O, 4, 2, 8, 2>(a, st);
+        case 32: return launch_stream_i8<O, 3, 2, 8, 4>(a, st);
+        case 22: return launch_stream_i8<O, 2, 2, 8, 4>(a, st);
+        case 14: return launch_stream_i8<O, 1, 4, 8, 4>(a, st);
+        case 12: return launch_stream_i8<O, 1, 2, 8, 4>(a, st);
+        default: return launch_stream_i8<O, 1, 1, 16, 4>(a, st);
+        }
+    });
 }
 
 } // namespace spinn
