@@ -57,14 +57,14 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
         const int q0 = clamped(a.starts, s, a.q_rows), q1 = clamped(a.starts, s + 1, a.q_rows);
         const int k0 = clamped(ks, s, a.kv_rows), k1 = clamped(ks, s + 1, a.kv_rows);
         const int n = lane < a.seqs ? (max(q1 - q0, 0) * a.group + rows - 1) / rows : 0;
-        // tiles of the sequences that come first: more tiles, or as many and an earlier lane
-        const uint64_t key = (uint64_t)n << 32 | (uint32_t)(64 - lane);
+        // tiles of the sequences that come first: those of more tiles (under 2^24), or as many and an earlier lane
+        const uint32_t key = (uint32_t)n << 6 | (uint32_t)(63 - lane);
         int before = 0;
         if (a.seqs > 1) {
 #pragma unroll 8
             for (int i = 0; i < ((a.seqs + 7) & ~7); ++i) { // lanes behind the last sequence have no tiles
-                const int o = __builtin_amdgcn_readlane(n, i);
-                before += ((uint64_t)(uint32_t)o << 32 | (uint32_t)(64 - i)) > key ? o : 0;
+                const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+                before += o > key ? (int)(o >> 6) : 0;
             }
         }
         const unsigned long long mine = __ballot(item >= before && item - before < n);
@@ -147,15 +147,15 @@ __device__ __forceinline__ float other_half(float v) { // lane ^ 32's
     return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & 32) ? r[0] : r[1]));
 }
 
-// 16 bytes a lane from base + off to lds + 16 lane; all_ready() waits for it. In assembly, since the compiler would wait for all
+// 16 bytes a lane from base + off to byte `to` + 16 lane of LDS; all_ready() waits for it. In assembly, since the compiler would wait for all
 // of these before every transposing read of LDS that follows, whatever it reads (16000 rows: 2020 -> 1916 us).
-__device__ __forceinline__ void async_run(const char *base, uint32_t off, const char *lds) {
-    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base) : "memory", "m0");
-}
-__device__ __forceinline__ void async_run(const char *from, const char *lds) { // from an address of its own each
-    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory", "m0");
+// lanes: all (~0) or none (0), without a branch.
+__device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32_t to, uint64_t lanes = ~0ull) {
+    uint64_t all;
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, exec\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
+                 : "=&s"(all)
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "s"(lanes)
+                 : "memory", "m0");
 }
 
 // This wave's copies have landed and its LDS reads are done, and so are every other wave's.
@@ -164,7 +164,7 @@ __device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) l
 // T: element; DP: head_dim padded to a multiple of 32; KB: keys of a tile; QB: blocks of 32 rows per wave;
 // RUNS: rows of q, k and v are whole, aligned 16-byte runs.
 template <class T, int DP, int KB, int QB, bool RUNS>
-__global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUNS ? 3 : 2) : 1) void prompt_kernel(PromptArgs a) {
     typedef Tile<T, DP> Lay;
     constexpr int E = Lay::E, kRow = Lay::kRow, NC = kRow / 32; // NC: operand pieces of a row
     constexpr int B = KB / 32, DB = DP / 32;
@@ -191,75 +191,84 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
     const char *kb = (const char *)((const T *)a.k + (int64_t)k0 * a.k_stride + (int64_t)kvh * a.dim);
     const char *vb = (const char *)((const T *)a.v + (int64_t)k0 * a.v_stride + (int64_t)kvh * a.dim);
     const uint32_t k_bytes = (uint32_t)(a.k_stride * (int)sizeof(T)), v_bytes = (uint32_t)(a.v_stride * (int)sizeof(T));
-    uint32_t k_from[PI], v_from[PI]; // bytes from a whole tile's first row to a lane's runs
-#pragma unroll
-    for (int p = 0; p < PI; ++p) {
-        const int at = (wave * PI + p) * 1024 + lane * 16, row = at / kRow, run = at % kRow / 16;
-        k_from[p] = (uint32_t)row * k_bytes + (uint32_t)Lay::k_run(row, run) * 16u;
-        v_from[p] = (uint32_t)row * v_bytes + (uint32_t)Lay::v_run(row, run) * 16u;
-    }
-    auto fetch = [&](int t, int buf) { // tile t; rows behind the last key are copies of it
-        const int left = nk - t * KB - 1; // last row of the tile that there is
-        const char *kt = kb + (int64_t)t * KB * k_bytes, *vt = vb + (int64_t)t * KB * v_bytes;
-        char *to = lds + buf * 2 * kTile + wave * PI * 1024;
-        if (RUNS && left >= KB - 1 && a.dim == DP) {
-#pragma unroll
-            for (int p = 0; p < PI; ++p) {
-                async_run(kt, k_from[p], to + p * 1024);
-                async_run(vt, v_from[p], to + kTile + p * 1024);
-            }
-            return;
-        }
+    // Bytes from a tile's first row to a lane's runs. Runs behind dim are copies of the last one: Q's are zeros there.
+    uint32_t k_from[PI], v_from[PI];
+    auto from_rows = [&](int left) { // of a tile whose row `left` is the last that there is: rows behind it are copies of it
 #pragma unroll
         for (int p = 0; p < PI; ++p) {
-            const int off = (wave * PI + p) * 1024 + lane * 16, row = off / kRow, run = off % kRow / 16;
-            const int over = max(row - left, 0), from = row - over;
-            const int kr = Lay::k_run(row, run), vr = Lay::v_run(row, run);
-            if constexpr (RUNS) {
-                if (kr * E < a.dim) async_run(kt, k_from[p] - (uint32_t)over * k_bytes, to + p * 1024);
-                if (vr * E < a.dim) async_run(vt, v_from[p] - (uint32_t)over * v_bytes, to + kTile + p * 1024);
-            } else {
-                const T *kp = (const T *)(kt + (int64_t)from * k_bytes), *vp = (const T *)(vt + (int64_t)from * v_bytes);
-                uint32_t kw[4], vw[4];
-                if (a.dim >= E) {
-                    load_loose<T, E>(kp, kr * E, a.dim, kw);
-                    load_loose<T, E>(vp, vr * E, a.dim, vw);
-                } else {
-                    const u32x4 x = load_edge<T>(kp + kr * E, a.dim - kr * E), y = load_edge<T>(vp + vr * E, a.dim - vr * E);
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        kw[w] = x[w];
-                        vw[w] = y[w];
-                    }
-                }
-                *reinterpret_cast<u32x4 *>(to + p * 1024 + lane * 16) = (u32x4){kw[0], kw[1], kw[2], kw[3]};
-                *reinterpret_cast<u32x4 *>(to + kTile + p * 1024 + lane * 16) = (u32x4){vw[0], vw[1], vw[2], vw[3]};
-            }
+            const int at = (wave * PI + p) * 1024 + lane * 16, row = min(at / kRow, left), place = at % kRow / 16;
+            const int last = a.dim / E - 1, kr = min(Lay::k_run(at / kRow, place), last), vr = min(Lay::v_run(at / kRow, place), last);
+            k_from[p] = (uint32_t)row * k_bytes + (uint32_t)kr * 16u;
+            v_from[p] = (uint32_t)row * v_bytes + (uint32_t)vr * 16u;
         }
     };
-    if (RUNS && a.dim < DP) { // runs behind dim are never fetched; K's count as zeros
-        for (int i = threadIdx.x; i < 4 * kTile / 16; i += 256) reinterpret_cast<u32x4 *>(lds)[i] = (u32x4){0, 0, 0, 0};
-        __syncthreads();
-    }
-
+    if constexpr (RUNS) from_rows(min(nk, KB) - 1);
+    const char *k_at = kb, *v_at = vb; // the tile to fetch next
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
+    uint32_t fetch_to = wave * PI * 1024; // its bytes of LDS, from lds on
+    uint64_t lanes = ~0ull;
+    auto fetch_piece = [&](int p) { // of 2 PI
+        if (p < PI) async_run(k_at, k_from[p], lds_at + fetch_to + p * 1024, lanes);
+        else async_run(v_at, v_from[p - PI], lds_at + fetch_to + kTile + (p - PI) * 1024, lanes);
+    };
+    auto next_fetch = [&](int t) { // what is fetched next is tile t
+        k_at = kb + (int64_t)t * KB * k_bytes;
+        v_at = vb + (int64_t)t * KB * v_bytes;
+        fetch_to = (t & 1) * 2 * kTile + wave * PI * 1024;
+        if (RUNS && nk - t * KB < KB) from_rows(nk - t * KB - 1); // the last one
+    };
+    auto fetch_loose = [&](int t) { // all of it through registers
+        const int left = nk - t * KB - 1;
+#pragma unroll
+        for (int p = 0; p < PI; ++p) {
+            const int off = (wave * PI + p) * 1024 + lane * 16, row = min(off / kRow, left), place = off % kRow / 16;
+            const int kr = Lay::k_run(off / kRow, place), vr = Lay::v_run(off / kRow, place);
+            const T *kp = (const T *)(k_at + (int64_t)row * k_bytes), *vp = (const T *)(v_at + (int64_t)row * v_bytes);
+            uint32_t kw[4], vw[4];
+            if (a.dim >= E) {
+                load_loose<T, E>(kp, kr * E, a.dim, kw);
+                load_loose<T, E>(vp, vr * E, a.dim, vw);
+            } else {
+                const u32x4 x = load_edge<T>(kp + kr * E, a.dim - kr * E), y = load_edge<T>(vp + vr * E, a.dim - vr * E);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    kw[w] = x[w];
+                    vw[w] = y[w];
+                }
+            }
+            *reinterpret_cast<u32x4 *>(lds + fetch_to + p * 1024 + lane * 16) = (u32x4){kw[0], kw[1], kw[2], kw[3]};
+            *reinterpret_cast<u32x4 *>(lds + fetch_to + kTile + p * 1024 + lane * 16) = (u32x4){vw[0], vw[1], vw[2], vw[3]};
+        }
+    };
     const int tiles = (most + KB - 1) / KB;
-    if (tiles > 0) fetch(0, 0);
+    if (tiles > 0) {
+        if constexpr (RUNS) {
+#pragma unroll
+            for (int p = 0; p < 2 * PI; ++p) fetch_piece(p);
+        } else {
+            fetch_loose(0);
+        }
+    }
+    // where a row of the tile lies in q and o, in elements from the first one's token and the kv head's first query head
+    const int tok0 = token_of(a, row0);
+    auto row_at = [&](int row, int64_t stride) {
+        const int tok = token_of(a, row);
+        return (uint32_t)(tok - tok0) * (uint32_t)stride + (uint32_t)((row - tok * a.group) * a.dim);
+    };
+    const T *const q_first = (const T *)a.q + (int64_t)(q0 + tok0) * a.q_stride + (int64_t)kvh * a.group * a.dim;
     // Q's rows come through the odd tiles' place where they fit, whole lines at a time, a wave's own ones (24 sequences of 500 rows,
     // 32 heads of 128: 89.6 us, straight to registers 91.1; heads of 64 gain nothing, 155 and 151 at 1000 rows)
     constexpr bool kStageQ = RUNS && DP > 64 && BM * kRow <= 2 * kTile;
     if constexpr (kStageQ) {
         constexpr int PQ = 32 * QB * kRow / 1024;
-        char *to = lds + 2 * kTile + wave * PQ * 1024;
+        const uint32_t to = lds_at + 2 * kTile + wave * PQ * 1024;
 #pragma unroll
         for (int p = 0; p < PQ; ++p) {
-            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = Lay::k_run(r, off % kRow / 16);
-            const int row = min(row0 + r, rows - 1), tok = token_of(a, row);
-            const T *from = (const T *)a.q + (int64_t)(q0 + tok) * a.q_stride + (int64_t)(kvh * a.group + row - tok * a.group) * a.dim + run * E;
-            if (run * E < a.dim) async_run((const char *)from, to + p * 1024);
+            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = min(Lay::k_run(r, off % kRow / 16), a.dim / E - 1);
+            async_run((const char *)q_first, row_at(min(row0 + r, rows - 1), a.q_stride) * (uint32_t)sizeof(T) + (uint32_t)run * 16u, to + p * 1024);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-
     int limit[QB];
     int head[QB], token[QB]; // of a lane's rows, the token from the sequence's first
     u32x4 q[QB][NC];
@@ -269,12 +278,12 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         limit[i] = limit_of(row);
         token[i] = token_of(a, r);
         head[i] = kvh * a.group + (r - token[i] * a.group);
-        const T *qp = (const T *)a.q + (int64_t)(q0 + token[i]) * a.q_stride + (int64_t)head[i] * a.dim;
+        const T *qp = q_first + row_at(r, a.q_stride);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d0 = (2 * c + h) * E;
             if constexpr (kStageQ)
-                q[i][c] = *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, 2 * c + h) * 16);
+                q[i][c] = d0 >= a.dim ? (u32x4){0, 0, 0, 0} : *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, 2 * c + h) * 16);
             else if constexpr (RUNS) q[i][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
             else q[i][c] = load_edge<T>(qp + d0, a.dim - d0);
 #pragma unroll
@@ -308,15 +317,30 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
     }
     for (int t = 0; t < tiles; ++t) {
         all_ready(); // tile t is there, and every wave is done with tile t - 1
-        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+        if (t + 1 < tiles) {
+            next_fetch(t + 1);
+            if constexpr (!RUNS) fetch_loose(t + 1);
+        } else {
+            lanes = 0;
+        }
         const int first = t * KB;
-        if (first >= wave_max) continue;
+        if (first >= wave_max) {
+            if constexpr (RUNS) {
+#pragma unroll
+                for (int p = 0; p < 2 * PI; ++p) fetch_piece(p);
+            }
+            continue;
+        }
         const char *kt = lds + (t & 1) * 2 * kTile, *vt = kt + kTile;
 
         f32x16 s[QB][B] = {};
         // pieces of K's rows are read kAhead products before they are needed
         constexpr int kAhead = NC < 8 ? NC : 8;
         auto read_k = [&](int j) { return *reinterpret_cast<const u32x4 *>(kt + k_off[j % NC % NK] + j % NC / NK * NK * 32 + j / NC * 32 * kRow); };
+        // The next tile's copies go out one by one between the products: a copy waits at its issue for those of the other waves to
+        // pass (64 bytes a cycle for all of the CU), 600 cycles for the eight of a wave in a row.
+        constexpr int kEvery = B * NC / (2 * PI); // products a copy
+        static_assert(B * NC % (2 * PI) == 0, "");
         u32x4 kf[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) kf[j] = read_k(j);
@@ -325,6 +349,7 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         for (int j = 0; j < B * NC; ++j) {
 #pragma unroll
             for (int i = 0; i < QB; ++i) s[i][j / NC] = mfma32(kf[j % kAhead], q[i][j % NC], s[i][j / NC], T());
+            if (RUNS && j % kEvery == kEvery - 1) fetch_piece(j / kEvery);
             __builtin_amdgcn_sched_group_barrier(0x8, QB * (sizeof(T) == 2 ? 1 : 4), 0);
             if (j + kAhead < B * NC) {
                 kf[j % kAhead] = read_k(j + kAhead);
@@ -342,11 +367,14 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         }
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
-            float top = s[i][0][0];
+            float tops[4]; // shorter chains
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tops[r] = s[i][0][r];
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][b][r]);
+                for (int r = b ? 0 : 4; r < 16; ++r) tops[r % 4] = fmaxf(tops[r % 4], s[i][b][r]);
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top = fmaxf(top, other_half(top)) * a.scale2;
             if (__any(top > m[i] + kLag)) {
                 const float to = fmaxf(m[i], top), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - to);
@@ -408,7 +436,6 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
         const float sum = l[i] + other_half(l[i]);
         const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
         const int64_t grow = q0 + token[i];
-        T *op = (T *)a.o + grow * a.o_stride + (int64_t)head[i] * a.dim;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -418,25 +445,25 @@ __global__ __launch_bounds__(256, QB == 1 && DP <= 128 ? 2 : 1) void prompt_kern
                 T4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = (T)(o[i][d][4 * r4 + e] * inv);
-                if (a.o_runs) { // rows of whole runs go through LDS, so that a store takes whole lines
-                    const int run = at4 / E;
-                    *reinterpret_cast<T4 *>(lds + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, run) * 16 + at4 % E * (int)sizeof(T)) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (at4 + e < a.dim && row < rows) op[at4 + e] = v[e];
-                }
+                *reinterpret_cast<T4 *>(lds + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, at4 / E) * 16 + at4 % E * (int)sizeof(T)) = v;
             }
         if (a.lse && h == 0 && row < rows) a.lse[grow * a.heads + head[i]] = sum == 0.f ? -INFINITY : (m[i] - kUp + __log2f(sum)) * kLn2;
     }
+    // a wave's rows, whole lines at a time
+    T *const o_first = (T *)a.o + (int64_t)(q0 + tok0) * a.o_stride + (int64_t)kvh * a.group * a.dim;
     if (a.o_runs) {
         constexpr int PO = 32 * QB * kRow / 1024;
 #pragma unroll
         for (int p = 0; p < PO; ++p) {
-            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = off % kRow / 16, row = row0 + r, tok = token_of(a, row);
+            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = off % kRow / 16;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + r * kRow + Lay::k_run(r, run) * 16);
-            T *op = (T *)a.o + (int64_t)(q0 + tok) * a.o_stride + (int64_t)(kvh * a.group + row - tok * a.group) * a.dim + run * E;
-            if (row < rows && run * E < a.dim) *reinterpret_cast<u32x4 *>(op) = v;
+            if (row0 + r < rows && run * E < a.dim) *reinterpret_cast<u32x4 *>(o_first + (row_at(row0 + r, a.o_stride) + run * E)) = v;
+        }
+    } else {
+        for (int r = wave * 32 * QB; r < (wave + 1) * 32 * QB && row0 + r < rows; ++r) {
+            T *op = o_first + row_at(row0 + r, a.o_stride);
+            for (int d = lane; d < a.dim; d += 64)
+                op[d] = *reinterpret_cast<const T *>(lds + r * kRow + Lay::k_run(r, d / E) * 16 + d % E * (int)sizeof(T));
         }
     }
 }
@@ -488,7 +515,7 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.q_rows = d->q_rows;
     a.kv_rows = d->kv_rows;
     const int per = 16 / e;
-    const bool runs = a.dim % per == 0 && (d->q_stride | d->k_stride | d->v_stride) % per == 0 && aligned16(q) && aligned16(k) && aligned16(v);
+    const bool runs = a.dim % per == 0 && d->q_stride * e <= (1 << 25) && (d->q_stride | d->k_stride | d->v_stride) % per == 0 && aligned16(q) && aligned16(k) && aligned16(v);
     a.o_runs = a.dim % per == 0 && d->o_stride % per == 0 && aligned16(o);
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
