@@ -22,6 +22,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The maximum that a row's weights are relative to may lag behind by 2^kLag, so that sums are rescaled seldom.
 constexpr float kLag = 8.f;
+constexpr int kRows = 128; // of a workgroup
 
 struct PromptArgs {
     const void *q, *k, *v;
@@ -31,7 +32,8 @@ struct PromptArgs {
     int64_t q_stride, k_stride, v_stride, o_stride;
     float scale2;      // |scale| log2 e
     uint32_t flip;     // sign bits of two 16-bit elements or one fp32 where the scale is negative
-    int32_t seqs, heads, kv_heads, group, dim, causal, q_rows, kv_rows;
+    float *part_o, *part_ml; // [item][kv head][split][kRows][head_dim padded], [..][2] (maximum and sum, base 2)
+    int32_t seqs, heads, kv_heads, group, dim, causal, q_rows, kv_rows, splits;
     uint32_t group_mul, group_shift; // row / group = row * group_mul >> 32 + group_shift (group_mul 0: row)
     int32_t o_runs;    // rows of o are whole, aligned 16-byte runs
 };
@@ -161,14 +163,13 @@ __device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32
 // This wave's copies have landed and its LDS reads are done, and so are every other wave's.
 __device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// T: element; DP: head_dim padded to a multiple of 32; KB: keys of a tile; QB: blocks of 32 rows per wave;
+// T: element; DP: head_dim padded to a multiple of 32; KB: keys of a tile;
 // RUNS: rows of q, k and v are whole, aligned 16-byte runs.
-template <class T, int DP, int KB, int QB, bool RUNS>
+template <class T, int DP, int KB, bool RUNS>
 __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUNS ? 3 : 2) : 1) void prompt_kernel(PromptArgs a) {
     typedef Tile<T, DP> Lay;
     constexpr int E = Lay::E, kRow = Lay::kRow, NC = kRow / 32; // NC: operand pieces of a row
     constexpr int B = KB / 32, DB = DP / 32;
-    constexpr int BM = 128 * QB;
     constexpr int kTile = KB * kRow;                     // bytes of a tile of K or V
     constexpr int PI = kTile / 1024 / 4;                 // a wave's 1 KB copies of one
     static_assert(kTile % 4096 == 0, "");
@@ -177,17 +178,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
     __shared__ __attribute__((aligned(16))) char lds[4 * kTile]; // K, V of the even tiles, then of the odd ones
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
-    const int kvh = (int)blockIdx.x % a.kv_heads, item = (int)blockIdx.x / a.kv_heads;
-    const Place at = find_place(a, item, BM);
+    const int kvh = (int)blockIdx.x % a.kv_heads, sp = (int)blockIdx.x / a.kv_heads % a.splits, item = (int)blockIdx.x / a.kv_heads / a.splits;
+    const Place at = find_place(a, item, kRows);
     if (at.tile < 0) return;
-    const int q0 = at.q0, nq = at.nq, k0 = at.k0, nk = at.nk;
-    const int rows = nq * a.group, row0 = at.tile * BM;
+    const int q0 = at.q0, nq = at.nq;
+    const int rows = nq * a.group, row0 = at.tile * kRows;
     // rows beyond the last take part as copies of it
-    auto limit_of = [&](int row) { // keys that a row sees
-        return a.causal ? min(max(token_of(a, min(row, rows - 1)) + nk - nq + 1, 0), nk) : nk;
+    auto keys_of = [&](int row) { // how many a row sees
+        return a.causal ? min(max(token_of(a, min(row, rows - 1)) + at.nk - nq + 1, 0), at.nk) : at.nk;
     };
-    const int wrow = row0 + wave * 32 * QB;
-    const int wave_min = limit_of(wrow), wave_max = limit_of(wrow + 32 * QB - 1), most = limit_of(row0 + BM - 1);
+    // This split's tiles of those that the last row sees; from here on keys are counted from their first.
+    const int all = (keys_of(row0 + kRows - 1) + KB - 1) / KB;
+    const int t_first = (int)((int64_t)all * sp / a.splits), tiles = (int)((int64_t)all * (sp + 1) / a.splits) - t_first;
+    const int k0 = at.k0 + t_first * KB, nk = min(at.nk - t_first * KB, tiles * KB);
+    auto limit_of = [&](int row) { return min(max(keys_of(row) - t_first * KB, 0), nk); };
+    const int wrow = row0 + wave * 32, limit = limit_of(wrow + n);
+    const int wave_min = limit_of(wrow), wave_max = limit_of(wrow + 31);
     const char *kb = (const char *)((const T *)a.k + (int64_t)k0 * a.k_stride + (int64_t)kvh * a.dim);
     const char *vb = (const char *)((const T *)a.v + (int64_t)k0 * a.v_stride + (int64_t)kvh * a.dim);
     const uint32_t k_bytes = (uint32_t)(a.k_stride * (int)sizeof(T)), v_bytes = (uint32_t)(a.v_stride * (int)sizeof(T));
@@ -240,7 +246,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
             *reinterpret_cast<u32x4 *>(lds + fetch_to + kTile + p * 1024 + lane * 16) = (u32x4){vw[0], vw[1], vw[2], vw[3]};
         }
     };
-    const int tiles = (most + KB - 1) / KB;
     if (tiles > 0) {
         if constexpr (RUNS) {
 #pragma unroll
@@ -258,36 +263,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
     const T *const q_first = (const T *)a.q + (int64_t)(q0 + tok0) * a.q_stride + (int64_t)kvh * a.group * a.dim;
     // Q's rows come through the odd tiles' place where they fit, whole lines at a time, a wave's own ones (24 sequences of 500 rows,
     // 32 heads of 128: 89.6 us, straight to registers 91.1; heads of 64 gain nothing, 155 and 151 at 1000 rows)
-    constexpr bool kStageQ = RUNS && DP > 64 && BM * kRow <= 2 * kTile;
+    constexpr bool kStageQ = RUNS && DP > 64 && kRows * kRow <= 2 * kTile;
     if constexpr (kStageQ) {
-        constexpr int PQ = 32 * QB * kRow / 1024;
+        constexpr int PQ = 32 * kRow / 1024;
         const uint32_t to = lds_at + 2 * kTile + wave * PQ * 1024;
 #pragma unroll
         for (int p = 0; p < PQ; ++p) {
-            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = min(Lay::k_run(r, off % kRow / 16), a.dim / E - 1);
+            const int off = p * 1024 + lane * 16, r = wave * 32 + off / kRow, run = min(Lay::k_run(r, off % kRow / 16), a.dim / E - 1);
             async_run((const char *)q_first, row_at(min(row0 + r, rows - 1), a.q_stride) * (uint32_t)sizeof(T) + (uint32_t)run * 16u, to + p * 1024);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    int limit[QB];
-    int head[QB], token[QB]; // of a lane's rows, the token from the sequence's first
-    u32x4 q[QB][NC];
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        const int row = wrow + 32 * i + n, r = min(row, rows - 1);
-        limit[i] = limit_of(row);
-        token[i] = token_of(a, r);
-        head[i] = kvh * a.group + (r - token[i] * a.group);
-        const T *qp = q_first + row_at(r, a.q_stride);
+    const int my_row = min(wrow + n, rows - 1), token = token_of(a, my_row), head = kvh * a.group + (my_row - token * a.group);
+    u32x4 q[NC];
+    {
+        const T *qp = q_first + row_at(my_row, a.q_stride);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d0 = (2 * c + h) * E;
             if constexpr (kStageQ)
-                q[i][c] = d0 >= a.dim ? (u32x4){0, 0, 0, 0} : *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, 2 * c + h) * 16);
-            else if constexpr (RUNS) q[i][c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
-            else q[i][c] = load_edge<T>(qp + d0, a.dim - d0);
+                q[c] = d0 >= a.dim ? (u32x4){0, 0, 0, 0}
+                                   : *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * 32 + n) * kRow + Lay::k_run(n, 2 * c + h) * 16);
+            else if constexpr (RUNS) q[c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
+            else q[c] = load_edge<T>(qp + d0, a.dim - d0);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) q[i][c][w] ^= a.flip;
+            for (int w = 0; w < 4; ++w) q[c][w] ^= a.flip;
         }
     }
 
@@ -308,13 +308,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         }
     }
 
-    f32x16 o[QB][DB] = {};
-    float m[QB], l[QB]; // base 2; l: this lane's half of the keys
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
-    }
+    f32x16 o[DB] = {};
+    float m = -INFINITY, l = 0.f; // base 2; l: this lane's half of the keys
     for (int t = 0; t < tiles; ++t) {
         all_ready(); // tile t is there, and every wave is done with tile t - 1
         if (t + 1 < tiles) {
@@ -333,7 +328,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         }
         const char *kt = lds + (t & 1) * 2 * kTile, *vt = kt + kTile;
 
-        f32x16 s[QB][B] = {};
+        f32x16 s[B] = {};
         // pieces of K's rows are read kAhead products before they are needed
         constexpr int kAhead = NC < 8 ? NC : 8;
         auto read_k = [&](int j) { return *reinterpret_cast<const u32x4 *>(kt + k_off[j % NC % NK] + j % NC / NK * NK * 32 + j / NC * 32 * kRow); };
@@ -347,10 +342,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
         for (int j = 0; j < B * NC; ++j) {
-#pragma unroll
-            for (int i = 0; i < QB; ++i) s[i][j / NC] = mfma32(kf[j % kAhead], q[i][j % NC], s[i][j / NC], T());
+            s[j / NC] = mfma32(kf[j % kAhead], q[j % NC], s[j / NC], T());
             if (RUNS && j % kEvery == kEvery - 1) fetch_piece(j / kEvery);
-            __builtin_amdgcn_sched_group_barrier(0x8, QB * (sizeof(T) == 2 ? 1 : 4), 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, sizeof(T) == 2 ? 1 : 4, 0);
             if (j + kAhead < B * NC) {
                 kf[j % kAhead] = read_k(j + kAhead);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -358,52 +352,46 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         }
         if (first + KB > wave_min) {
 #pragma unroll
-            for (int i = 0; i < QB; ++i)
-#pragma unroll
-                for (int b = 0; b < B; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (first + 32 * b + 8 * (r / 4) + 4 * h + r % 4 >= limit[i]) s[i][b][r] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            float tops[4]; // shorter chains
-#pragma unroll
-            for (int r = 0; r < 4; ++r) tops[r] = s[i][0][r];
-#pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int r = b ? 0 : 4; r < 16; ++r) tops[r % 4] = fmaxf(tops[r % 4], s[i][b][r]);
-            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            top = fmaxf(top, other_half(top)) * a.scale2;
-            if (__any(top > m[i] + kLag)) {
-                const float to = fmaxf(m[i], top), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - to);
-                m[i] = to;
-                l[i] *= alpha;
+                for (int r = 0; r < 16; ++r)
+                    if (first + 32 * b + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[b][r] = -INFINITY;
+        }
+        float tops[4]; // shorter chains
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[i][d] *= alpha;
+        for (int r = 0; r < 4; ++r) tops[r] = s[0][r];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int r = b ? 0 : 4; r < 16; ++r) tops[r % 4] = fmaxf(tops[r % 4], s[b][r]);
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        top = fmaxf(top, other_half(top)) * a.scale2;
+        if (__any(top > m + kLag)) {
+            const float to = fmaxf(m, top), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m - kUp;
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], a.scale2, -base));
+                l += s[b][r];
             }
-            const float base = m[i] == -INFINITY ? 0.f : m[i] - kUp;
-#pragma unroll
-            for (int b = 0; b < B; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[i][b][r] = __builtin_amdgcn_exp2f(fmaf(s[i][b][r], a.scale2, -base));
-                    l[i] += s[i][b][r];
-                }
-        }
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             if constexpr (sizeof(T) == 2) {
                 // weights enter the second product rounded once to T, as its operands have to be: off by half a step of T each, where
-                // the result is rounded by as much (their sum is taken of the unrounded ones)
+                // the result is rounded by as much (their sum is taken of the unrounded ones). In all 1.3 to 1.4 times the error of
+                // the result's rounding alone; a second part of each weight would cost half as much again of the products.
 #pragma unroll
                 for (int cc = 0; cc < 2; ++cc) {
-                    u32x4 p[QB];
+                    u32x4 p;
 #pragma unroll
-                    for (int i = 0; i < QB; ++i)
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) p[i][w] = pack2<T>(s[i][b][8 * cc + 2 * w], s[i][b][8 * cc + 2 * w + 1]);
+                    for (int w = 0; w < 4; ++w) p[w] = pack2<T>(s[b][8 * cc + 2 * w], s[b][8 * cc + 2 * w + 1]);
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
                         typedef __attribute__((address_space(3))) s16x4 *Piece;
@@ -411,9 +399,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
                         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)vp);
                         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)(vp + 8 * kRow));
                         const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
-                        const u32x4 vf = {wl[0], wl[1], wh[0], wh[1]};
-#pragma unroll
-                        for (int i = 0; i < QB; ++i) o[i][d] = mfma32(vf, p[i], o[i][d], T());
+                        o[d] = mfma32((u32x4){wl[0], wl[1], wh[0], wh[1]}, p, o[d], T());
                     }
                 }
             } else {
@@ -422,45 +408,53 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
                         const float vf = *reinterpret_cast<const float *>(vt + v_off[d % NV] + d / NV * NV * 128 + (32 * b + 8 * (r / 4) + r % 4) * kRow);
-#pragma unroll
-                        for (int i = 0; i < QB; ++i) o[i][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[i][b][r], o[i][d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[b][r], o[d], 0, 0, 0);
                     }
             }
         }
     }
 
-    __syncthreads(); // the tiles' place takes o's
+    const float sum = l + other_half(l);
+    const bool mine = wrow + n < rows;
+    if (a.splits > 1) { // as they are, for prompt_join_kernel
+        const int64_t part = ((int64_t)(item * a.kv_heads + kvh) * a.splits + sp) * kRows + wave * 32 + n;
+        if (mine) {
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        const int row = wrow + 32 * i + n;
-        const float sum = l[i] + other_half(l[i]);
-        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-        const int64_t grow = q0 + token[i];
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int at4 = 32 * d + 8 * r4 + 4 * h;
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                T4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)(o[i][d][4 * r4 + e] * inv);
-                *reinterpret_cast<T4 *>(lds + (wave * 32 * QB + 32 * i + n) * kRow + Lay::k_run(n, at4 / E) * 16 + at4 % E * (int)sizeof(T)) = v;
-            }
-        if (a.lse && h == 0 && row < rows) a.lse[grow * a.heads + head[i]] = sum == 0.f ? -INFINITY : (m[i] - kUp + __log2f(sum)) * kLn2;
+                for (int r4 = 0; r4 < 4; ++r4)
+                    *reinterpret_cast<f32x4 *>(a.part_o + part * DP + 32 * d + 8 * r4 + 4 * h) =
+                        (f32x4){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+            if (h == 0) *reinterpret_cast<float2 *>(a.part_ml + part * 2) = make_float2(m - kUp, sum);
+        }
+        return;
     }
+    __syncthreads(); // the tiles' place takes o's
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int at4 = 32 * d + 8 * r4 + 4 * h;
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(o[d][4 * r4 + e] * inv);
+            *reinterpret_cast<T4 *>(lds + (wave * 32 + n) * kRow + Lay::k_run(n, at4 / E) * 16 + at4 % E * (int)sizeof(T)) = v;
+        }
+    if (a.lse && h == 0 && mine) a.lse[(int64_t)(q0 + token) * a.heads + head] = sum == 0.f ? -INFINITY : (m - kUp + __log2f(sum)) * kLn2;
     // a wave's rows, whole lines at a time
     T *const o_first = (T *)a.o + (int64_t)(q0 + tok0) * a.o_stride + (int64_t)kvh * a.group * a.dim;
     if (a.o_runs) {
-        constexpr int PO = 32 * QB * kRow / 1024;
+        constexpr int PO = 32 * kRow / 1024;
 #pragma unroll
         for (int p = 0; p < PO; ++p) {
-            const int off = p * 1024 + lane * 16, r = wave * 32 * QB + off / kRow, run = off % kRow / 16;
+            const int off = p * 1024 + lane * 16, r = wave * 32 + off / kRow, run = off % kRow / 16;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + r * kRow + Lay::k_run(r, run) * 16);
             if (row0 + r < rows && run * E < a.dim) *reinterpret_cast<u32x4 *>(o_first + (row_at(row0 + r, a.o_stride) + run * E)) = v;
         }
     } else {
-        for (int r = wave * 32 * QB; r < (wave + 1) * 32 * QB && row0 + r < rows; ++r) {
+        for (int r = wave * 32; r < (wave + 1) * 32 && row0 + r < rows; ++r) {
             T *op = o_first + row_at(row0 + r, a.o_stride);
             for (int d = lane; d < a.dim; d += 64)
                 op[d] = *reinterpret_cast<const T *>(lds + r * kRow + Lay::k_run(r, d / E) * 16 + d % E * (int)sizeof(T));
@@ -468,24 +462,82 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
     }
 }
 
-template <class T, int DP, int KB, int QB>
-int launch(const PromptArgs &a, bool runs, hipStream_t st) {
-    constexpr int BM = 128 * QB;
-    const int64_t items = (int64_t)a.q_rows * a.group / BM + std::min(a.seqs, a.q_rows);
-    const int64_t grid = items * a.kv_heads;
+// The splits' sums of a row, added in split order: a wave a row, a lane a split's weight, then four elements.
+template <class T>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, int part_row) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int kBlocks = kRows / 4; // of an (item, kv head)
+    const int block = (int)blockIdx.x / kBlocks, r = (int)blockIdx.x % kBlocks * 4 + wave, kvh = block % a.kv_heads;
+    const Place at = find_place(a, block / a.kv_heads, kRows);
+    const int row = at.tile * kRows + r;
+    if (at.tile < 0 || row >= at.nq * a.group) return;
+    const int tok = token_of(a, row), head = kvh * a.group + (row - tok * a.group);
+    const int64_t part = (int64_t)block * a.splits * kRows + r; // its first split
+    const float2 ml = lane < a.splits ? *reinterpret_cast<const float2 *>(a.part_ml + (part + (int64_t)lane * kRows) * 2) : make_float2(-INFINITY, 0.f);
+    float M = ml.x;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+    const float w = __builtin_amdgcn_exp2f(ml.x - (M == -INFINITY ? 0.f : M));
+    float L = ml.y * w;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    if (a.lse && lane == 0) a.lse[(int64_t)(at.q0 + tok) * a.heads + head] = L == 0.f ? -INFINITY : (M + __log2f(L)) * kLn2;
+    T *op = (T *)a.o + (int64_t)(at.q0 + tok) * a.o_stride + (int64_t)head * a.dim;
+    const int d0 = lane * 4;
+    if (d0 >= a.dim) return;
+    const float *from = a.part_o + part * part_row + d0;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s)
+        v += *reinterpret_cast<const f32x4 *>(from + (int64_t)s * kRows * part_row) *
+             __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (d0 + e < a.dim) op[d0 + e] = (T)(v[e] * inv);
+}
+
+// How the rows and keys are cut.
+struct Cut {
+    int64_t items; // tiles of kRows rows at most
+    int pad;       // head_dim padded
+    int splits;
+};
+Cut cut(const SpinnHipPromptAttentionDesc *d) {
+    Cut c;
+    const int64_t group = d->heads / d->kv_heads;
+    c.items = (int64_t)d->q_rows * group / kRows + std::min(d->seqs, d->q_rows);
+    c.pad = d->head_dim <= 64 ? 64 : (d->head_dim <= 96 ? 96 : (d->head_dim <= 128 ? 128 : 256));
+    // Keys are split where workgroups of whole rows leave most of the device idle: into as many parts as two workgroups a CU take, of
+    // 8 tiles at least, up to the join's 64. The parts' sums and the second launch cost some 10 us, so that is for 16 tiles less at least
+    // (32 heads on 8 of 128, bf16: 16 rows over 4000 keys 68 -> 19 us, over 64000 1014 -> 66, 100 over 4000 69 -> 27; 1000 over 1000,
+    // which stays whole, 24, in two 36).
+    const int64_t tiles = ((int64_t)d->kv_rows / std::max(d->seqs, 1) + 63) / 64; // of an ordinary sequence
+    const int64_t most = std::min({2 * device_cu_count() / std::max<int64_t>(c.items * d->kv_heads, 1), tiles / 8, (int64_t)64});
+    c.splits = most >= 2 && tiles * (most - 1) / most >= 16 ? (int)most : 1;
+    return c;
+}
+
+template <class T, int DP, int KB>
+int launch(const PromptArgs &a, const Cut &c, bool runs, hipStream_t st) {
+    const int64_t grid = c.items * a.kv_heads * c.splits;
     if (!launch_fits(grid, 256)) return SPINN_HIP_EUNSUPPORTED;
-    if (runs) prompt_kernel<T, DP, KB, QB, true><<<(unsigned)grid, 256, 0, st>>>(a);
-    else prompt_kernel<T, DP, KB, QB, false><<<(unsigned)grid, 256, 0, st>>>(a);
+    if (runs) prompt_kernel<T, DP, KB, true><<<(unsigned)grid, 256, 0, st>>>(a);
+    else prompt_kernel<T, DP, KB, false><<<(unsigned)grid, 256, 0, st>>>(a);
+    if (c.splits > 1) prompt_join_kernel<T><<<(unsigned)(c.items * a.kv_heads * (kRows / 4)), 256, 0, st>>>(a, DP);
     return check_launch();
 }
 
 } // namespace
 
-size_t prompt_attention_workspace_bytes(const SpinnHipPromptAttentionDesc *) { return 0; }
+size_t prompt_attention_workspace_bytes(const SpinnHipPromptAttentionDesc *d) {
+    const Cut c = cut(d);
+    return c.splits > 1 ? (size_t)(c.items * d->kv_heads * c.splits) * kRows * (c.pad + 2) * 4 : 0;
+}
 
 int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const void *k, const void *v, const int32_t *starts,
                      const int32_t *kv_starts, void *o, float *lse, void *ws, hipStream_t st) {
-    (void)ws;
+    const Cut c = cut(d);
     PromptArgs a{};
     a.q = q;
     a.k = k;
@@ -508,6 +560,9 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.group = d->heads / d->kv_heads;
     a.dim = d->head_dim;
     a.causal = d->causal;
+    a.splits = c.splits;
+    a.part_o = (float *)ws;
+    a.part_ml = (float *)ws + c.items * d->kv_heads * c.splits * kRows * c.pad;
     if (a.group > 1) { // exact for rows under 2^31
         while ((2u << a.group_shift) < (uint32_t)a.group) ++a.group_shift;
         a.group_mul = (uint32_t)(((1ull << (32 + a.group_shift)) + a.group - 1) / a.group);
@@ -520,10 +575,10 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
         constexpr int K = sizeof(T) == 2 ? 64 : 32;
-        if (a.dim <= 64) return launch<T, 64, K, 1>(a, runs, st);
-        if (a.dim <= 96) return launch<T, 96, K, 1>(a, runs, st);
-        if (a.dim <= 128) return launch<T, 128, K, 1>(a, runs, st);
-        return launch<T, 256, 32, 1>(a, runs, st);
+        if (c.pad == 64) return launch<T, 64, K>(a, c, runs, st);
+        if (c.pad == 96) return launch<T, 96, K>(a, c, runs, st);
+        if (c.pad == 128) return launch<T, 128, K>(a, c, runs, st);
+        return launch<T, 256, 32>(a, c, runs, st);
     });
 }
 

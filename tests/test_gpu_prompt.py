@@ -182,3 +182,48 @@ def test_streams_at_once(hip):
     for p in ps:
         o, tol, _, _ = p.ref(0.3, 1)
         assert_close(p.o.cpu().reshape(o.shape), o, tol, "streams")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("causal", [1, 0], ids=["causal", "full"])
+@pytest.mark.parametrize("lens,kv_lens,heads,kv,dim", [([3], [5000], 4, 2, 64), ([1], [2500], 1, 1, 128), ([1, 0, 20, 7], [3000, 100, 9000, 0], 8, 2, 80),
+                                                       ([130], [4100], 2, 1, 96), ([5, 5], [1300, 3000], 3, 3, 33), ([2], [2600], 2, 1, 256)], ids=str)
+def test_few_rows_over_many_keys(hip, dtype, causal, lens, kv_lens, heads, kv, dim):
+    """Keys split over workgroups and joined: parts of ordinary length, short and empty ones, sequences without keys."""
+    p = Prompt(gen(len(lens) + dim), dtype, lens, heads, kv, dim, kv_lens=kv_lens, lead=1, tail=2)
+    check(hip, p, dim ** -0.5, causal, what=f"few rows {lens} {kv_lens}")
+    assert p.ws is not None, "not split"
+    first, lse = p.o.clone(), p.lse.clone()
+    p.run(hip, dim ** -0.5, causal)
+    assert torch.equal(first, p.o) and torch.equal(lse.view(torch.int32), p.lse.view(torch.int32))
+
+
+def test_captured_with_other_lengths(hip):
+    """A captured call replayed while the starts in memory change; its workspace dirtied between the replays."""
+    import ctypes as C
+
+    from tests.decodeops import ptr, stream, workspace
+    p = Prompt(gen(11), BF16, [40, 40], 4, 2, 64, kv_lens=[2000, 3000])
+    for rows in ((p.rows, p.kv_rows), (p.rows, p.kv_rows // 16)):  # split and not
+        d = hip.PromptAttentionDesc(dtype=BF16, seqs=2, heads=4, kv_heads=2, head_dim=64, causal=1, q_rows=rows[0], kv_rows=rows[1], scale=0.2,
+                                    q_stride=p.q.stride(0), k_stride=p.k.stride(0), v_stride=p.v.stride(0), o_stride=p.o.stride(0))
+        size = hip.lib().spinn_hip_prompt_attention_workspace_size(C.byref(d))
+        ws = workspace(size)
+        starts, kv_starts = (torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(2))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            hip.check(hip.lib().spinn_hip_prompt_attention(C.byref(d), ptr(p.q), ptr(p.k), ptr(p.v), ptr(starts), ptr(kv_starts), ptr(p.o), None,
+                                                           ptr(ws), size, stream()), "prompt")
+        for a, b in (([0, 40, 80], [0, rows[1] // 3, rows[1]]), ([0, 1, 30], [0, 70, 90]), ([5, 5, 80], [0, 0, rows[1]])):
+            starts.copy_(torch.tensor(a, dtype=torch.int32))
+            kv_starts.copy_(torch.tensor(b, dtype=torch.int32))
+            p.o.fill_(7.0)
+            if ws is not None:
+                ws.fill_(0xFF)
+            graph.replay()
+            torch.cuda.synchronize()
+            p.starts, p.kv_starts = a, b
+            o, tol, _, _ = p.ref(0.2, 1)
+            got = p.o.cpu().reshape(o.shape)
+            assert_close(got[a[0]:a[2]], o[a[0]:a[2]], tol[a[0]:a[2]], f"replay {a} {b}")
+            assert (got[a[2]:] == 7).all() and (got[:a[0]] == 7).all()
