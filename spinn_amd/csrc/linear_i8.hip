@@ -183,7 +183,7 @@ inline int64_t m_tiles(const SpinnHipLinearI8Desc *d) { return ((int64_t)d->m + 
 //  * stream kernel on MT x NT blocks: 2 + 0.02 f (MT + NT) a round of its grid (45 x 5120 x 8192: 1 x 4 blocks 16.2, 2 x 2
 //    18.4, 2 x 4 17.5, 4 x 4 25.0; 64 x 14336 x 4096: 18.8 on 4 x 4, 23.0 on 2 x 4, 36.6 on 1 x 4; 100 x 4096 x 4096: 8.7 on 2 x 4, 11.4 on
 //    1 x 4, 12.9 on 4 x 4; 8 x 14336 x 4096: 12.5 on 1 x 2, 14.9 on 1 x 1);
-//  * 64 x 128 tiles: 5.5 + 0.2 f / splits, 5 more where K is split, 5.5 + 0.18 f a round from more than one per CU (200 x 1024 x 16384:
+//  * 64 x 128 tiles: 5.5 + 0.2 f / splits, 6 more where K is split, 5.5 + 0.18 f a round from more than one per CU (200 x 1024 x 16384:
 //    54.6 whole, 34.1 in two, 22.6 in four, the stream kernel 24.8; 500 x 1024 x 1024: 8.2, stream 5.0);
 //  * 128 x 128 tiles: 5.5 + 0.23 f up to one per CU (150 x 14336 x 4096: 24.0, 64 x 128 27.5, stream 38.1); beyond, and for
 //    256 x 256 from one per CU, as the other types.
@@ -205,7 +205,7 @@ Choice choose(const SpinnHipLinearI8Desc *d) {
     }
     const int64_t tiles = grid(4, 8);
     const int64_t splits = std::max<int64_t>(1, std::min(cus / tiles, f / 16));
-    const double whole = tiles <= cus ? 5.5 + 0.2 * f : 5.5 + 0.18 * f * rounds(tiles), parts = 10.5 + 0.2 * f / splits;
+    const double whole = tiles <= cus ? 5.5 + 0.2 * f : 5.5 + 0.18 * f * rounds(tiles), parts = 11.5 + 0.2 * f / splits;
     if (std::min(whole, parts) < least) {
         least = std::min(whole, parts);
         c.kind = Choice::kTile64;
