@@ -536,7 +536,7 @@ int spinn_hip_prompt_attention(const SpinnHipPromptAttentionDesc *d, const void 
 /*
  * Rows to 8-bit integers with a scale each: scale[i] = max_j |x[i,j]| / 127 in fp32, xq[i,j] = x[i,j] / scale[i] rounded
  * to the nearest integer, ties to even (of the exact quotient; 0 where the scale is 0; within +-127). A row with a NaN or an
- * infinity gets scale NaN and zeros. Rows are ldx and ldq apart; x needs its element's alignment, xq starts at a
+ * infinity gets scale NaN and zeros. Rows are ldx and ldq apart (up to 2^28); x needs its element's alignment, xq starts at a
  * multiple of 16, ldq is one and at least k; xq[i, k .. k rounded up to 16) is filled with zeros.
  */
 int spinn_hip_quantize_rows(int32_t dtype, int64_t rows, int32_t k, const void *x, int64_t ldx, int8_t *xq, int64_t ldq,

@@ -132,7 +132,7 @@ int spinn_hip_quantize_rows(int32_t dtype, int64_t rows, int32_t k, const void *
                             float *scale, void *stream) {
     constexpr int64_t kFar = (int64_t)1 << 28;
     if (!dtype_bytes(dtype) || rows < 0 || rows > ((int64_t)1 << 31) || k <= 0 || k > INT32_MAX - 1024) return SPINN_HIP_EINVAL;
-    if (ldx < k || ldq < k || ldq % 16 || ldx > kFar * 16 || ldq > kFar * 16) return SPINN_HIP_EINVAL;
+    if (ldx < k || ldq < k || ldq % 16 || ldx > kFar || ldq > kFar) return SPINN_HIP_EINVAL;
     if (rows == 0) return SPINN_HIP_OK;
     if (!x || !xq || !scale || !aligned16(xq) || !multiple_of(x, dtype_bytes(dtype))) return SPINN_HIP_EINVAL;
     return quantize_rows(dtype, rows, k, x, ldx, xq, ldq, scale, (hipStream_t)stream);

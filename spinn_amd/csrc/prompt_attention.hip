@@ -77,6 +77,7 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
         return {tile, first, __builtin_amdgcn_readlane(q1, seq) - first, kfirst,
                 max(__builtin_amdgcn_readlane(k1, seq) - kfirst, 0)};
     }
+    constexpr int kMany = 1 << 28; // sums stop here, behind all items: those of starts that do not ascend would pass 32 bits
     int first = 0, left = a.seqs, before = 0;
     while (true) { // 64 shares of the sequences left, until a share is one
         const int each = (left + 63) / 64;
@@ -84,18 +85,18 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
         for (int i = 0; i < each; ++i) {
             const int s = lane * each + i;
             if (s < left)
-                n += (max(clamped(a.starts, first + s + 1, a.q_rows) - clamped(a.starts, first + s, a.q_rows), 0) * a.group + rows - 1) / rows;
+                n = min(n + (max(clamped(a.starts, first + s + 1, a.q_rows) - clamped(a.starts, first + s, a.q_rows), 0) * a.group + rows - 1) / rows, kMany);
         }
         int upto = n;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const int o = __shfl_up(upto, d);
-            if (lane >= d) upto += o;
+            if (lane >= d) upto = min(upto + o, kMany);
         }
         const unsigned long long behind = __ballot(before + upto > item);
         if (!behind) return {-1, 0, 0, 0, 0};
         const int w = __ffsll(behind) - 1;
-        before += __builtin_amdgcn_readlane(upto - n, w);
+        before += w ? __builtin_amdgcn_readlane(upto, w - 1) : 0;
         first += w * each;
         left = min(each, left - w * each);
         if (each == 1) {
@@ -151,13 +152,13 @@ __device__ __forceinline__ float other_half(float v) { // lane ^ 32's
 
 // 16 bytes a lane from base + off to byte `to` + 16 lane of LDS; all_ready() waits for it. In assembly, since the compiler would wait for all
 // of these before every transposing read of LDS that follows, whatever it reads (16000 rows: 2020 -> 1916 us).
-// lanes: all (~0) or none (0), without a branch.
+// lanes: those that take part; none are left out without a branch.
 __device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32_t to, uint64_t lanes = ~0ull) {
-    uint64_t all;
-    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, exec\n\ts_mov_b64 exec, %4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
-                 : "=&s"(all)
+    uint64_t here;
+    asm volatile("s_mov_b32 m0, %1\n\ts_and_saveexec_b64 %0, %4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
+                 : "=&s"(here)
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "s"(lanes)
-                 : "memory", "m0");
+                 : "memory", "m0", "scc");
 }
 
 // This wave's copies have landed and its LDS reads are done, and so are every other wave's.
@@ -570,7 +571,7 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.q_rows = d->q_rows;
     a.kv_rows = d->kv_rows;
     const int per = 16 / e;
-    const bool runs = a.dim % per == 0 && d->q_stride * e <= (1 << 25) && (d->q_stride | d->k_stride | d->v_stride) % per == 0 && aligned16(q) && aligned16(k) && aligned16(v);
+    const bool runs = a.dim % per == 0 && d->q_stride * e <= (1 << 24) && (d->q_stride | d->k_stride | d->v_stride) % per == 0 && aligned16(q) && aligned16(k) && aligned16(v);
     a.o_runs = a.dim % per == 0 && d->o_stride % per == 0 && aligned16(o);
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;

@@ -185,7 +185,9 @@ int rope_run(const SpinnHipRopeDesc *d, int64_t tokens, const int32_t *position,
     const int64_t per_token = (int64_t)a.heads * a.units;
     // 1024 units or more a workgroup (sines and cosines shared by what there is), but two workgroups a CU first
     int64_t n = 1;
-    while (n * per_token < 1024 && tokens / (2 * n) >= 2 * device_cu_count() && 2 * n * half * 8 <= 32768) n *= 2;
+    while (2 * n * half * 8 <= 32768 && ((n * per_token < 1024 && tokens / (2 * n) >= 2 * device_cu_count()) || !launch_fits((tokens + n - 1) / n, 256)) &&
+           2 * n * per_token < (int64_t)1 << 31)
+        n *= 2;
     a.per_block = (int32_t)n;
     const int64_t grid = (tokens + n - 1) / n;
     if (!launch_fits(grid, 256)) return SPINN_HIP_EUNSUPPORTED;

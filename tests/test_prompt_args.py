@@ -169,7 +169,7 @@ def test_quantize_arguments(native):
     def call(dtype=F32, rows=2, k=33, x=P, ldx=33, xq=Q, ldq=48, scale=P):
         return L.spinn_hip_quantize_rows(dtype, rows, k, x, ldx, xq, ldq, scale, None)
 
-    for kw in (dict(dtype=3), dict(rows=-1), dict(k=0), dict(ldx=32), dict(ldq=32), dict(ldq=40), dict(x=None), dict(xq=None), dict(scale=None),
+    for kw in (dict(dtype=3), dict(rows=-1), dict(k=0), dict(ldx=32), dict(ldq=32), dict(ldq=40), dict(ldx=(1 << 28) + 1), dict(ldq=(1 << 28) + 16), dict(x=None), dict(xq=None), dict(scale=None),
                dict(x=ODD), dict(xq=C.c_void_p(8200))):
         assert call(**kw) == EINVAL, kw
     assert call(rows=0, x=None, xq=None, scale=None) == 0
