@@ -4,10 +4,16 @@
 // 4 head_dim flops a visible pair: the matrix cores bound it, and beside them the exponentials, one a pair.
 //
 // The rows of a tile are (token, query head of the group) pairs, so that all heads that share a kv head share its
-// tiles in LDS. S^T = K Q^T: an accumulator's column, so a lane, is one row of queries, its maximum and sum
-// are the lane's own and its partner's (lane ^ 32), and a mask is one number a lane. The products' elements that a lane
+// tiles in LDS. S^T = K Q^T: an accumulator's column, so a lane and one (fp32: three) more, is one row of queries; its maximum and sum
+// need an exchange among those, and a mask is one number a lane. The products' elements that a lane
 // holds are exactly the operand that O^T = V^T P^T wants from it (contraction over keys may run in any order); V^T comes
-// out of LDS transposed by the read itself (16-bit types) or is read element by element (fp32).
+// out of LDS transposed by the read itself (16-bit types) or by whole runs of a row (fp32).
+//
+// 16-bit types: 128 rows a workgroup, tiles of 64 keys, 32 x 32 instructions, two workgroups a CU (heads of 128). 16000 rows, 32 heads on 8
+// of 128, bf16, causal: 1830 to 2040 us by the card, up to 1150 TFLOP/s, bound by power (1400 us on zeros); 24 sequences of 37 to 2000 rows: 327 us.
+// fp32: 64 rows, tiles of 16 keys, 16 x 16 instructions at the same rate: less padding (80 columns are five blocks) and small
+// enough for five workgroups a CU. 8 x 577 rows, 16 heads of 80: 127 us, 107 TFLOP/s (32 x 32 instructions, 128 rows: 179); 4 x 2000 of 128
+// 618 (670); 2 x 1000, 8 heads on 2 of 256: 141 (277).
 #include "decode.h"
 #include <cmath>
 #include <type_traits>
@@ -16,13 +22,16 @@ namespace spinn {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The maximum that a row's weights are relative to may lag behind by 2^kLag, so that sums are rescaled seldom.
 constexpr float kLag = 8.f;
-constexpr int kRows = 128; // of a workgroup
+// Rows of a wave and of a workgroup: the matrix instructions' size, 32 x 32 for 16-bit types, 16 x 16 for fp32.
+template <class T> constexpr int kWaveRows = sizeof(T) == 2 ? 32 : 16;
+template <class T> constexpr int kRows = 4 * kWaveRows<T>;
 
 struct PromptArgs {
     const void *q, *k, *v;
@@ -36,6 +45,7 @@ struct PromptArgs {
     int32_t seqs, heads, kv_heads, group, dim, causal, q_rows, kv_rows, splits;
     uint32_t group_mul, group_shift; // row / group = row * group_mul >> 32 + group_shift (group_mul 0: row)
     int32_t o_runs;    // rows of o are whole, aligned 16-byte runs
+    int32_t at_once;   // all workgroups are on the device together
 };
 
 __device__ __forceinline__ int token_of(const PromptArgs &a, int row) {
@@ -59,7 +69,7 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
         const int q0 = clamped(a.starts, s, a.q_rows), q1 = clamped(a.starts, s + 1, a.q_rows);
         const int k0 = clamped(ks, s, a.kv_rows), k1 = clamped(ks, s + 1, a.kv_rows);
         const int n = lane < a.seqs ? (max(q1 - q0, 0) * a.group + rows - 1) / rows : 0;
-        // tiles of the sequences that come first: those of more tiles (under 2^24), or as many and an earlier lane
+        // tiles of the sequences that come first: those of more tiles (up to 2^25), or as many and an earlier lane
         const uint32_t key = (uint32_t)n << 6 | (uint32_t)(63 - lane);
         int before = 0;
         if (a.seqs > 1) {
@@ -107,31 +117,35 @@ __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int r
     }
 }
 
-// How 16-byte runs of a row lie in LDS, so that lanes that read a column of them, and lanes that read pieces of four rows, meet all banks.
+// How 16-byte runs of a row lie in LDS, so that lanes that read a column of them (K), and lanes that read pieces of four rows (V in 16-bit
+// types), meet all banks. V in fp32 is read by whole 256 bytes of a row.
 template <class T, int DP>
 struct Tile {
     static constexpr int E = 16 / (int)sizeof(T);
     static constexpr int kRow = DP * (int)sizeof(T);  // bytes
     static constexpr int kRuns = kRow / 16;
     static constexpr int kPow2 = (kRuns & -kRuns) < 16 ? (kRuns & -kRuns) : 16; // runs that may change places among each other
-    __device__ __forceinline__ static int k_run(int row, int run) { return run ^ ((row / (16 / kPow2)) & (kPow2 - 1)); }
     static constexpr int kBlocks = kRow / 64, kBlockPow2 = (kBlocks & -kBlocks) < 4 ? (kBlocks & -kBlocks) : 4;
-    __device__ __forceinline__ static int v_run(int row, int run) {
-        if constexpr (sizeof(T) == 2) return run ^ (((row / (4 / kBlockPow2)) & (kBlockPow2 - 1)) << 2);
-        else return DP % 64 == 0 ? run ^ (((row >> 2) & 1) << 3) : run;
+    static constexpr int log2of(int n) { return n > 1 ? 1 + log2of(n / 2) : 0; }
+    __device__ __forceinline__ static int k_run(int row, int run) { return run_of(false, row, run); }
+    __device__ __forceinline__ static int v_run(int row, int run) { return run_of(true, row, run); }
+    __device__ __forceinline__ static int run_of(bool v, int row, int run) { // without a branch on v, which a wave knows
+        const int down = v ? log2of(4 / kBlockPow2) : log2of(16 / kPow2), up = v ? 2 : 0;
+        const int mask = v ? (sizeof(T) == 2 ? kBlockPow2 - 1 : 0) : kPow2 - 1;
+        return run ^ ((row >> down & mask) << up);
     }
 };
 
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, _Float16) {
+__device__ __forceinline__ f32x16 mfma_piece(u32x4 a, u32x4 b, f32x16 c, _Float16) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, __bf16) {
+__device__ __forceinline__ f32x16 mfma_piece(u32x4 a, u32x4 b, f32x16 c, __bf16) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c, float) {
+__device__ __forceinline__ f32x4 mfma_piece(u32x4 a, u32x4 b, f32x4 c, float) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, (uint32_t)a[e]), __builtin_bit_cast(float, (uint32_t)b[e]), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (uint32_t)a[e]), __builtin_bit_cast(float, (uint32_t)b[e]), c, 0, 0, 0);
     return c;
 }
 
@@ -144,41 +158,71 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-__device__ __forceinline__ float other_half(float v) { // lane ^ 32's
+// A row's value out of those of its lanes, lane % 32 (or 16).
+template <int R, class F>
+__device__ __forceinline__ float across(float v, F f) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return __builtin_bit_cast(float, (uint32_t)((threadIdx.x & 32) ? r[0] : r[1]));
+    const auto far = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    v = f(__builtin_bit_cast(float, (uint32_t)far[0]), __builtin_bit_cast(float, (uint32_t)far[1]));
+    if constexpr (R == 16) {
+        const uint32_t c = __builtin_bit_cast(uint32_t, v);
+        const auto near = __builtin_amdgcn_permlane16_swap(c, c, false, false);
+        v = f(__builtin_bit_cast(float, (uint32_t)near[0]), __builtin_bit_cast(float, (uint32_t)near[1]));
+    }
+    return v;
 }
 
 // 16 bytes a lane from base + off to byte `to` + 16 lane of LDS; all_ready() waits for it. In assembly, since the compiler would wait for all
 // of these before every transposing read of LDS that follows, whatever it reads (16000 rows: 2020 -> 1916 us).
-// lanes: those that take part; none are left out without a branch.
-__device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32_t to, uint64_t lanes = ~0ull) {
+// lanes: -1 all of those that are here, 0 none, without a branch.
+__device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32_t to, int lanes = -1) {
     uint64_t here;
     asm volatile("s_mov_b32 m0, %1\n\ts_and_saveexec_b64 %0, %4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
                  : "=&s"(here)
-                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "s"(lanes)
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "s"((int64_t)__builtin_amdgcn_readfirstlane(lanes))
                  : "memory", "m0", "scc");
 }
 
 // This wave's copies have landed and its LDS reads are done, and so are every other wave's.
 __device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// T: element; DP: head_dim padded to a multiple of 32; KB: keys of a tile;
+// Workgroups on a CU, as registers and LDS allow.
+template <class T, int DP, bool RUNS>
+constexpr int kBlocks = sizeof(T) == 4 ? (DP == 64 ? 5 : DP <= 96 ? 4 + RUNS : DP == 128 ? 3 + RUNS : 2) : DP <= 128 ? (DP == 96 && RUNS ? 3 : 2) : 1;
+
+// What a matrix product has just left in s may be read. The compiler counts the wait that is due along one way into a block only
+// (16 x 16 x 4 fp32: 10 instructions by the masked way, 1 by the other, where it put none), so it is written out here.
+template <class T, int B, class Acc>
+__device__ __forceinline__ void settle(Acc (&s)[B]) {
+    if constexpr (sizeof(T) == 2) asm volatile("s_nop 7\n\ts_nop 3" : "+v"(s[B - 1]));
+    else asm volatile("s_nop 7\n\ts_nop 1" : "+v"(s[B - 1]));
+#pragma unroll
+    for (int b = 0; b < B - 1; ++b) asm volatile("" : "+v"(s[b]));
+}
+
+// T: element; DP: head_dim padded to whole matrix operands; KB: keys of a tile;
 // RUNS: rows of q, k and v are whole, aligned 16-byte runs.
 template <class T, int DP, int KB, bool RUNS>
-__global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUNS ? 3 : 2) : 1) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(PromptArgs a) {
     typedef Tile<T, DP> Lay;
-    constexpr int E = Lay::E, kRow = Lay::kRow, NC = kRow / 32; // NC: operand pieces of a row
-    constexpr int B = KB / 32, DB = DP / 32;
-    constexpr int kTile = KB * kRow;                     // bytes of a tile of K or V
-    constexpr int PI = kTile / 1024 / 4;                 // a wave's 1 KB copies of one
-    static_assert(kTile % 4096 == 0, "");
+    constexpr int R = kWaveRows<T>, G = 64 / R, kRows = ::spinn::kRows<T>; // G: lanes of a row
+    typedef float Acc __attribute__((ext_vector_type(R * R / 64)));
+    constexpr int A4 = R * R / 256; // fours of an accumulator: rows 4 G i + 4 h ..
+    constexpr int E = Lay::E, kRow = Lay::kRow, NC = kRow / (16 * G); // NC: operand pieces of a row
+    constexpr int B = KB / R, DB = DP / R;
+    // fp32: the columns of O that four (two, one) accumulators in a row hold go round among them, so that a lane's pieces of V's row lie
+    // next to each other, and so do four elements of O's.
+    constexpr int kFull = DB / 4 * 4, kRest = DB % 4;
+    static_assert(sizeof(T) == 2 || kRest != 3, "");
+    constexpr int kTile = KB * kRow;        // bytes of a tile of K or V
+    constexpr int kCopies = kTile / 1024;   // of 1 KB: two waves copy K, two V
+    constexpr int P = (kCopies + 1) / 2;    // a wave's
+    static_assert(kTile % 1024 == 0 && NC * 16 * G == kRow && P <= B * NC, "");
     // fp16's weights are kept 2^7 higher: its least number is 2^-24, which many small ones together fall under
     constexpr float kUp = __is_same(T, _Float16) ? 7.f : 0.f;
     __shared__ __attribute__((aligned(16))) char lds[4 * kTile]; // K, V of the even tiles, then of the odd ones
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 31, h = lane >> 5;
+    const int n = lane % R, h = lane / R;
     const int kvh = (int)blockIdx.x % a.kv_heads, sp = (int)blockIdx.x / a.kv_heads % a.splits, item = (int)blockIdx.x / a.kv_heads / a.splits;
     const Place at = find_place(a, item, kRows);
     if (at.tile < 0) return;
@@ -193,64 +237,59 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
     const int t_first = (int)((int64_t)all * sp / a.splits), tiles = (int)((int64_t)all * (sp + 1) / a.splits) - t_first;
     const int k0 = at.k0 + t_first * KB, nk = min(at.nk - t_first * KB, tiles * KB);
     auto limit_of = [&](int row) { return min(max(keys_of(row) - t_first * KB, 0), nk); };
-    const int wrow = row0 + wave * 32, limit = limit_of(wrow + n);
-    const int wave_min = limit_of(wrow), wave_max = limit_of(wrow + 31);
-    const char *kb = (const char *)((const T *)a.k + (int64_t)k0 * a.k_stride + (int64_t)kvh * a.dim);
-    const char *vb = (const char *)((const T *)a.v + (int64_t)k0 * a.v_stride + (int64_t)kvh * a.dim);
-    const uint32_t k_bytes = (uint32_t)(a.k_stride * (int)sizeof(T)), v_bytes = (uint32_t)(a.v_stride * (int)sizeof(T));
+    const int wrow = row0 + wave * R, limit = limit_of(wrow + n);
+    const int wave_min = limit_of(wrow), wave_max = limit_of(wrow + R - 1);
+    const bool is_v = wave >= 2; // what this wave copies
+    const int64_t stride = is_v ? a.v_stride : a.k_stride;
+    const char *const from_first = (const char *)((const T *)(is_v ? a.v : a.k) + (int64_t)k0 * stride + (int64_t)kvh * a.dim);
+    const uint32_t row_bytes = (uint32_t)(stride * (int)sizeof(T));
+    const int copy0 = (wave & 1) * P; // its first copy of the tile's
     // Bytes from a tile's first row to a lane's runs. Runs behind dim are copies of the last one: Q's are zeros there.
-    uint32_t k_from[PI], v_from[PI];
+    uint32_t from[P];
     auto from_rows = [&](int left) { // of a tile whose row `left` is the last that there is: rows behind it are copies of it
+        int here = lane;
+        asm volatile("" : "+v"(here)); // so that nothing for the last tile is kept in registers throughout
 #pragma unroll
-        for (int p = 0; p < PI; ++p) {
-            const int at = (wave * PI + p) * 1024 + lane * 16, row = min(at / kRow, left), place = at % kRow / 16;
-            const int last = a.dim / E - 1, kr = min(Lay::k_run(at / kRow, place), last), vr = min(Lay::v_run(at / kRow, place), last);
-            k_from[p] = (uint32_t)row * k_bytes + (uint32_t)kr * 16u;
-            v_from[p] = (uint32_t)row * v_bytes + (uint32_t)vr * 16u;
+        for (int p = 0; p < P; ++p) {
+            const int at = (copy0 + p) * 1024 + here * 16, run = min(Lay::run_of(is_v, at / kRow, at % kRow / 16), a.dim / E - 1);
+            from[p] = (uint32_t)min(at / kRow, left) * row_bytes + (uint32_t)run * 16u;
         }
     };
     if constexpr (RUNS) from_rows(min(nk, KB) - 1);
-    const char *k_at = kb, *v_at = vb; // the tile to fetch next
+    const char *from_at = from_first; // the tile to fetch next
     const uint32_t lds_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)lds;
-    uint32_t fetch_to = wave * PI * 1024; // its bytes of LDS, from lds on
-    uint64_t lanes = ~0ull;
-    auto fetch_piece = [&](int p) { // of 2 PI
-        if (p < PI) async_run(k_at, k_from[p], lds_at + fetch_to + p * 1024, lanes);
-        else async_run(v_at, v_from[p - PI], lds_at + fetch_to + kTile + (p - PI) * 1024, lanes);
+    uint32_t fetch_to = is_v * kTile + copy0 * 1024; // its bytes of LDS, from lds on
+    int lanes = -1;
+    auto fetch_piece = [&](int p) { // of P; the second wave's may be one less
+        async_run(from_at, from[p], lds_at + fetch_to + p * 1024, kCopies % 2 && p == P - 1 && copy0 ? 0 : lanes);
     };
     auto next_fetch = [&](int t) { // what is fetched next is tile t
-        k_at = kb + (int64_t)t * KB * k_bytes;
-        v_at = vb + (int64_t)t * KB * v_bytes;
-        fetch_to = (t & 1) * 2 * kTile + wave * PI * 1024;
+        from_at = from_first + (int64_t)t * KB * row_bytes;
+        fetch_to = (t & 1) * 2 * kTile + is_v * kTile + copy0 * 1024;
         if (RUNS && nk - t * KB < KB) from_rows(nk - t * KB - 1); // the last one
     };
     auto fetch_loose = [&](int t) { // all of it through registers
         const int left = nk - t * KB - 1;
 #pragma unroll
-        for (int p = 0; p < PI; ++p) {
-            const int off = (wave * PI + p) * 1024 + lane * 16, row = min(off / kRow, left), place = off % kRow / 16;
-            const int kr = Lay::k_run(off / kRow, place), vr = Lay::v_run(off / kRow, place);
-            const T *kp = (const T *)(k_at + (int64_t)row * k_bytes), *vp = (const T *)(v_at + (int64_t)row * v_bytes);
-            uint32_t kw[4], vw[4];
+        for (int p = 0; p < P; ++p) {
+            const int at = (copy0 + p) * 1024 + lane * 16, run = Lay::run_of(is_v, at / kRow, at % kRow / 16);
+            const T *rp = (const T *)(from_at + (int64_t)min(at / kRow, left) * row_bytes);
+            if (kCopies % 2 && p == P - 1 && copy0) break;
+            uint32_t w[4];
             if (a.dim >= E) {
-                load_loose<T, E>(kp, kr * E, a.dim, kw);
-                load_loose<T, E>(vp, vr * E, a.dim, vw);
+                load_loose<T, E>(rp, run * E, a.dim, w);
             } else {
-                const u32x4 x = load_edge<T>(kp + kr * E, a.dim - kr * E), y = load_edge<T>(vp + vr * E, a.dim - vr * E);
+                const u32x4 x = load_edge<T>(rp + run * E, a.dim - run * E);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    kw[w] = x[w];
-                    vw[w] = y[w];
-                }
+                for (int i = 0; i < 4; ++i) w[i] = x[i];
             }
-            *reinterpret_cast<u32x4 *>(lds + fetch_to + p * 1024 + lane * 16) = (u32x4){kw[0], kw[1], kw[2], kw[3]};
-            *reinterpret_cast<u32x4 *>(lds + fetch_to + kTile + p * 1024 + lane * 16) = (u32x4){vw[0], vw[1], vw[2], vw[3]};
+            *reinterpret_cast<u32x4 *>(lds + fetch_to + p * 1024 + lane * 16) = (u32x4){w[0], w[1], w[2], w[3]};
         }
     };
     if (tiles > 0) {
         if constexpr (RUNS) {
 #pragma unroll
-            for (int p = 0; p < 2 * PI; ++p) fetch_piece(p);
+            for (int p = 0; p < P; ++p) fetch_piece(p);
         } else {
             fetch_loose(0);
         }
@@ -266,11 +305,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
     // 32 heads of 128: 89.6 us, straight to registers 91.1; heads of 64 gain nothing, 155 and 151 at 1000 rows)
     constexpr bool kStageQ = RUNS && DP > 64 && kRows * kRow <= 2 * kTile;
     if constexpr (kStageQ) {
-        constexpr int PQ = 32 * kRow / 1024;
+        constexpr int PQ = R * kRow / 1024;
         const uint32_t to = lds_at + 2 * kTile + wave * PQ * 1024;
 #pragma unroll
         for (int p = 0; p < PQ; ++p) {
-            const int off = p * 1024 + lane * 16, r = wave * 32 + off / kRow, run = min(Lay::k_run(r, off % kRow / 16), a.dim / E - 1);
+            const int off = p * 1024 + lane * 16, r = wave * R + off / kRow, run = min(Lay::k_run(r, off % kRow / 16), a.dim / E - 1);
             async_run((const char *)q_first, row_at(min(row0 + r, rows - 1), a.q_stride) * (uint32_t)sizeof(T) + (uint32_t)run * 16u, to + p * 1024);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -281,10 +320,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         const T *qp = q_first + row_at(my_row, a.q_stride);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int d0 = (2 * c + h) * E;
+            const int d0 = (G * c + h) * E;
             if constexpr (kStageQ)
                 q[c] = d0 >= a.dim ? (u32x4){0, 0, 0, 0}
-                                   : *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * 32 + n) * kRow + Lay::k_run(n, 2 * c + h) * 16);
+                                   : *reinterpret_cast<const u32x4 *>(lds + 2 * kTile + (wave * R + n) * kRow + Lay::k_run(n, G * c + h) * 16);
             else if constexpr (RUNS) q[c] = d0 < a.dim ? *reinterpret_cast<const u32x4 *>(qp + d0) : (u32x4){0, 0, 0, 0};
             else q[c] = load_edge<T>(qp + d0, a.dim - d0);
 #pragma unroll
@@ -292,26 +331,29 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         }
     }
 
-    // where a lane reads: K's row n (+ 32 a block), piece c; V's rows 4h + (lane % 16) / 4 (+ 8, + 16 cc, + 32 b), columns of block db
-    // (the swap of runs is among the first ones; the others follow at the same distances)
-    constexpr int NK = Lay::kPow2 / 2, NV = sizeof(T) == 2 ? Lay::kBlockPow2 : (DP % 64 == 0 ? 2 : 1);
+    // where a lane reads: K's row n (+ R a block), piece c; V's rows 4h + (lane % 16) / 4 (+ 8, + 16 cc, + 32 b), columns of block db
+    // (the swap of runs is among the first ones; the others follow at the same distances), or in fp32 rows 4h + r (+ 16 b)
+    constexpr int NK = Lay::kPow2 / G, NV = sizeof(T) == 2 ? Lay::kBlockPow2 : 1;
     int k_off[NK], v_off[NV];
 #pragma unroll
-    for (int c = 0; c < NK; ++c) k_off[c] = n * kRow + Lay::k_run(n, 2 * c + h) * 16;
+    for (int c = 0; c < NK; ++c) k_off[c] = n * kRow + Lay::k_run(n, G * c + h) * 16;
 #pragma unroll
     for (int d = 0; d < NV; ++d) {
-        if constexpr (sizeof(T) == 2) {
-            const int row = 4 * h + (lane & 15) / 4, run = 4 * d + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
-            v_off[d] = row * kRow + Lay::v_run(row, run) * 16 + (lane & 1) * 8;
-        } else {
-            const int row = 4 * h, run = 8 * d + n / 4;
-            v_off[d] = row * kRow + Lay::v_run(row, run) * 16 + (n & 3) * 4;
-        }
+        const int row = 4 * h + (lane & 15) / 4, run = 4 * d + 2 * ((lane >> 4) & 1) + (lane & 3) / 2;
+        v_off[d] = sizeof(T) == 2 ? row * kRow + Lay::v_run(row, run) * 16 + (lane & 1) * 8 : 4 * h * kRow;
     }
 
-    f32x16 o[DB] = {};
-    float m = -INFINITY, l = 0.f; // base 2; l: this lane's half of the keys
+    Acc o[DB] = {};
+    float m = -INFINITY, l = 0.f; // base 2; l: this lane's share of the keys
     for (int t = 0; t < tiles; ++t) {
+        // fp32: workgroups that are all on the device at once end together if those behind go first; the oldest ones would (8 x 577 rows, 16
+        // heads of 80: 127.5 us, 133 without). Where others follow, they fill that gap themselves (8 x 2000 of 64: 672 with this, 628 without).
+        if (sizeof(T) == 4 && a.at_once) {
+            if (t == 0) __builtin_amdgcn_s_setprio(3);
+            else if (t == tiles / 4) __builtin_amdgcn_s_setprio(2);
+            else if (t == tiles / 2) __builtin_amdgcn_s_setprio(1);
+            else if (t == tiles * 3 / 4) __builtin_amdgcn_s_setprio(0);
+        }
         all_ready(); // tile t is there, and every wave is done with tile t - 1
         if (t + 1 < tiles) {
             next_fetch(t + 1);
@@ -323,40 +365,55 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
         if (first >= wave_max) {
             if constexpr (RUNS) {
 #pragma unroll
-                for (int p = 0; p < 2 * PI; ++p) fetch_piece(p);
+                for (int p = 0; p < P; ++p) fetch_piece(p);
             }
             continue;
         }
         const char *kt = lds + (t & 1) * 2 * kTile, *vt = kt + kTile;
 
-        f32x16 s[B] = {};
+        Acc s[B] = {};
         // pieces of K's rows are read kAhead products before they are needed
-        constexpr int kAhead = NC < 8 ? NC : 8;
-        auto read_k = [&](int j) { return *reinterpret_cast<const u32x4 *>(kt + k_off[j % NC % NK] + j % NC / NK * NK * 32 + j / NC * 32 * kRow); };
+        constexpr int kMostAhead = sizeof(T) == 2 ? 8 : 4, kAhead = NC < kMostAhead ? NC : kMostAhead;
+        auto read_k = [&](int j) { return *reinterpret_cast<const u32x4 *>(kt + k_off[j % NC % NK] + j % NC / NK * NK * 16 * G + j / NC * R * kRow); };
         // The next tile's copies go out one by one between the products: a copy waits at its issue for those of the other waves to
         // pass (64 bytes a cycle for all of the CU), 600 cycles for the eight of a wave in a row.
-        constexpr int kEvery = B * NC / (2 * PI); // products a copy
-        static_assert(B * NC % (2 * PI) == 0, "");
         u32x4 kf[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) kf[j] = read_k(j);
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
         for (int j = 0; j < B * NC; ++j) {
-            s[j / NC] = mfma32(kf[j % kAhead], q[j % NC], s[j / NC], T());
-            if (RUNS && j % kEvery == kEvery - 1) fetch_piece(j / kEvery);
+            s[j / NC] = mfma_piece(kf[j % kAhead], q[j % NC], s[j / NC], T());
+            if constexpr (RUNS) {
+                const int p = ((j + 1) * P - 1) / (B * NC); // the copy whose turn comes within product j's
+                if (j == (p + 1) * B * NC / P - 1) fetch_piece(p);
+            }
             __builtin_amdgcn_sched_group_barrier(0x8, sizeof(T) == 2 ? 1 : 4, 0);
             if (j + kAhead < B * NC) {
                 kf[j % kAhead] = read_k(j + kAhead);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         }
+        settle<T>(s);
         if (first + KB > wave_min) {
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (first + 32 * b + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[b][r] = -INFINITY;
+                for (int r = 0; r < 4 * A4; ++r)
+                    if (first + R * b + 4 * G * (r / 4) + 4 * h + r % 4 >= limit) s[b][r] = -INFINITY;
+        }
+        float vf[2][DB]; // fp32: V's row r of each four, read while the row before the last one is multiplied
+        auto read_v = [&](int b, int r) {
+            const char *row = vt + v_off[0] + (R * b + r) * kRow;
+#pragma unroll
+            for (int d = 0; d < kFull; d += 4) *reinterpret_cast<f32x4 *>(&vf[r % 2][d]) = *reinterpret_cast<const f32x4 *>(row + d * 64 + n * 16);
+            if constexpr (kRest == 2) *reinterpret_cast<f32x2 *>(&vf[r % 2][kFull]) = *reinterpret_cast<const f32x2 *>(row + kFull * 64 + n * 8);
+            if constexpr (kRest == 1) vf[r % 2][kFull] = *reinterpret_cast<const float *>(row + kFull * 64 + n * 4);
+        };
+        if constexpr (sizeof(T) == 4) {
+            read_v(0, 0);
+            read_v(0, 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
         float tops[4]; // shorter chains
 #pragma unroll
@@ -364,9 +421,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
 #pragma unroll
         for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int r = b ? 0 : 4; r < 16; ++r) tops[r % 4] = fmaxf(tops[r % 4], s[b][r]);
+            for (int r = b ? 0 : 4; r < 4 * A4; ++r) tops[r % 4] = fmaxf(tops[r % 4], s[b][r]);
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        top = fmaxf(top, other_half(top)) * a.scale2;
+        top = across<R>(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale2;
         if (__any(top > m + kLag)) {
             const float to = fmaxf(m, top), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
             m = to;
@@ -378,7 +435,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
 #pragma unroll
         for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4 * A4; ++r) {
                 s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], a.scale2, -base));
                 l += s[b][r];
             }
@@ -400,32 +457,42 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
                         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)vp);
                         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Piece)(vp + 8 * kRow));
                         const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
-                        o[d] = mfma32((u32x4){wl[0], wl[1], wh[0], wh[1]}, p, o[d], T());
+                        o[d] = mfma_piece((u32x4){wl[0], wl[1], wh[0], wh[1]}, p, o[d], T());
                     }
                 }
             } else {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
+                for (int r = 0; r < 4; ++r) {
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const float vf = *reinterpret_cast<const float *>(vt + v_off[d % NV] + d / NV * NV * 128 + (32 * b + 8 * (r / 4) + r % 4) * kRow);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[b][r], o[d], 0, 0, 0);
-                    }
+                    for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[r % 2][d], s[b][r], o[d], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (r < 2) read_v(b, r + 2);
+                    else if (b + 1 < B) read_v(b + 1, r - 2);
+                }
             }
         }
     }
 
-    const float sum = l + other_half(l);
+    // four elements of o next to each other, and where: k of DB A4
+    auto four = [&](int k) {
+        if constexpr (sizeof(T) == 2) {
+            return (f32x4){o[k / A4][k % A4 * 4], o[k / A4][k % A4 * 4 + 1], o[k / A4][k % A4 * 4 + 2], o[k / A4][k % A4 * 4 + 3]};
+        } else {
+            const int W = k < kFull ? 4 : kRest, d = k < kFull ? k / 4 * 4 : kFull, t = (k - d) * 4;
+            return (f32x4){o[d + t % W][t / W], o[d + (t + 1) % W][(t + 1) / W], o[d + (t + 2) % W][(t + 2) / W], o[d + (t + 3) % W][(t + 3) / W]};
+        }
+    };
+    auto four_at = [&](int k) {
+        if constexpr (sizeof(T) == 2) return R * (k / A4) + 4 * G * (k % A4) + 4 * h;
+        else return k < kFull ? k / 4 * 64 + 16 * h + k % 4 * 4 : kFull * 16 + 4 * kRest * h + (k - kFull) * 4;
+    };
+    const float sum = across<R>(l, [](float x, float y) { return x + y; });
     const bool mine = wrow + n < rows;
     if (a.splits > 1) { // as they are, for prompt_join_kernel
-        const int64_t part = ((int64_t)(item * a.kv_heads + kvh) * a.splits + sp) * kRows + wave * 32 + n;
+        const int64_t part = ((int64_t)(item * a.kv_heads + kvh) * a.splits + sp) * kRows + wave * R + n;
         if (mine) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4)
-                    *reinterpret_cast<f32x4 *>(a.part_o + part * DP + 32 * d + 8 * r4 + 4 * h) =
-                        (f32x4){o[d][4 * r4], o[d][4 * r4 + 1], o[d][4 * r4 + 2], o[d][4 * r4 + 3]};
+            for (int k = 0; k < DB * A4; ++k) *reinterpret_cast<f32x4 *>(a.part_o + part * DP + four_at(k)) = four(k);
             if (h == 0) *reinterpret_cast<float2 *>(a.part_ml + part * 2) = make_float2(m - kUp, sum);
         }
         return;
@@ -433,29 +500,28 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
     __syncthreads(); // the tiles' place takes o's
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int k = 0; k < DB * A4; ++k) {
+        const int at4 = four_at(k);
+        const f32x4 w = four(k);
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 v;
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const int at4 = 32 * d + 8 * r4 + 4 * h;
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            T4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(o[d][4 * r4 + e] * inv);
-            *reinterpret_cast<T4 *>(lds + (wave * 32 + n) * kRow + Lay::k_run(n, at4 / E) * 16 + at4 % E * (int)sizeof(T)) = v;
-        }
+        for (int e = 0; e < 4; ++e) v[e] = (T)(w[e] * inv);
+        *reinterpret_cast<T4 *>(lds + (wave * R + n) * kRow + Lay::k_run(n, at4 / E) * 16 + at4 % E * (int)sizeof(T)) = v;
+    }
     if (a.lse && h == 0 && mine) a.lse[(int64_t)(q0 + token) * a.heads + head] = sum == 0.f ? -INFINITY : (m - kUp + __log2f(sum)) * kLn2;
     // a wave's rows, whole lines at a time
     T *const o_first = (T *)a.o + (int64_t)(q0 + tok0) * a.o_stride + (int64_t)kvh * a.group * a.dim;
     if (a.o_runs) {
-        constexpr int PO = 32 * kRow / 1024;
+        constexpr int PO = R * kRow / 1024;
 #pragma unroll
         for (int p = 0; p < PO; ++p) {
-            const int off = p * 1024 + lane * 16, r = wave * 32 + off / kRow, run = off % kRow / 16;
+            const int off = p * 1024 + lane * 16, r = wave * R + off / kRow, run = off % kRow / 16;
             const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + r * kRow + Lay::k_run(r, run) * 16);
             if (row0 + r < rows && run * E < a.dim) *reinterpret_cast<u32x4 *>(o_first + (row_at(row0 + r, a.o_stride) + run * E)) = v;
         }
     } else {
-        for (int r = wave * 32; r < (wave + 1) * 32 && row0 + r < rows; ++r) {
+        for (int r = wave * R; r < (wave + 1) * R && row0 + r < rows; ++r) {
             T *op = o_first + row_at(row0 + r, a.o_stride);
             for (int d = lane; d < a.dim; d += 64)
                 op[d] = *reinterpret_cast<const T *>(lds + r * kRow + Lay::k_run(r, d / E) * 16 + d % E * (int)sizeof(T));
@@ -467,8 +533,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? (sizeof(T) == 2 && DP == 96 && RUN
 template <class T>
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, int part_row) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int kBlocks = kRows / 4; // of an (item, kv head)
-    const int block = (int)blockIdx.x / kBlocks, r = (int)blockIdx.x % kBlocks * 4 + wave, kvh = block % a.kv_heads;
+    constexpr int kRows = ::spinn::kRows<T>, kFours = kRows / 4; // of an (item, kv head)
+    const int block = (int)blockIdx.x / kFours, r = (int)blockIdx.x % kFours * 4 + wave, kvh = block % a.kv_heads;
     const Place at = find_place(a, block / a.kv_heads, kRows);
     const int row = at.tile * kRows + r;
     if (at.tile < 0 || row >= at.nq * a.group) return;
@@ -500,15 +566,17 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, int part
 
 // How the rows and keys are cut.
 struct Cut {
-    int64_t items; // tiles of kRows rows at most
+    int rows;      // of a tile
+    int64_t items; // tiles at most
     int pad;       // head_dim padded
     int splits;
 };
 Cut cut(const SpinnHipPromptAttentionDesc *d) {
     Cut c;
     const int64_t group = d->heads / d->kv_heads;
-    c.items = (int64_t)d->q_rows * group / kRows + std::min(d->seqs, d->q_rows);
-    c.pad = d->head_dim <= 64 ? 64 : (d->head_dim <= 96 ? 96 : (d->head_dim <= 128 ? 128 : 256));
+    c.rows = dtype_bytes(d->dtype) == 4 ? kRows<float> : kRows<__bf16>;
+    c.items = (int64_t)d->q_rows * group / c.rows + std::min(d->seqs, d->q_rows);
+    c.pad = d->head_dim <= 64 ? 64 : (d->head_dim <= 80 && c.rows == kRows<float> ? 80 : (d->head_dim <= 96 ? 96 : (d->head_dim <= 128 ? 128 : 256)));
     // Keys are split where workgroups of whole rows leave most of the device idle: into as many parts as two workgroups a CU take, of
     // 8 tiles at least, up to the join's 64. The parts' sums and the second launch cost some 10 us, so that is for 16 tiles less at least
     // (32 heads on 8 of 128, bf16: 16 rows over 4000 keys 68 -> 19 us, over 64000 1014 -> 66, 100 over 4000 69 -> 27; 1000 over 1000,
@@ -520,12 +588,13 @@ Cut cut(const SpinnHipPromptAttentionDesc *d) {
 }
 
 template <class T, int DP, int KB>
-int launch(const PromptArgs &a, const Cut &c, bool runs, hipStream_t st) {
+int launch(PromptArgs &a, const Cut &c, bool runs, hipStream_t st) {
     const int64_t grid = c.items * a.kv_heads * c.splits;
     if (!launch_fits(grid, 256)) return SPINN_HIP_EUNSUPPORTED;
+    a.at_once = grid <= (runs ? kBlocks<T, DP, true> : kBlocks<T, DP, false>) * device_cu_count();
     if (runs) prompt_kernel<T, DP, KB, true><<<(unsigned)grid, 256, 0, st>>>(a);
     else prompt_kernel<T, DP, KB, false><<<(unsigned)grid, 256, 0, st>>>(a);
-    if (c.splits > 1) prompt_join_kernel<T><<<(unsigned)(c.items * a.kv_heads * (kRows / 4)), 256, 0, st>>>(a, DP);
+    if (c.splits > 1) prompt_join_kernel<T><<<(unsigned)(c.items * a.kv_heads * (c.rows / 4)), 256, 0, st>>>(a, DP);
     return check_launch();
 }
 
@@ -533,7 +602,7 @@ int launch(const PromptArgs &a, const Cut &c, bool runs, hipStream_t st) {
 
 size_t prompt_attention_workspace_bytes(const SpinnHipPromptAttentionDesc *d) {
     const Cut c = cut(d);
-    return c.splits > 1 ? (size_t)(c.items * d->kv_heads * c.splits) * kRows * (c.pad + 2) * 4 : 0;
+    return c.splits > 1 ? (size_t)(c.items * d->kv_heads * c.splits) * c.rows * (c.pad + 2) * 4 : 0;
 }
 
 int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const void *k, const void *v, const int32_t *starts,
@@ -563,7 +632,7 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.causal = d->causal;
     a.splits = c.splits;
     a.part_o = (float *)ws;
-    a.part_ml = (float *)ws + c.items * d->kv_heads * c.splits * kRows * c.pad;
+    a.part_ml = (float *)ws + c.items * d->kv_heads * c.splits * c.rows * c.pad;
     if (a.group > 1) { // exact for rows under 2^31
         while ((2u << a.group_shift) < (uint32_t)a.group) ++a.group_shift;
         a.group_mul = (uint32_t)(((1ull << (32 + a.group_shift)) + a.group - 1) / a.group);
@@ -575,11 +644,14 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.o_runs = a.dim % per == 0 && d->o_stride % per == 0 && aligned16(o);
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
-        constexpr int K = sizeof(T) == 2 ? 64 : 32;
+        constexpr int K = sizeof(T) == 2 ? 64 : 16;
         if (c.pad == 64) return launch<T, 64, K>(a, c, runs, st);
+        if constexpr (sizeof(T) == 4) {
+            if (c.pad == 80) return launch<T, 80, K>(a, c, runs, st);
+        }
         if (c.pad == 96) return launch<T, 96, K>(a, c, runs, st);
         if (c.pad == 128) return launch<T, 128, K>(a, c, runs, st);
-        return launch<T, 256, 32>(a, c, runs, st);
+        return launch<T, 256, sizeof(T) == 2 ? 32 : 16>(a, c, runs, st);
     });
 }
 
