@@ -58,8 +58,8 @@ struct Place {
     int q0, nq, k0, nk;
 };
 __device__ __forceinline__ int clamped(const int32_t *starts, int i, int rows) { return min(max(starts[i], 0), rows); }
-// Sequence by sequence, so that what runs at a time shares keys in the L2 (24 sequences of 37 to 2000 rows: 406 us; all their last
-// tiles first, then the ones before them, 421), each from its end, where a causal mask leaves the most keys. Up to 64, one a
+// Sequence by sequence, so that what runs at a time shares keys in the L2 (24 sequences of 37 to 2000 rows, in an earlier form: 406 us; all their
+// last tiles first, then the ones before them, 421), each from its end, where a causal mask leaves the most keys. Up to 64, one a
 // lane, the longest first, so that what starts last is short.
 __device__ __forceinline__ Place find_place(const PromptArgs &a, int item, int rows) {
     const int lane = threadIdx.x & 63;
@@ -173,7 +173,7 @@ __device__ __forceinline__ float across(float v, F f) {
 }
 
 // 16 bytes a lane from base + off to byte `to` + 16 lane of LDS; all_ready() waits for it. In assembly, since the compiler would wait for all
-// of these before every transposing read of LDS that follows, whatever it reads (16000 rows: 2020 -> 1916 us).
+// of these before every transposing read of LDS that follows, whatever it reads (16000 rows, before other steps: 2020 -> 1916 us).
 // lanes: -1 all of those that are here, 0 none, without a branch.
 __device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32_t to, int lanes = -1) {
     uint64_t here;
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
     };
     const T *const q_first = (const T *)a.q + (int64_t)(q0 + tok0) * a.q_stride + (int64_t)kvh * a.group * a.dim;
     // Q's rows come through the odd tiles' place where they fit, whole lines at a time, a wave's own ones (24 sequences of 500 rows,
-    // 32 heads of 128: 89.6 us, straight to registers 91.1; heads of 64 gain nothing, 155 and 151 at 1000 rows)
+    // 32 heads on 8 of 128: 89.6 us, straight to registers 91.1; heads of 64 gain nothing, 155 and 151 at 1000 rows; fp32's do not fit)
     constexpr bool kStageQ = RUNS && DP > 64 && kRows * kRow <= 2 * kTile;
     if constexpr (kStageQ) {
         constexpr int PQ = R * kRow / 1024;
@@ -406,8 +406,9 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
         auto read_v = [&](int b, int r) {
             const char *row = vt + v_off[0] + (R * b + r) * kRow;
 #pragma unroll
-            for (int d = 0; d < kFull; d += 4) *reinterpret_cast<f32x4 *>(&vf[r % 2][d]) = *reinterpret_cast<const f32x4 *>(row + d * 64 + n * 16);
-            if constexpr (kRest == 2) *reinterpret_cast<f32x2 *>(&vf[r % 2][kFull]) = *reinterpret_cast<const f32x2 *>(row + kFull * 64 + n * 8);
+            for (int d = 0; d < kFull; ++d) vf[r % 2][d] = (*reinterpret_cast<const f32x4 *>(row + d / 4 * 256 + n * 16))[d % 4];
+#pragma unroll
+            for (int d = kFull; kRest == 2 && d < DB; ++d) vf[r % 2][d] = (*reinterpret_cast<const f32x2 *>(row + kFull * 64 + n * 8))[d % 2];
             if constexpr (kRest == 1) vf[r % 2][kFull] = *reinterpret_cast<const float *>(row + kFull * 64 + n * 4);
         };
         if constexpr (sizeof(T) == 4) {
@@ -555,7 +556,6 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, int part
     if (d0 >= a.dim) return;
     const float *from = a.part_o + part * part_row + d0;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
     for (int s = 0; s < a.splits; ++s)
         v += *reinterpret_cast<const f32x4 *>(from + (int64_t)s * kRows * part_row) *
              __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
