@@ -76,28 +76,34 @@ __device__ __forceinline__ u32x4 load_edge(const T *p, int left) {
 // row's end starts early enough to stay inside, and a shift (17 sequences of 12724 to 28547 slots, 8 heads of 33,
 // bf16: 266 us, element by element 756).
 template <class T, int N>
-__device__ __forceinline__ void load_loose(const T *row, int d0, int dim, uint32_t (&to)[N * sizeof(T) / 4]) {
-    constexpr int W = N * sizeof(T) / 4;
+struct LooseRun {
+    static constexpr int W = N * sizeof(T) / 4;
     typedef uint32_t Words __attribute__((ext_vector_type(W)));
     typedef Words Loose __attribute__((aligned(sizeof(T))));
-    const int at = min(d0, dim - N), skip = (d0 - at) * (int)sizeof(T) * 8; // bits of elements before d0
-    const Words w = *reinterpret_cast<const Loose *>(row + at);
-    if constexpr (W == 2) {
-        const uint64_t v = __builtin_bit_cast(uint64_t, w);
-        const uint64_t r = skip < 64 ? v >> skip : 0ull;
-        to[0] = (uint32_t)r;
-        to[1] = (uint32_t)(r >> 32);
-    } else {
-        static_assert(W == 4, "");
-        const uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
-        const int s = skip & 63;
-        const uint64_t both = s ? lo >> s | hi << (64 - s) : lo, top = hi >> s;
-        const uint64_t r0 = skip < 64 ? both : (skip < 128 ? top : 0ull), r1 = skip < 64 ? top : 0ull;
-        to[0] = (uint32_t)r0;
-        to[1] = (uint32_t)(r0 >> 32);
-        to[2] = (uint32_t)r1;
-        to[3] = (uint32_t)(r1 >> 32);
+    __device__ __forceinline__ static Words load(const T *row, int d0, int dim) { return *reinterpret_cast<const Loose *>(row + min(d0, dim - N)); }
+    __device__ __forceinline__ static void shift(const Words w, int d0, int dim, uint32_t (&to)[W]) {
+        const int skip = (d0 - min(d0, dim - N)) * (int)sizeof(T) * 8; // bits of elements before d0
+        if constexpr (W == 2) {
+            const uint64_t v = __builtin_bit_cast(uint64_t, w);
+            const uint64_t r = skip < 64 ? v >> skip : 0ull;
+            to[0] = (uint32_t)r;
+            to[1] = (uint32_t)(r >> 32);
+        } else {
+            static_assert(W == 4, "");
+            const uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+            const int s = skip & 63;
+            const uint64_t both = s ? lo >> s | hi << (64 - s) : lo, top = hi >> s;
+            const uint64_t r0 = skip < 64 ? both : (skip < 128 ? top : 0ull), r1 = skip < 64 ? top : 0ull;
+            to[0] = (uint32_t)r0;
+            to[1] = (uint32_t)(r0 >> 32);
+            to[2] = (uint32_t)r1;
+            to[3] = (uint32_t)(r1 >> 32);
+        }
     }
+};
+template <class T, int N>
+__device__ __forceinline__ void load_loose(const T *row, int d0, int dim, uint32_t (&to)[N * sizeof(T) / 4]) {
+    LooseRun<T, N>::shift(LooseRun<T, N>::load(row, d0, dim), d0, dim, to);
 }
 
 // How rows are read.

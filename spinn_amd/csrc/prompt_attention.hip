@@ -188,7 +188,7 @@ __device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) l
 
 // Workgroups on a CU, as registers and LDS allow.
 template <class T, int DP, bool RUNS>
-constexpr int kBlocks = sizeof(T) == 4 ? (DP == 64 ? 5 : DP <= 96 ? 4 + RUNS : DP == 128 ? 3 + RUNS : 2) : DP <= 128 ? (DP == 96 && RUNS ? 3 : 2) : 1;
+constexpr int kBlocks = sizeof(T) == 4 ? (DP <= 64 ? 4 + RUNS : DP <= 96 ? 4 + RUNS : DP == 128 ? 3 + RUNS : 2) : DP <= 128 ? (DP == 96 && RUNS ? 3 : 2) : 1;
 
 // What a matrix product has just left in s may be read. The compiler counts the wait that is due along one way into a block only
 // (16 x 16 x 4 fp32: 10 instructions by the masked way, 1 by the other, where it put none), so it is written out here.
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
     uint32_t from[P];
     auto from_rows = [&](int left) { // of a tile whose row `left` is the last that there is: rows behind it are copies of it
         int here = lane;
-        asm volatile("" : "+v"(here)); // so that nothing for the last tile is kept in registers throughout
+        asm volatile("" : "+v"(here)); // so that nothing of this is kept in registers throughout
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int at = (copy0 + p) * 1024 + here * 16, run = min(Lay::run_of(is_v, at / kRow, at % kRow / 16), a.dim / E - 1);
@@ -268,21 +268,33 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
         fetch_to = (t & 1) * 2 * kTile + is_v * kTile + copy0 * 1024;
         if (RUNS && nk - t * KB < KB) from_rows(nk - t * KB - 1); // the last one
     };
-    auto fetch_loose = [&](int t) { // all of it through registers
+    // The same through registers. 16-bit types: they go to LDS when the tile before is done (24 x 500 rows, 32 heads on 8 of 99, bf16: 237 us, at
+    // once 287; 2 x 1000, 8 heads of 255: 119 and 176); fp32, with more waves to wait for: at once (2 x 1000, 8 heads of 255: 222, late 298;
+    // smaller ones within 4 %).
+    constexpr bool kLate = sizeof(T) == 2;
+    typedef LooseRun<T, E> Run;
+    u32x4 kept[RUNS ? 1 : P];
+    auto load_loose_tile = [&](int t) {
         const int left = nk - t * KB - 1;
+        int here = lane;
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(here)); // as in from_rows; fp32 has the registers
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int at = (copy0 + p) * 1024 + lane * 16, run = Lay::run_of(is_v, at / kRow, at % kRow / 16);
-            const T *rp = (const T *)(from_at + (int64_t)min(at / kRow, left) * row_bytes);
+            const int at = (copy0 + p) * 1024 + here * 16, d0 = Lay::run_of(is_v, at / kRow, at % kRow / 16) * E;
             if (kCopies % 2 && p == P - 1 && copy0) break;
-            uint32_t w[4];
-            if (a.dim >= E) {
-                load_loose<T, E>(rp, run * E, a.dim, w);
-            } else {
-                const u32x4 x = load_edge<T>(rp + run * E, a.dim - run * E);
+            const T *rp = (const T *)(from_at + (int64_t)min(at / kRow, left) * row_bytes);
+            kept[p] = a.dim >= E ? Run::load(rp, d0, a.dim) : load_edge<T>(rp + d0, a.dim - d0);
+        }
+    };
+    auto store_loose_tile = [&]() {
+        int here = lane;
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(here));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = x[i];
-            }
+        for (int p = 0; p < P; ++p) {
+            const int at = (copy0 + p) * 1024 + here * 16, d0 = Lay::run_of(is_v, at / kRow, at % kRow / 16) * E;
+            if (kCopies % 2 && p == P - 1 && copy0) break;
+            uint32_t w[4] = {kept[p][0], kept[p][1], kept[p][2], kept[p][3]};
+            if (a.dim >= E) Run::shift(kept[p], d0, a.dim, w);
             *reinterpret_cast<u32x4 *>(lds + fetch_to + p * 1024 + lane * 16) = (u32x4){w[0], w[1], w[2], w[3]};
         }
     };
@@ -291,7 +303,8 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
 #pragma unroll
             for (int p = 0; p < P; ++p) fetch_piece(p);
         } else {
-            fetch_loose(0);
+            load_loose_tile(0);
+            store_loose_tile();
         }
     }
     // where a row of the tile lies in q and o, in elements from the first one's token and the kv head's first query head
@@ -357,7 +370,10 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
         all_ready(); // tile t is there, and every wave is done with tile t - 1
         if (t + 1 < tiles) {
             next_fetch(t + 1);
-            if constexpr (!RUNS) fetch_loose(t + 1);
+            if constexpr (!RUNS) {
+                load_loose_tile(t + 1);
+                if constexpr (!kLate) store_loose_tile();
+            }
         } else {
             lanes = 0;
         }
@@ -366,6 +382,8 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
             if constexpr (RUNS) {
 #pragma unroll
                 for (int p = 0; p < P; ++p) fetch_piece(p);
+            } else if constexpr (kLate) {
+                if (lanes) store_loose_tile();
             }
             continue;
         }
@@ -472,6 +490,9 @@ __global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(Pro
                 }
             }
         }
+        if constexpr (!RUNS && kLate) {
+            if (lanes) store_loose_tile();
+        }
     }
 
     // four elements of o next to each other, and where: k of DB A4
@@ -576,7 +597,9 @@ Cut cut(const SpinnHipPromptAttentionDesc *d) {
     const int64_t group = d->heads / d->kv_heads;
     c.rows = dtype_bytes(d->dtype) == 4 ? kRows<float> : kRows<__bf16>;
     c.items = (int64_t)d->q_rows * group / c.rows + std::min(d->seqs, d->q_rows);
-    c.pad = d->head_dim <= 64 ? 64 : (d->head_dim <= 80 && c.rows == kRows<float> ? 80 : (d->head_dim <= 96 ? 96 : (d->head_dim <= 128 ? 128 : 256)));
+    // Each of these has its kernel: 24 x 500 rows, 32 heads on 8 of 32, bf16: 43 us, with 64 columns 52; 8 x 1000, 16 heads of 32, fp32: 137 and 206.
+    for (const int pad : {256, 128, 96, 80, 64, 32})
+        if (d->head_dim <= pad && (pad != 80 || c.rows == kRows<float>)) c.pad = pad;
     // Keys are split where workgroups of whole rows leave most of the device idle: into as many parts as two workgroups a CU take, of
     // 8 tiles at least, up to the join's 64. The parts' sums and the second launch cost some 10 us, so that is for 16 tiles less at least
     // (32 heads on 8 of 128, bf16: 16 rows over 4000 keys 68 -> 19 us, over 64000 1014 -> 66, 100 over 4000 69 -> 27; 1000 over 1000,
@@ -645,6 +668,7 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     return with_dtype(d->dtype, [&](auto t) {
         typedef decltype(t) T;
         constexpr int K = sizeof(T) == 2 ? 64 : 16;
+        if (c.pad == 32) return launch<T, 32, K>(a, c, runs, st);
         if (c.pad == 64) return launch<T, 64, K>(a, c, runs, st);
         if constexpr (sizeof(T) == 4) {
             if (c.pad == 80) return launch<T, 80, K>(a, c, runs, st);
