@@ -16,6 +16,7 @@
 // 618 (670); 2 x 1000, 8 heads on 2 of 256: 141 (277).
 #include "decode.h"
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 namespace spinn {
@@ -636,8 +637,8 @@ int prompt_attention(const SpinnHipPromptAttentionDesc *d, const void *q, const 
     a.k_stride = d->k_stride;
     a.v_stride = d->v_stride;
     a.o_stride = d->o_stride;
-    // a scale of (nearly) nothing still multiplies the -inf of hidden keys
-    a.scale2 = std::max(std::fabs(d->scale) * kLog2e, 1e-37f);
+    // A scale of nothing still multiplies the -inf of hidden keys: the least number takes its place, with which no score passes 2^-21.
+    a.scale2 = std::max(std::fabs(d->scale) * kLog2e, std::numeric_limits<float>::denorm_min());
     const int e = dtype_bytes(d->dtype);
     a.flip = d->scale < 0 ? (e == 2 ? 0x80008000u : 0x80000000u) : 0u;
     a.seqs = d->seqs;
