@@ -523,7 +523,7 @@ typedef struct {
     int32_t head_dim;        /* 1..SPINN_HIP_KV_MAX_DIM */
     int32_t causal;
     int32_t q_rows, kv_rows; /* rows of q, o and lse, and of k and v; the split and the workspace go by them */
-    float scale;             /* finite */
+    float scale;             /* within +-2^127 */
     int32_t reserved;        /* 0 */
     int64_t q_stride, k_stride, v_stride, o_stride; /* up to 2^24 */
 } SpinnHipPromptAttentionDesc;

@@ -38,7 +38,8 @@ bool rope_ok(const SpinnHipRopeDesc *d) {
 bool prompt_ok(const SpinnHipPromptAttentionDesc *d) {
     if (!d || !dtype_bytes(d->dtype) || d->reserved != 0 || d->seqs < 0 || d->heads <= 0 || d->kv_heads <= 0) return false;
     if (d->heads % d->kv_heads || d->head_dim <= 0 || d->head_dim > SPINN_HIP_KV_MAX_DIM) return false;
-    if (d->causal < 0 || d->causal > 1 || d->q_rows < 0 || d->kv_rows < 0 || !std::isfinite(d->scale)) return false;
+    if (d->causal < 0 || d->causal > 1 || d->q_rows < 0 || d->kv_rows < 0) return false;
+    if (!(std::fabs(d->scale) <= 0x1p127f)) return false; // times log2 e it is still a number
     if (d->seqs > (1 << 24)) return false;
     // rows of (token, head) pairs and their tiles, and keys a tile behind the last, within 31 bits
     constexpr int64_t kMost = (int64_t)1 << 30;
