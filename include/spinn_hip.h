@@ -479,7 +479,8 @@ enum {
  * (i, i + rot_dim / 2), turns by the angle position[t] f_i:
  *   y_a = magnitude (cos x_a - sin x_b), y_b = magnitude (sin x_a + cos x_b);
  * the rest of a head is copied. Head h of token t is at x + t*x_stride + h*x_head_stride, y alike; y may be x itself (same strides),
- * else they overlap nowhere. Angles are exact to 2^-32 of a turn at any position (negative ones turn back).
+ * else they overlap nowhere. Angles are exact to 2^-32 of a turn at any position (negative ones
+ * turn back) for frequencies up to 2^30.
  * The frequencies are laid out once by spinn_hip_rope_table (which reads rot_dim, scaling, base, factor, low, high and
  * trained alone), 16-byte aligned, and read from `table` afterwards.
  */

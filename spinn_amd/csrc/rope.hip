@@ -2,8 +2,8 @@
 //
 // Memory bounds it: every element is read and written once. The sines and cosines of a token are the same in all of its heads,
 // so a workgroup computes those of its tokens once into LDS and then walks over the heads in 16-byte
-// runs. Angles: a frequency is kept as a fraction of a turn in 64-bit fixed point, whose product with the position, modulo
-// 2^64, is the angle without its whole turns, exactly: positions in the millions are as good as the first.
+// runs. Angles: a frequency is kept as a fraction of a turn in 64-bit fixed point, right to its last two units, whose product with the position,
+// modulo 2^64, is the angle without its whole turns, to 2^-32: positions in the thousands of millions are as good as the first.
 // 16384 x 40 heads of 128, bf16: 62 to 66 us, 5.1 to 5.4 TB/s; 5001 x 17 heads, 32 of 80, interleaved, fp32: 10.5 us, 5.2 TB/s; 32 x 20 heads of
 // 128: 6.8 us a call, a launch.
 #include "decode.h"
@@ -27,7 +27,7 @@ struct RopeArgs {
 
 // (sin, cos) of 2 pi p / 2^64: the nearest quarter turn and what is left of it, within 1/8 of a turn.
 // sin x = x + x^3 S(x^2) and cos x = 1 - x^2/2 + x^4 C(x^2), S and C fitted on [-pi/4, pi/4] with the least error of the
-// results (4e-9 relative and 1e-10).
+// results (5e-9 relative and 1e-10).
 __device__ __forceinline__ void sin_cos_turns(uint64_t p, float &s, float &c) {
     const uint32_t q = (uint32_t)((p + (1ull << 61)) >> 62);
     const int64_t r = (int64_t)(p - ((uint64_t)q << 62));
@@ -108,22 +108,81 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     }
 }
 
+// Numbers of 106 bits, hi + lo: a position of up to 2^31 multiplies what an angle's frequency is off by.
+struct Wide {
+    double hi, lo;
+};
+__device__ Wide normal(double a, double b) { // a + b, |a| >= |b|
+#pragma clang fp contract(off)
+    const double s = a + b;
+    return {s, b - (s - a)};
+}
+__device__ Wide sum(double a, double b) {
+#pragma clang fp contract(off)
+    const double s = a + b, t = s - a;
+    return {s, (a - (s - t)) + (b - t)};
+}
+__device__ Wide operator+(Wide a, Wide b) {
+#pragma clang fp contract(off)
+    const Wide s = sum(a.hi, b.hi), t = sum(a.lo, b.lo), u = normal(s.hi, s.lo + t.hi);
+    return normal(u.hi, u.lo + t.lo);
+}
+__device__ Wide operator-(Wide a) { return {-a.hi, -a.lo}; }
+__device__ Wide operator*(Wide a, Wide b) {
+#pragma clang fp contract(off)
+    const double p = a.hi * b.hi, e = fma(a.hi, b.hi, -p);
+    return normal(p, e + (a.hi * b.lo + a.lo * b.hi));
+}
+__device__ Wide operator/(Wide a, Wide b) { // three quotients of what is left
+#pragma clang fp contract(off)
+    const double q1 = a.hi / b.hi;
+    const Wide r1 = a + -(b * Wide{q1, 0.0});
+    const double q2 = r1.hi / b.hi;
+    const Wide r2 = r1 + -(b * Wide{q2, 0.0});
+    return normal(q1, q2) + Wide{r2.hi / b.hi, 0.0};
+}
+__device__ Wide power(Wide a, int n) {
+    Wide r = {1.0, 0.0};
+    for (; n; n >>= 1) {
+        if (n & 1) r = r * a;
+        a = a * a;
+    }
+    return r;
+}
+
+// One entry a lane: its frequency in turns a position, without the whole ones, in units of 2^-64. Within 2 of them for frequencies up to 2^30.
 __global__ __launch_bounds__(256) void rope_table_kernel(uint64_t *out, int half, int scaling, double base, double factor,
                                                          double low, double high, double trained) {
     const int i = threadIdx.x;
     if (i >= half) return;
-    constexpr double kTwoPi = 6.283185307179586476925286766559;
-    double f = pow(base, -(double)i / half); // radians a position
-    if (scaling == SPINN_ROPE_LINEAR) {
-        f /= factor;
-    } else if (scaling == SPINN_ROPE_BY_PARTS) {
-        const double r = trained * f / kTwoPi;
-        const double t = fmin(fmax((r - low) / (high - low), 0.0), 1.0);
-        f = t * f + (1.0 - t) * f / factor;
+    // f = base^(-i / half): two steps of Newton's method for f^half base^i = 1 from the library's power, which is off by up to 2^-46. Each
+    // squares the distance (times half); the powers' own roundings are 2^-95 of the equation's, 2^-95 / half of f. Exponents apart, so that
+    // nothing leaves the range.
+    int exp_b, exp_f;
+    const double mant_b = frexp(base, &exp_b);
+    Wide f = {pow(base, -(double)i / half), 0.0};
+    frexp(f.hi, &exp_f);
+    const Wide base_i = power({mant_b, 0.0}, i);
+    for (int step = 0; step < 2; ++step) {
+        const Wide p = power({ldexp(f.hi, -exp_f), ldexp(f.lo, -exp_f)}, half) * base_i;
+        const int e = exp_f * half + exp_b * i;
+        const Wide off = Wide{1.0, 0.0} + Wide{-ldexp(p.hi, e), -ldexp(p.lo, e)};
+        f = f + f * (off / Wide{(double)half, 0.0});
     }
-    double turns = f / kTwoPi;
-    turns -= floor(turns);
-    out[i] = (uint64_t)(turns * 18446744073709551616.0);
+    const Wide per_radian = {0x1.45f306dc9c883p-3, -0x1.6b01ec5417056p-57};
+    Wide turns = f * per_radian;
+    if (scaling == SPINN_ROPE_LINEAR) {
+        turns = turns / Wide{factor, 0.0};
+    } else if (scaling == SPINN_ROPE_BY_PARTS) {
+        const Wide t = (turns * Wide{trained, 0.0} + Wide{-low, 0.0}) / sum(high, -low);
+        const Wide stretched = turns / Wide{factor, 0.0};
+        if (t.hi <= 0.0) turns = stretched;
+        else if (t.hi < 1.0) turns = t * turns + (Wide{1.0, 0.0} + -t) * stretched;
+    }
+    constexpr double kUnits = 18446744073709551616.0; // 2^64
+    const double part = (turns.hi - floor(turns.hi)) * kUnits, rest = (turns.lo - rint(turns.lo)) * kUnits;
+    const double whole = floor(part);
+    out[i] = (uint64_t)whole + (uint64_t)(int64_t)rint(rest + (part - whole));
 }
 
 // mul and shift so that i / n = mulhi(i, mul) >> shift for all i < 2^31 (mul 0: i itself).
