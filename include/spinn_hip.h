@@ -451,6 +451,11 @@ int spinn_hip_beam_reorder(const SpinnHipBeamState *states, int n_states, int32_
  * lengths_out, next_out, held_out and free_count_out may each be its input itself; other arrays overlap nowhere. The rest
  * of page_table and free_pages stays as it was. Lengths and positions count as at least 0, held and *free_count
  * as 0 to max_pages and n_pages; seqs = 0 returns at once.
+ * Rows are packed: one that is idle or ended has none. spinn_hip_kv_attention reads row s for sequence s, so that it takes the rows of a
+ * step as they are only where every sequence has exactly one token and is served; spinn_hip_prompt_attention shows a token the keys of
+ * the same rows alone, so that it is for sequences that begin. A step that mixes them assigns in two calls, first to prompts and then to
+ * single tokens, and moves the latter's rows by spinn_hip_beam_reorder with batch = 1: row s = row starts[s] before attention,
+ * row t = row seq[t] behind it. Several tokens of a sequence that has others in its pages go one a step.
  */
 typedef struct {
     int32_t seqs;       /* 0..SPINN_HIP_ASSIGN_MAX_SEQS */
