@@ -459,7 +459,7 @@ int spinn_hip_beam_reorder(const SpinnHipBeamState *states, int n_states, int32_
  */
 typedef struct {
     int32_t seqs;       /* 0..SPINN_HIP_ASSIGN_MAX_SEQS */
-    int32_t page_size, n_pages, max_pages; /* as in SpinnHipKvDesc */
+    int32_t page_size, n_pages, max_pages; /* as in SpinnHipKvDesc; n_pages <= 2^29 */
     int32_t max_tokens; /* entries of seq, slot and position: 0..2^28 */
     int32_t reserved;   /* 0 */
 } SpinnHipKvAssignDesc;
@@ -486,6 +486,7 @@ enum {
  * the rest of a head is copied. Head h of token t is at x + t*x_stride + h*x_head_stride, y alike; y may be x itself (same strides),
  * else they overlap nowhere. Angles are exact to 2^-32 of a turn at any position (negative ones
  * turn back) for frequencies up to 2^30.
+ * tokens <= 2^28, heads * head_dim <= 2^30, strides from head_dim to 2^32.
  * The frequencies are laid out once by spinn_hip_rope_table (which reads rot_dim, scaling, base, factor, low, high and
  * trained alone), 16-byte aligned, and read from `table` afterwards.
  */
@@ -516,15 +517,18 @@ int spinn_hip_rope(const SpinnHipRopeDesc *d, int64_t tokens, const int32_t *pos
  *   o[i,h] = sum_j p_j v_j, p = softmax over the visible j of scale * q[i,h].k_j,
  * query head h reading kv head h / (heads / kv_heads). Of nk keys row i of nq sees all, or if `causal` those j <= i + nk - nq.
  * A row that sees none gives o = 0 and lse = -inf. Rows of a sequence's keys and values are finite.
+ * In 16-bit types the p_j enter the sum rounded to the type, half a step each, while what they are divided by and lse take them in fp32: o is off by up to
+ * that of sum_j p_j |v_j| and its own rounding (values that are all the same may come back a step off). spinn_hip_kv_attention
+ * keeps 22 bits and more of them, so that the two agree within this.
  * starts and kv_starts [seqs + 1] are on the device, ascend, and are cut to [0, q_rows] and [0, kv_rows]; rows of o
- * and lse outside every sequence stay as they were, and rows of k and v outside are not read.
+ * and lse outside every sequence stay as they were, and rows of k and v outside are not read. q_rows * heads and kv_rows are at most 2^30.
  * Rows of q and o hold heads * head_dim contiguous elements, those of k and v kv_heads * head_dim. lse [q_rows, heads]
  * fp32 (NULL = not wanted): log of the softmax's denominator. o overlaps no input.
  * Single tokens over a paged cache: spinn_hip_kv_attention.
  */
 typedef struct {
     int32_t dtype;
-    int32_t seqs;
+    int32_t seqs;            /* 0..2^24 */
     int32_t heads, kv_heads; /* heads: multiple of kv_heads */
     int32_t head_dim;        /* 1..SPINN_HIP_KV_MAX_DIM */
     int32_t causal;
@@ -543,7 +547,8 @@ int spinn_hip_prompt_attention(const SpinnHipPromptAttentionDesc *d, const void 
  * Rows to 8-bit integers with a scale each: scale[i] = max_j |x[i,j]| / 127 in fp32, xq[i,j] = x[i,j] / scale[i] rounded
  * to the nearest integer, ties to even (of the exact quotient; 0 where the scale is 0; within +-127). A row with a NaN or an
  * infinity gets scale NaN and zeros. Rows are ldx and ldq apart (up to 2^28); x needs its element's alignment, xq starts at a
- * multiple of 16, ldq is one and at least k; xq[i, k .. k rounded up to 16) is filled with zeros.
+ * multiple of 16, ldq is one and at least k; xq[i, k .. k rounded up to 16) is filled with zeros. A launch takes
+ * 2^26 - 4 rows up to k = 1024, 2^24 - 1 up to 4096, 2^22 - 1 beyond (more: SPINN_HIP_EUNSUPPORTED).
  */
 int spinn_hip_quantize_rows(int32_t dtype, int64_t rows, int32_t k, const void *x, int64_t ldx, int8_t *xq, int64_t ldq,
                             float *scale, void *stream);
@@ -553,7 +558,8 @@ int spinn_hip_quantize_rows(int32_t dtype, int64_t rows, int32_t k, const void *
  *   y[i,j] = act( x_scale[i] w_scale[j] sum_k x[i,k] w(j,k) + bias[j] + residual[i,j] ).
  * The sum is exact (32-bit integers, k <= SPINN_HIP_I8_MAX_K). w(j,k), bias, residual, y and the packed weights are as
  * there; dtype is that of bias, residual and y. Rows of x start at multiples of 16 bytes (ldx too, 0 = k rounded up to 16) and
- * hold k rounded up to 16 bytes that may be read; what is behind k does not count. y overlaps no input but the residual.
+ * hold k rounded up to 16 bytes that may be read; what is behind k does not count. y overlaps no input but the residual. Strides are up to 2^28.
+ * In fp32: (sum w_scale) x_scale, then bias and residual, each step rounded.
  */
 typedef struct {
     int32_t m, n, k;

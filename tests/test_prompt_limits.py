@@ -20,3 +20,20 @@ def test_scales(native, scale, taken):
     assert (L.spinn_hip_prompt_attention_workspace_size(C.byref(d)) > 0) == taken
     rc = L.spinn_hip_prompt_attention(C.byref(d), P, P, P, P, P, Q, None, None, 0, None)
     assert rc == (EWORKSPACE if taken else EINVAL)
+
+
+def test_rows_of_a_launch(native):
+    """One row more than spinn_hip_quantize_rows takes."""
+    L = native.lib()
+    for k, most in ((1, (1 << 26) - 4), (1024, (1 << 26) - 4), (1025, (1 << 24) - 1), (4096, (1 << 24) - 1), (4097, (1 << 22) - 1)):
+        ldq = (k + 15) // 16 * 16
+        assert L.spinn_hip_quantize_rows(1, most + 1, k, P, k, Q, ldq, P, None) == -2, (k, most)
+
+
+@pytest.mark.parametrize("change,taken", [({}, True), (dict(seqs=1 << 24), True), (dict(seqs=(1 << 24) + 1), False), (dict(kv_rows=1 << 30), True),
+                                          (dict(kv_rows=(1 << 30) + 1), False), (dict(q_stride=1 << 24), True), (dict(q_stride=(1 << 24) + 1), False),
+                                          (dict(q_stride=511), False), (dict(seqs=0, q_rows=1 << 27), True), (dict(seqs=0, q_rows=(1 << 27) + 1), False)], ids=str)
+def test_prompt_sizes(native, change, taken):
+    """A call without rows or sequences ends well where its descriptor is taken."""
+    d = prompt_desc(native, **{"q_rows": 0, **change})
+    assert native.lib().spinn_hip_prompt_attention(C.byref(d), P, P, P, P, P, Q, None, None, 0, None) == (0 if taken else EINVAL)
