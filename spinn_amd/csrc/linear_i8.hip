@@ -189,12 +189,20 @@ inline int64_t m_tiles(const SpinnHipLinearI8Desc *d) { return ((int64_t)d->m + 
 //  * 64 x 128 tiles: 5.5 + 0.2 f / splits, 6 more where K is split, 5.5 + 0.18 f a round from more than one per CU (200 x 1024 x 16384:
 //    54.6 whole, 34.1 in two, 22.6 in four, the stream kernel 24.8; 500 x 1024 x 1024: 8.2, stream 5.0);
 //  * 128 x 128 tiles: 5.5 + 0.23 f up to one per CU (150 x 14336 x 4096: 24.0, 64 x 128 27.5, stream 38.1); beyond, and for
-//    256 x 256 from one per CU, as the other types.
+//    256 x 256 from one per CU, as the other types;
+//  * up to 128 rows of so many columns that there are more 128 x 128 tiles than CUs (a vocabulary), where rounds of a grid tell nothing any more: up to
+//    16 rows the stream kernel on 1 x 2 blocks (1 x 128000 x 4096: 81, 1 x 1 87, 1 x 4 88, 64 x 128 tiles 87; 8 rows 84, 108, 93, 89), up to 64
+//    tiles of 64 x 128 (64 rows: 98, 128 x 128 101, 256 x 256 130, stream 137 at best; 17 rows 90, 92, 124, 99), then 128 x 128 (65 rows: 101, 64 x 128
+//    117, 256 x 256 129; 128 x 40000 x 8192: 88, 94, 98).
 Choice choose(const SpinnHipLinearI8Desc *d) {
     const int64_t cus = device_cu_count(), mt = m_tiles(d), nt = n_tiles(d), f = frags(d);
     auto grid = [&](int64_t rows, int64_t cols) { return ((mt + rows - 1) / rows) * ((nt + cols - 1) / cols); };
     auto rounds = [&](int64_t blocks) { return (blocks + cus - 1) / cus; };
-    if (grid(8, 8) > cus) return choose(mt, nt, f);
+    if (grid(8, 8) > cus) {
+        if (mt > 8) return choose(mt, nt, f);
+        if (mt == 1) return {Choice::kStream, 1, 2, 1};
+        return {mt <= 4 ? Choice::kTile64 : Choice::kTile128, 1, 1, 1};
+    }
     Choice c{Choice::kStream, 1, 1, 1};
     double least = 1e30;
     static const int blocks[][2] = {{1, 1}, {1, 2}, {1, 4}, {2, 2}, {2, 4}, {3, 2}, {3, 4}, {4, 2}, {4, 4}};
