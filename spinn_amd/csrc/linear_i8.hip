@@ -33,18 +33,24 @@ __device__ __forceinline__ void load_unit(const T *row, int u, int k, float (&v)
 }
 
 // v / s to the nearest integer, ties to even, decided by the remainder of a first guess: the remainder is exact
-// where it is near s / 2. tiny: s has few bits or none above fp32's least number, where a reciprocal would overflow.
-__device__ __forceinline__ int quantized(float v, float s, float inv, bool tiny) {
-    if (tiny) return s > 0.f ? (int)fmin(fmax(rint((double)v / (double)s), -127.0), 127.0) : 0;
+// where it is near s / 2.
+__device__ __forceinline__ int quantized(float v, float s, float inv) {
     float r = fminf(fmaxf(rintf(v * inv), -127.f), 127.f);
     const float d = fmaf(-r, s, v), far = fabsf(d), half = 0.5f * s;
     const int i = (int)r;
     return far > half || (far == half && (i & 1)) ? min(max(i + (d > 0.f ? 1 : -1), -127), 127) : i;
 }
 
-// A row per NW waves, 4 / NW (at least one) rows a workgroup; up to HOLD units of a lane stay in registers between the two passes.
+// The same where s has few bits or none above fp32's least number and a reciprocal would overflow.
+__device__ __forceinline__ int quantized_tiny(float v, float s) {
+    return s > 0.f ? (int)fmin(fmax(rint((double)v / (double)s), -127.0), 127.0) : 0;
+}
+
+// A row per NW waves, 4 / NW (at least one) rows a workgroup; a lane's first unit stays in registers between the two passes. Only rows of 16 waves have more.
 // 1 x 4096 bf16 is one workgroup's latency (4 us); many rows are bound by memory (4000 x 4096: 9.4 us behind the launch before it, 5.2 TB/s).
-template <class T, int NW, int HOLD>
+// From 4097 elements on k / 16 of a row's 1024 lanes work, up to 16384 (launches in a row: 4000 x 4096 14.2 us, 3.5 TB/s; x 5120 27.8, 2.2; x 8192
+// 29.9, 3.3; x 14336 44.0, 3.9).
+template <class T, int NW>
 __global__ __launch_bounds__(64 * (NW < 4 ? 4 : NW)) void quantize_rows_kernel(const T *__restrict__ x, int64_t ldx, int8_t *__restrict__ xq,
                                                                            int64_t ldq, float *__restrict__ scale, int64_t rows, int k) {
     constexpr int R = NW < 4 ? 4 / NW : 1;
@@ -53,22 +59,18 @@ __global__ __launch_bounds__(64 * (NW < 4 ? 4 : NW)) void quantize_rows_kernel(c
     const int first = (wave % NW) * 64 + lane, units = (int)(((int64_t)k + kUnit - 1) / kUnit);
     const bool in = row < rows;
     const T *xr = x + (in ? row : 0) * ldx;
-    float v[HOLD][kUnit];
+    float v[kUnit];
     uint32_t top = 0; // bits of the largest magnitude; infinities and NaN are above all numbers
     auto look = [&](const float (&w)[kUnit]) {
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) top = max(top, __builtin_bit_cast(uint32_t, w[i]) & 0x7fffffffu);
     };
-#pragma unroll
-    for (int h = 0; h < HOLD; ++h) {
-        const int u = first + h * 64 * NW;
-        if (in && u < units) {
-            load_unit<T>(xr, u, k, v[h]);
-            look(v[h]);
-        }
+    if (in && first < units) {
+        load_unit<T>(xr, first, k, v);
+        look(v);
     }
-    if (in)
-        for (int u = first + HOLD * 64 * NW; u < units; u += 64 * NW) {
+    if (NW == 16 && in)
+        for (int u = first + 64 * NW; u < units; u += 64 * NW) {
             float w[kUnit];
             load_unit<T>(xr, u, k, w);
             look(w);
@@ -87,36 +89,35 @@ __global__ __launch_bounds__(64 * (NW < 4 ? 4 : NW)) void quantize_rows_kernel(c
     const bool bad = top >= 0x7f800000u;
     const float most = __builtin_bit_cast(float, top);
     const float s = bad ? __builtin_bit_cast(float, 0x7fc00000u) : most / 127.f;
-    const bool tiny = top < 0x0d800000u; // 2^-100
     const float inv = 1.f / s;
     if (first == 0) scale[row] = s;
     int8_t *out = xq + row * ldq;
     auto store = [&](int u, const float (&w)[kUnit]) {
         u32x4 b = {0, 0, 0, 0};
-        if (!bad) {
+        if (top < 0x0d800000u) { // 2^-100
 #pragma unroll
-            for (int i = 0; i < kUnit; ++i) b[i / 4] |= (uint32_t)(uint8_t)quantized(w[i], s, inv, tiny) << (8 * (i % 4));
+            for (int i = 0; i < kUnit; ++i) b[i / 4] |= (uint32_t)(uint8_t)quantized_tiny(w[i], s) << (8 * (i % 4));
+        } else if (!bad) {
+#pragma unroll
+            for (int i = 0; i < kUnit; ++i) b[i / 4] |= (uint32_t)(uint8_t)quantized(w[i], s, inv) << (8 * (i % 4));
         }
         *reinterpret_cast<u32x4 *>(out + (int64_t)u * kUnit) = b;
     };
-#pragma unroll
-    for (int h = 0; h < HOLD; ++h) {
-        const int u = first + h * 64 * NW;
-        if (u < units) store(u, v[h]);
-    }
-    for (int u = first + HOLD * 64 * NW; u < units; u += 64 * NW) {
-        float w[kUnit];
-        load_unit<T>(xr, u, k, w);
-        store(u, w);
-    }
+    if (first < units) store(first, v);
+    if (NW == 16)
+        for (int u = first + 64 * NW; u < units; u += 64 * NW) {
+            float w[kUnit];
+            load_unit<T>(xr, u, k, w);
+            store(u, w);
+        }
 }
 
-template <class T, int NW, int HOLD>
+template <class T, int NW>
 int launch_quantize(int64_t rows, int k, const void *x, int64_t ldx, int8_t *xq, int64_t ldq, float *scale, hipStream_t st) {
     constexpr int R = NW < 4 ? 4 / NW : 1, threads = 64 * (NW < 4 ? 4 : NW);
     const int64_t grid = (rows + R - 1) / R;
     if (!launch_fits(grid, threads)) return SPINN_HIP_EUNSUPPORTED;
-    quantize_rows_kernel<T, NW, HOLD><<<(unsigned)grid, threads, 0, st>>>((const T *)x, ldx, xq, ldq, scale, rows, k);
+    quantize_rows_kernel<T, NW><<<(unsigned)grid, threads, 0, st>>>((const T *)x, ldx, xq, ldq, scale, rows, k);
     return check_launch();
 }
 
@@ -231,9 +232,9 @@ Choice choose(const SpinnHipLinearI8Desc *d) {
 int quantize_rows(int dtype, int64_t rows, int k, const void *x, int64_t ldx, int8_t *xq, int64_t ldq, float *scale, hipStream_t st) {
     return with_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
-        if (k <= 1024) return launch_quantize<T, 1, 1>(rows, k, x, ldx, xq, ldq, scale, st);
-        if (k <= 4096) return launch_quantize<T, 4, 1>(rows, k, x, ldx, xq, ldq, scale, st);
-        return launch_quantize<T, 16, 1>(rows, k, x, ldx, xq, ldq, scale, st);
+        if (k <= 1024) return launch_quantize<T, 1>(rows, k, x, ldx, xq, ldq, scale, st);
+        if (k <= 4096) return launch_quantize<T, 4>(rows, k, x, ldx, xq, ldq, scale, st);
+        return launch_quantize<T, 16>(rows, k, x, ldx, xq, ldq, scale, st);
     });
 }
 
