@@ -182,7 +182,7 @@ __device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) l
 
 // Workgroups on a CU, as registers and LDS allow.
 template <class T, int DP, bool RUNS>
-constexpr int kBlocks = sizeof(T) == 4 ? (DP <= 64 ? 4 + RUNS : DP <= 96 ? 4 + RUNS : DP == 128 ? 3 + RUNS : 2) : DP <= 128 ? (DP == 96 && RUNS ? 3 : 2) : 1;
+constexpr int kAtOnce = sizeof(T) == 4 ? (DP <= 96 ? 4 + RUNS : DP == 128 ? 3 + RUNS : 2) : DP <= 128 ? (DP == 96 && RUNS ? 3 : 2) : 1;
 
 // What a matrix product has just left in s may be read. The compiler counts the wait that is due along one way into a block only
 // (16 x 16 x 4 fp32: 10 instructions by the masked way, 1 by the other, where it put none), so it is written out here.
@@ -197,7 +197,7 @@ __device__ __forceinline__ void settle(Acc (&s)[B]) {
 // T: element; DP: head_dim padded to whole matrix operands; KB: keys of a tile;
 // RUNS: rows of q, k and v are whole, aligned 16-byte runs.
 template <class T, int DP, int KB, bool RUNS>
-__global__ __launch_bounds__(256, (kBlocks<T, DP, RUNS>)) void prompt_kernel(PromptArgs a) {
+__global__ __launch_bounds__(256, (kAtOnce<T, DP, RUNS>)) void prompt_kernel(PromptArgs a) {
     typedef Tile<T, DP> Lay;
     constexpr int R = kWaveRows<T>, G = 64 / R, kRows = ::spinn::kRows<T>; // G: lanes of a row
     typedef float Acc __attribute__((ext_vector_type(R * R / 64)));
@@ -608,7 +608,7 @@ template <class T, int DP, int KB>
 int launch(PromptArgs &a, const Cut &c, bool runs, hipStream_t st) {
     const int64_t grid = c.items * a.kv_heads * c.splits;
     if (!launch_fits(grid, 256)) return SPINN_HIP_EUNSUPPORTED;
-    a.at_once = grid <= (runs ? kBlocks<T, DP, true> : kBlocks<T, DP, false>) * device_cu_count();
+    a.at_once = grid <= (runs ? kAtOnce<T, DP, true> : kAtOnce<T, DP, false>) * device_cu_count();
     if (runs) prompt_kernel<T, DP, KB, true><<<(unsigned)grid, 256, 0, st>>>(a);
     else prompt_kernel<T, DP, KB, false><<<(unsigned)grid, 256, 0, st>>>(a);
     if (c.splits > 1) prompt_join_kernel<T><<<(unsigned)(c.items * a.kv_heads * (c.rows / 4)), 256, 0, st>>>(a, DP);
