@@ -40,7 +40,6 @@ HIP_FLAGS = [
     "-std=c++17",
     # packed-fp32 instructions stay off: the compiler may not form them
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    "-Wno-inline-asm",  # m0 among what a statement changes is meant
     f"-I{INCLUDE}",
 ]
 C_FLAGS = ["-O2", "-fPIC", "-std=gnu11", "-Wall", "-Wextra", "-Wno-unused-parameter", f"-I{INCLUDE}"]

@@ -169,6 +169,8 @@ __device__ __forceinline__ float across(float v, F f) {
 // 16 bytes a lane from base + off to byte `to` + 16 lane of LDS; all_ready() waits for it. In assembly, since the compiler would wait for all
 // of these before every transposing read of LDS that follows, whatever it reads (16000 rows, before other steps: 2020 -> 1916 us).
 // lanes: -1 all of those that are here, 0 none, without a branch.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // m0 among what the statement changes is meant
 __device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32_t to, int lanes = -1) {
     uint64_t here;
     asm volatile("s_mov_b32 m0, %1\n\ts_and_saveexec_b64 %0, %4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
@@ -176,6 +178,7 @@ __device__ __forceinline__ void async_run(const char *base, uint32_t off, uint32
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(base), "s"((int64_t)__builtin_amdgcn_readfirstlane(lanes))
                  : "memory", "m0", "scc");
 }
+#pragma clang diagnostic pop
 
 // This wave's copies have landed and its LDS reads are done, and so are every other wave's.
 __device__ __forceinline__ void all_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
