@@ -516,7 +516,8 @@ int spinn_hip_rope(const SpinnHipRopeDesc *d, int64_t tokens, const int32_t *pos
  * kv_starts[s] .. of k and v (kv_starts = NULL: the same):
  *   o[i,h] = sum_j p_j v_j, p = softmax over the visible j of scale * q[i,h].k_j,
  * query head h reading kv head h / (heads / kv_heads). Of nk keys row i of nq sees all, or if `causal` those j <= i + nk - nq.
- * A row that sees none gives o = 0 and lse = -inf. Rows of a sequence's keys and values are finite.
+ * A row that sees none gives o = 0 and lse = -inf. Rows of a sequence's keys and values are finite, and so are their scores and sums in fp32, where a
+ * weight is up to 2^8 before the quotient (fp16 2^15): up to |v| of 2^119 / nk.
  * In 16-bit types the p_j enter the sum rounded to the type, half a step each, while what they are divided by and lse take them in fp32: o is off by up to
  * that of sum_j p_j |v_j| and its own rounding (values that are all the same may come back a step off). spinn_hip_kv_attention
  * keeps 22 bits and more of them, so that the two agree within this.
