@@ -4,8 +4,8 @@
 // needed; then the pages' numbers are copied between the stack of free ones and the rows of the table, and each token
 // finds its sequence by a search among the starts. Nothing here has work to speak of: dependent steps bound it. The
 // sums are one workgroup's, 1024 sequences at a time; few tokens are placed by it, too, in the same launch, many by a
-// second one, which needs all the starts. 64 sequences of one token: a launch (7.6 us a call); 500, of which 50 bring prompts of
-// up to 8000 tokens and 25 end: 22 us, 5 of them the second launch's.
+// second one, which needs all the starts. 64 sequences of one token: a launch (7.2 us a call); 500, of which 50 bring prompts of
+// up to 8000 tokens and 25 end: 22.8 us, 5 of them the second launch's.
 #include "decode.h"
 
 namespace spinn {

@@ -10,7 +10,7 @@
 // out of LDS transposed by the read itself (16-bit types) or by whole runs of a row (fp32).
 //
 // 16-bit types: 128 rows a workgroup, tiles of 64 keys, 32 x 32 instructions, two workgroups a CU (heads of 128). 16000 rows, 32 heads on 8
-// of 128, bf16, causal: 1830 to 2040 us by the card, up to 1150 TFLOP/s, bound by power (1400 us on zeros); 24 sequences of 37 to 2000 rows: 326 to 336 us.
+// of 128, bf16, causal: 1830 to 2040 us by the card, up to 1150 TFLOP/s, bound by power (1400 us on zeros); 24 sequences of 37 to 2000 rows: 326 to 342 us.
 // fp32: 64 rows, tiles of 16 keys, 16 x 16 instructions at the same rate: less padding (80 columns are five blocks) and small
 // enough for five workgroups a CU. 8 x 577 rows, 16 heads of 80: 127 us, 107 TFLOP/s (32 x 32 instructions, 128 rows: 179); 4 x 2000 of 128
 // 618 (670); 2 x 1000, 8 heads on 2 of 256: 141 (277).

@@ -4,7 +4,7 @@
 // so a workgroup computes those of its tokens once into LDS and then walks over the heads in 16-byte
 // runs. Angles: a frequency is kept as a fraction of a turn in 64-bit fixed point, right to its last two units, whose product with the position,
 // modulo 2^64, is the angle without its whole turns, to 2^-32: positions in the thousands of millions are as good as the first.
-// 16384 x 40 heads of 128, bf16: 62 to 66 us, 5.1 to 5.4 TB/s; 5001 x 17 heads, 32 of 80, interleaved, fp32: 10.5 us, 5.2 TB/s; 32 x 20 heads of
+// 16384 x 40 heads of 128, bf16: 62 to 67 us, 5.0 to 5.4 TB/s; 5001 x 17 heads, 32 of 80, interleaved, fp32: 10.5 us, 5.2 TB/s; 32 x 20 heads of
 // 128: 6.8 us a call, a launch.
 #include "decode.h"
 
